@@ -324,6 +324,7 @@ def lm_head_shard_records(
                                                       vocab_offset, total_vocab, round_bf16)
 
 
+from cid_engine.head import lm_head_cross_entropy  # noqa: E402
 from cid_engine.step import refine_step, refine_step_from_hidden  # noqa: E402
 from cid_engine.loop import DisplayRefineLoop  # noqa: E402
 
@@ -340,6 +341,7 @@ __all__ = [
     "display_token_statistics",
     "display_token_statistics_with_repetition",
     "live_slot_occupancy",
+    "lm_head_cross_entropy",
     "lm_head_display_statistics",
     "lm_head_shard_records",
     "materialize_cell_snapshot",

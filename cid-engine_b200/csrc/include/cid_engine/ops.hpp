@@ -114,6 +114,19 @@ at::Tensor lm_head_shard_records(Backend backend, const at::Tensor& token_ids,
                                  std::int64_t vocab_offset, std::int64_t total_vocab,
                                  bool round_bf16);
 
+// Softmax cross entropy of labels over hidden @ weight^T without writing the
+// logits (additive): (loss, log_sum_exp), f32 of the labels' shape.
+std::tuple<at::Tensor, at::Tensor> lm_head_cross_entropy(Backend backend, const at::Tensor& labels,
+                                                         const at::Tensor& hidden,
+                                                         const at::Tensor& weight,
+                                                         std::int64_t ignore_index);
+// Its gradients of hidden and weight; an output that is not wanted is empty.
+std::tuple<at::Tensor, at::Tensor> lm_head_cross_entropy_backward(
+    Backend backend, const std::optional<at::Tensor>& grad_loss,
+    const std::optional<at::Tensor>& grad_log_sum_exp, const at::Tensor& labels,
+    const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& log_sum_exp,
+    std::int64_t ignore_index, bool need_hidden, bool need_weight);
+
 // Device status word (CID_STATUS_* bits) of `device`; read() synchronises.
 std::int64_t read_device_status(std::int64_t device, bool reset);
 

@@ -1,0 +1,971 @@
+// Softmax cross entropy of an LM head, without keeping the logits, and its
+// gradient.  For rows h_r (16-bit, H wide), weight rows w_v and labels y_r:
+//
+//   z_rv = h_r . w_v            (f32 accumulation on the tensor cores)
+//   lse_r = log sum_v exp z_rv,  loss_r = lse_r - z_{r, y_r}
+//   d_rv = a_r exp(z_rv - lse_r) - b_r [v = y_r],   a = g_loss + g_lse, b = g_loss
+//   dh = d W,   dW = d^T h
+//
+// Rows whose label is ignore_index take no part: a prepare kernel packs the
+// other rows (count n, left on the device), the products run over n rows only,
+// and nothing of an ignored row's hidden state is read, so NaN there reaches
+// nothing.  The n rows keep their order, and every sum has a fixed order:
+// repeated calls give identical bits.
+//
+// The backward goes over the vocabulary in pieces: a piece's logits are
+// computed again, turned into d (16 bits) in a workspace that stays in L2, and
+// multiplied with the weight (dh, summed in f32 over the pieces) and the
+// hidden rows (that piece's rows of dW).  8 n V H flops a step (2 forward, 2
+// again, 4 gradients) instead of 6 with kept logits, which would be n V floats.
+//
+// Roundings to 16 bits: d, because the tensor cores take 16-bit operands (the
+// same step as a 16-bit gradient of the logits; at most half a step of each
+// element, and the elements' errors are independent), and the outputs.  fp16 d
+// is scaled by a power of two from the largest coefficient, so that neither a
+// loss scale nor a division by the number of rows leaves fp16's range.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <climits>
+#include <cmath>
+#include <type_traits>
+
+#include "common.cuh"
+#include "tcgen05.cuh"
+
+namespace cid {
+namespace {
+
+constexpr int kBM = 128;  // rows of an output tile
+constexpr int kBN = 256;  // columns of an output tile
+constexpr int kBK = 64;   // K elements a stage: one 128-byte swizzle row
+constexpr int kUmmaK = 16;
+constexpr int kStages = 4;
+constexpr int kAccBufs = 2;
+constexpr uint32_t kTmemCols = kAccBufs * kBN;
+constexpr uint32_t kStageA = kBM * kBK * 2;
+constexpr uint32_t kStageB = kBN * kBK * 2;
+constexpr uint32_t kStageBytes = kStageA + kStageB;
+constexpr uint32_t kBlockBytes = 64 * kBK * 2;  // one 64 x 64 block of an MN-major operand
+constexpr size_t kSmemBytes = kStages * size_t{kStageBytes} + 1024 + 256;
+constexpr int kThreads = 192;  // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
+constexpr int kRowGroup = 32;  // row blocks that share weight tiles in L2
+constexpr int kPrepRows = 8;   // rows a prepare block packs, one a warp
+constexpr int kMaxSplits = 64;
+// Units the split of dh aims at: with four waves of 148 SMs the last wave
+// costs little, and the partial tiles stay within 75 MB.
+constexpr int64_t kSplitUnits = 592;
+
+enum Mode {
+  kLoss,     // A = hidden rows, B = weight rows: (max, sum of exp) a row and tile, label logits
+  kDlogits,  // the same product: d, 16 bits
+  kDhidden,  // A = d, B = weight (K = vocabulary, N contiguous): partial sums of dh
+  kDweight   // A = d^T, B = hidden (K = rows, both with M / N contiguous): dW
+};
+
+struct Params {
+  const int* count;     // [0] kept rows, [2] K splits of dh
+  int64_t hidden;       // H
+  int64_t cols;         // vocabulary columns of this piece
+  int64_t col0;         // first of them
+  int64_t pitch;        // elements between rows of d
+  const int* labels;    // packed rows: label, lse, coefficients
+  const float* lse;
+  const float* ca;
+  const float* cb;
+  const uint32_t* top;  // bits of the largest |coefficient| (fp16), or NULL
+  float2* records;      // [tiles][rec_stride]
+  float* label_logit;   // [rec_stride]
+  int64_t rec_stride;
+  void* d;              // kDlogits output
+  void* grad_weight;    // kDweight output
+  float* partial;       // kDhidden output: [split][tile] blocks of kBM x kBN floats
+  int accumulate;       // add to the partial sums of the pieces before
+  uint32_t* status;
+};
+
+// Power of two that brings the largest coefficient near 2^11 (fp16 d).
+__device__ __forceinline__ float coef_scale(const uint32_t* top) {
+  if (top == nullptr) return 1.0f;
+  const float m = __uint_as_float(*top);
+  if (!(m > 0.0f) || !(m < INFINITY)) return 1.0f;
+  int e = 12 - ilogbf(m);
+  e = e > 120 ? 120 : (e < -120 ? -120 : e);
+  return __int_as_float((e + 127) << 23);
+}
+
+// The unit grid of one launch, the same for every role of the kernel.
+struct Grid {
+  int64_t mt, nt, splits, units, kslices;
+};
+
+// K splits of dh: the number that makes the slowest SM's share of slices
+// smallest.  A unit costs its slices and about kUnitCost slices of epilogue.
+// The count is fixed by a whole piece's slices, so that every piece adds to the
+// same partial tiles.
+__device__ inline int dh_splits(int64_t tiles, int kslices, int sms) {
+  constexpr int kUnitCost = 8;
+  int best = 1;
+  int64_t best_cost = INT64_MAX;
+  for (int s = 1; s <= kMaxSplits; ++s) {
+    if (s > 1 && (tiles * s > kSplitUnits || s * 8 > kslices)) break;
+    const int64_t waves = (tiles * s + sms - 1) / sms;
+    const int64_t cost = waves * ((kslices + s - 1) / s + kUnitCost);
+    if (cost < best_cost) {
+      best_cost = cost;
+      best = s;
+    }
+  }
+  return best;
+}
+
+__device__ __forceinline__ Grid make_grid(Mode mode, const Params& p, int n) {
+  Grid g;
+  const int64_t rows = n > 0 ? n : 1;  // one block of zero rows writes zero gradients
+  if (mode == kLoss || mode == kDlogits) {
+    g.mt = (rows + kBM - 1) / kBM;
+    g.nt = (p.cols + kBN - 1) / kBN;
+    g.kslices = (p.hidden + kBK - 1) / kBK;
+    g.splits = 1;
+  } else if (mode == kDhidden) {
+    g.mt = (rows + kBM - 1) / kBM;
+    g.nt = (p.hidden + kBN - 1) / kBN;
+    g.kslices = (p.cols + kBK - 1) / kBK;
+    g.splits = p.count[2];
+  } else {
+    g.mt = (p.cols + kBM - 1) / kBM;
+    g.nt = (p.hidden + kBN - 1) / kBN;
+    g.kslices = (rows + kBK - 1) / kBK;
+    g.splits = 1;
+  }
+  g.units = g.mt * g.nt * g.splits;
+  return g;
+}
+
+struct Unit {
+  int64_t m, n, split, k0, k1;  // tile coordinates, K slices [k0, k1)
+};
+
+__device__ __forceinline__ Unit unit_at(Mode mode, const Grid& g, int64_t u) {
+  Unit x;
+  if (mode == kLoss || mode == kDlogits) {
+    // groups of kRowGroup row blocks; inside one, the row blocks of a weight
+    // tile run next to each other
+    const int64_t per = kRowGroup * g.nt;
+    const int64_t gi = u / per, first = gi * kRowGroup;
+    const int64_t in = g.mt - first < kRowGroup ? g.mt - first : kRowGroup;
+    const int64_t local = u - gi * per;
+    x.m = first + local % in;
+    x.n = local / in;
+    x.split = 0;
+  } else {
+    const int64_t tiles = g.mt * g.nt;
+    x.split = u / tiles;
+    const int64_t t = u - x.split * tiles;
+    x.m = t / g.nt;
+    x.n = t - x.m * g.nt;
+  }
+  const int64_t each = (g.kslices + g.splits - 1) / g.splits;
+  x.k0 = x.split * each;
+  x.k1 = x.k0 + each < g.kslices ? x.k0 + each : g.kslices;
+  if (x.k1 < x.k0) x.k1 = x.k0;
+  return x;
+}
+
+// Shared-memory descriptor of an MN-major operand in 64 x 64 blocks, each 64 K
+// rows of 128 bytes (64 M or N elements) in the 128-byte swizzle: 8-row atoms
+// 1024 bytes apart along K (stride byte offset), blocks kBlockBytes apart along
+// M or N (leading byte offset).
+__device__ __forceinline__ uint64_t mn_desc(uint32_t addr) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3fffu) |
+         (static_cast<uint64_t>(kBlockBytes >> 4) << 16) | (uint64_t{1024 >> 4} << 32) |
+         (uint64_t{1} << 46) | (uint64_t{2} << 61);
+}
+
+// Operands with M / N contiguous in memory (the others have K contiguous).
+template <Mode kMode>
+constexpr bool kAMn = kMode == kDweight;
+template <Mode kMode>
+constexpr bool kBMn = kMode == kDweight || kMode == kDhidden;
+
+// Instruction descriptor of kind::f16: D f32, A and B of type T (0 fp16, 1
+// bf16), bit 15 / 16: A / B with M / N contiguous, N >> 3 at 17, M >> 4 at 24.
+template <typename T, Mode kMode>
+__device__ __forceinline__ uint32_t idesc() {
+  constexpr uint32_t t = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  return (1u << 4) | (t << 7) | (t << 10) | ((kAMn<kMode> ? 1u : 0u) << 15) |
+         ((kBMn<kMode> ? 1u : 0u) << 16) | (uint32_t(kBN >> 3) << 17) |
+         (uint32_t(kBM >> 4) << 24);
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t r;
+  if (std::is_same<T, __nv_bfloat16>::value)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// 32 consecutive values of a row of 16-bit elements, columns c0.. of `width`
+// (a multiple of 8), 16-byte aligned.
+template <typename T>
+__device__ __forceinline__ void store32(T* row, int64_t c0, int64_t width, const float (&x)[32]) {
+#pragma unroll
+  for (int j = 0; j < 32; j += 8) {
+    if (c0 + j < width) {
+      uint4 v;
+      v.x = pack2<T>(x[j], x[j + 1]);
+      v.y = pack2<T>(x[j + 2], x[j + 3]);
+      v.z = pack2<T>(x[j + 4], x[j + 5]);
+      v.w = pack2<T>(x[j + 6], x[j + 7]);
+      *reinterpret_cast<uint4*>(row + c0 + j) = v;
+    }
+  }
+}
+
+struct EpiRow {
+  int64_t row;     // row of the output tile's matrix
+  bool valid;
+  int label;
+  float m, s;      // running maximum and sum of exp (kLoss)
+  float lse2, a, b;  // lse in base-2 exponent units, coefficients (kDlogits)
+};
+
+// ---------------------------------------------------------------------------
+// The product kernel: one persistent CTA per SM, warp-specialised
+// ---------------------------------------------------------------------------
+
+template <typename T, Mode kMode>
+__global__ void __launch_bounds__(kThreads, 1)
+    head_gemm_kernel(const __grid_constant__ CUtensorMap map_a,
+                     const __grid_constant__ CUtensorMap map_b, Params p) {
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  unsigned char* smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
+  unsigned char* stage_a = smem;
+  unsigned char* stage_b = smem + kStages * kStageA;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * kStageBytes);
+  uint64_t* empty = full + kStages;
+  uint64_t* acc_full = empty + kStages;
+  uint64_t* acc_empty = acc_full + kAccBufs;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + kAccBufs);
+  volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < kAccBufs; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 4);
+    }
+    *abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_slot)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const int n = *p.count;
+  const Grid g = make_grid(kMode, p, n);
+  const int64_t ksteps = (n > 0 ? n + kUmmaK - 1 : kUmmaK) / kUmmaK;  // of kDweight
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ---------------- TMA producer ----------------
+      int s = 0;
+      uint32_t ph = 0, issued = 0, issue_par = 0;
+      bool ok = true;
+      for (int64_t u = blockIdx.x; ok && u < g.units; u += gridDim.x) {
+        const Unit x = unit_at(kMode, g, u);
+        for (int64_t k = x.k0; k < x.k1; ++k) {
+          if (!mbar_wait(&empty[s], ph ^ 1u, abort, kWaitNs)) {
+            if (!*abort) raise_abort(abort, p.status);
+            ok = false;
+            break;
+          }
+          mbar_expect_tx(&full[s], kStageBytes);
+          unsigned char* a = stage_a + s * kStageA;
+          unsigned char* b = stage_b + s * kStageB;
+          const int32_t kx = static_cast<int32_t>(k * kBK);
+          if (kMode == kDweight) {
+            for (int i = 0; i < kBM / 64; ++i)
+              tma_load_2d(a + i * kBlockBytes, &map_a, static_cast<int32_t>(x.m * kBM + i * 64),
+                          kx, &full[s]);
+          } else {
+            tma_load_2d(a, &map_a, kx, static_cast<int32_t>(x.m * kBM), &full[s]);
+          }
+          if (kBMn<kMode>) {
+            const int32_t row = kx + (kMode == kDhidden ? static_cast<int32_t>(p.col0) : 0);
+            for (int i = 0; i < kBN / 64; ++i)
+              tma_load_2d(b + i * kBlockBytes, &map_b, static_cast<int32_t>(x.n * kBN + i * 64),
+                          row, &full[s]);
+          } else {
+            tma_load_2d(b, &map_b, kx, static_cast<int32_t>(p.col0 + x.n * kBN), &full[s]);
+          }
+          issued |= 1u << s;
+          issue_par = (issue_par & ~(1u << s)) | (ph << s);
+          if (++s == kStages) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+      // copies in flight land before the CTA exits (immediate unless aborted)
+      for (int i = 0; i < kStages; ++i)
+        if (issued & (1u << i)) mbar_wait(&full[i], (issue_par >> i) & 1u, nullptr, kDrainNs);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      // ---------------- MMA issuer ----------------
+      int s = 0, buf = 0;
+      uint32_t ph = 0, aph = 0;
+      uint64_t* last_bar = nullptr;
+      uint32_t last_par = 0;
+      bool ok = true;
+      for (int64_t u = blockIdx.x; ok && u < g.units; u += gridDim.x) {
+        const Unit x = unit_at(kMode, g, u);
+        if (!mbar_wait(&acc_empty[buf], aph ^ 1u, abort, kWaitNs)) {
+          if (!*abort) raise_abort(abort, p.status);
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem_base + static_cast<uint32_t>(buf * kBN);
+        for (int64_t k = x.k0; k < x.k1; ++k) {
+          if (!mbar_wait(&full[s], ph, abort, kWaitNs)) {
+            if (!*abort) raise_abort(abort, p.status);
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a0 = smem_u32(stage_a + s * kStageA);
+          const uint32_t b0 = smem_u32(stage_b + s * kStageB);
+          // rows past the last step of kDweight are not zero: they are not multiplied
+          const int64_t left = kMode == kDweight ? ksteps - k * (kBK / kUmmaK) : kBK / kUmmaK;
+#pragma unroll
+          for (int kk = 0; kk < kBK / kUmmaK; ++kk) {
+            if (kk >= left) break;
+            // K advance: 32 bytes inside a K-major row, two 8-row atoms otherwise
+            const uint64_t ad =
+                kAMn<kMode> ? mn_desc(a0 + kk * 2048) : sw128_desc(a0 + kk * 32);
+            const uint64_t bd =
+                kBMn<kMode> ? mn_desc(b0 + kk * 2048) : sw128_desc(b0 + kk * 32);
+            umma_f16(d, ad, bd, idesc<T, kMode>(), (k > x.k0 || kk > 0) ? 1u : 0u);
+          }
+          umma_commit(&empty[s]);
+          last_bar = &empty[s];
+          last_par = ph;
+          if (++s == kStages) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+        if (!ok) break;
+        umma_commit(&acc_full[buf]);
+        last_bar = &acc_full[buf];
+        last_par = aph;
+        if (++buf == kAccBufs) {
+          buf = 0;
+          aph ^= 1u;
+        }
+      }
+      // MMAs in flight finish before the TMEM is freed (immediate unless aborted)
+      if (last_bar != nullptr) mbar_wait(last_bar, last_par, nullptr, kDrainNs);
+    }
+  } else {
+    // ---------------- epilogue: thread = tile row, TMEM lane = tile row ----------------
+    const int quarter = warp & 3;
+    const int r = quarter * 32 + lane;
+    const float scale = coef_scale(p.top);
+    int buf = 0;
+    uint32_t aph = 0;
+    for (int64_t u = blockIdx.x; u < g.units; u += gridDim.x) {
+      const Unit x = unit_at(kMode, g, u);
+      EpiRow e{};
+      e.row = x.m * kBM + r;
+      e.valid = e.row < (kMode == kDweight ? p.cols : n);
+      e.label = -1;
+      e.m = -INFINITY;
+      if ((kMode == kLoss || kMode == kDlogits) && e.valid) {
+        e.label = p.labels[e.row];
+        if (kMode == kDlogits) {
+          e.lse2 = p.lse[e.row] * kLog2e;
+          e.a = p.ca[e.row] * scale;
+          e.b = p.cb[e.row] * scale;
+        }
+      }
+      bool got = mbar_wait(&acc_full[buf], aph, abort, kWaitNs);
+      got = __all_sync(0xffffffffu, got);
+      if (!got) {
+        if (lane == 0 && !*abort) raise_abort(abort, p.status);
+        break;
+      }
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
+                             static_cast<uint32_t>(buf * kBN);
+      float* part = nullptr;
+      if (kMode == kDhidden)
+        part = p.partial + ((x.split * g.mt + x.m) * g.nt + x.n) * (kBM * kBN) + r * kBN;
+#pragma unroll 1
+      for (int c = 0; c < kBN; c += 32) {
+        const int64_t c0 = x.n * kBN + c;  // column of the output tile's matrix
+        const int64_t width = kMode == kLoss || kMode == kDlogits ? p.cols : p.hidden;
+        if (c0 >= width && kMode != kDlogits) break;
+        uint32_t t[32];
+        tmem_issue32(taddr + static_cast<uint32_t>(c), t);
+        tmem_wait32(t);
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(t[j]);
+        if (kMode == kDhidden && x.k0 == x.k1) {  // a split without K slices: no product
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+        }
+        if (kMode == kLoss) {
+          if (c0 + 32 > width) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (c0 + j >= width) v[j] = -INFINITY;
+          }
+          const int64_t rel = e.label - p.col0 - c0;
+          if (rel >= 0 && rel < 32) {
+            float at = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j == rel) at = v[j];
+            p.label_logit[e.row] = at;
+          }
+          float cm = v[0];
+#pragma unroll
+          for (int j = 1; j < 32; ++j) cm = fmaxf(cm, v[j]);
+          if (cm > e.m) {
+            e.s = e.m == -INFINITY ? (e.s != e.s ? e.s : 0.0f) : e.s * ex2((e.m - cm) * kLog2e);
+            e.m = cm;
+          }
+          // a chunk of -inf alone adds nothing; NaN and +inf make the sum NaN
+          const float off = e.m == -INFINITY ? 0.0f : -e.m * kLog2e;
+          float a0 = 0.0f, a1 = 0.0f, b0 = 0.0f, b1 = 0.0f;
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            float x0, x1, x2, x3;
+            fma2(x0, x1, v[j], v[j + 1], kLog2e, off);
+            fma2(x2, x3, v[j + 2], v[j + 3], kLog2e, off);
+            add2(a0, a1, ex2(x0), ex2(x1));
+            add2(b0, b1, ex2(x2), ex2(x3));
+          }
+          e.s += (a0 + a1) + (b0 + b1);
+        } else if (kMode == kDlogits) {
+          const int64_t rel = e.label - p.col0 - c0;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            float q = e.a * ex2(fmaf(v[j], kLog2e, -e.lse2));
+            if (j == rel) q -= e.b;
+            v[j] = e.valid && c0 + j < width ? q : 0.0f;
+          }
+          store32<T>(static_cast<T*>(p.d) + e.row * p.pitch, c0, p.pitch, v);
+        } else if (kMode == kDhidden) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            float4 o = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+            float4* q = reinterpret_cast<float4*>(part + c + j);
+            if (p.accumulate) {
+              const float4 w = *q;
+              o.x += w.x;
+              o.y += w.y;
+              o.z += w.z;
+              o.w += w.w;
+            }
+            *q = o;
+          }
+        } else if (e.valid) {
+          const float inv = 1.0f / scale;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] *= inv;
+          store32<T>(static_cast<T*>(p.grad_weight) + (p.col0 + e.row) * p.hidden, c0, p.hidden,
+                     v);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty[buf]);
+      if (++buf == kAccBufs) {
+        buf = 0;
+        aph ^= 1u;
+      }
+      if (kMode == kLoss && e.valid)
+        p.records[x.n * p.rec_stride + e.row] = make_float2(e.m, e.s);
+    }
+  }
+
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base),
+                 "r"(kTmemCols)
+                 : "memory");
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Packing the kept rows
+// ---------------------------------------------------------------------------
+
+constexpr int kIgnored = -1;  // slot of a row without a label
+constexpr int kBadLabel = -2;  // slot of a row whose label is no token
+
+struct PrepParams {
+  const uint4* hidden;     // [rows][vecs]
+  int64_t rows, vecs;      // vecs = H / 8
+  const int64_t* labels;
+  int64_t ignore, vocab;
+  const float* lse;        // per row (backward), or NULL
+  const float* grad_loss;  // per row, or NULL for zero
+  const float* grad_lse;
+  uint4* packed;           // [padded rows][vecs]
+  int* slot_of;            // [rows]
+  int* plabel;             // packed
+  float* plse;
+  float* pa;
+  float* pb;
+  uint32_t* top;           // fp16 backward: bits of the largest |coefficient|
+  int* count;              // [0] kept rows, [2] K splits of dh
+  int piece_slices, sms;   // K slices of a whole piece of dh, SMs
+  uint32_t* status;
+};
+
+// One block packs kPrepRows rows: it counts the kept rows before its own
+// (reading their labels, 8 bytes each from L2), then a warp copies each row.
+// The last block leaves the count and zeroes the rows up to the next multiple
+// of 16, the K step of dW = d^T h.
+__global__ void __launch_bounds__(32 * kPrepRows) head_prepare_kernel(PrepParams p) {
+  __shared__ int warp_sum[kPrepRows];
+  __shared__ int slots[kPrepRows];
+  __shared__ int total;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * kPrepRows;
+  int before = 0;
+  for (int64_t i = threadIdx.x; i < r0; i += blockDim.x) {
+    const int64_t y = p.labels[i];
+    before += (y != p.ignore && y >= 0 && y < p.vocab) ? 1 : 0;
+  }
+  before = __reduce_add_sync(0xffffffffu, before);
+  if (lane == 0) warp_sum[warp] = before;
+  __syncthreads();
+  if (warp == 0) {
+    int base = lane < kPrepRows ? warp_sum[lane] : 0;
+    base = __reduce_add_sync(0xffffffffu, base);
+    const int64_t r = r0 + lane;
+    const bool mine = lane < kPrepRows && r < p.rows;
+    const int64_t y = mine ? p.labels[r] : p.ignore;
+    const bool ignored = y == p.ignore;
+    const bool kept = mine && !ignored && y >= 0 && y < p.vocab;
+    const unsigned mask = __ballot_sync(0xffffffffu, kept);
+    const int slot =
+        kept ? base + __popc(mask & ((1u << lane) - 1u)) : (ignored ? kIgnored : kBadLabel);
+    if (mine) {
+      p.slot_of[r] = slot;
+      if (slot == kBadLabel && p.status) atomicOr(p.status, CID_STATUS_TOKEN_ID_OUT_OF_RANGE);
+    }
+    if (kept) {
+      p.plabel[slot] = static_cast<int>(y);
+      if (p.lse != nullptr) {
+        const float gl = p.grad_loss ? p.grad_loss[r] : 0.0f;
+        const float ge = p.grad_lse ? p.grad_lse[r] : 0.0f;
+        p.plse[slot] = p.lse[r];
+        p.pa[slot] = gl + ge;
+        p.pb[slot] = gl;
+        if (p.top) atomicMax(p.top, __float_as_uint(fmaxf(fabsf(gl + ge), fabsf(gl))));
+      }
+    }
+    if (lane < kPrepRows) slots[lane] = mine ? slot : kIgnored;
+    if (lane == 0) total = base + __popc(mask);
+  }
+  __syncthreads();
+  const int slot = slots[warp];
+  if (slot >= 0) {
+    const uint4* src = p.hidden + (r0 + warp) * p.vecs;
+    uint4* dst = p.packed + slot * p.vecs;
+    for (int64_t i = lane; i < p.vecs; i += 32) dst[i] = src[i];
+  }
+  if (r0 + kPrepRows >= p.rows) {
+    const int n = total;
+    const int64_t pad = n > 0 ? (static_cast<int64_t>(n) + 15) / 16 * 16 : 16;
+    for (int64_t i = n * p.vecs + threadIdx.x; i < pad * p.vecs; i += blockDim.x)
+      p.packed[i] = make_uint4(0, 0, 0, 0);
+    if (threadIdx.x == 0) {
+      const int64_t mt = ((n > 0 ? n : 1) + kBM - 1) / kBM;
+      const int64_t nt = (p.vecs * 8 + kBN - 1) / kBN;
+      p.count[0] = n;
+      p.count[2] = dh_splits(mt * nt, p.piece_slices, p.sms);
+    }
+  }
+}
+
+// loss and log-sum-exp of 32 rows a block from the tiles' (max, sum of exp)
+__global__ void __launch_bounds__(256)
+    head_loss_kernel(const float2* records, int64_t tiles, int64_t rec_stride,
+                     const float* label_logit, const int* slot_of, int64_t rows, float* loss,
+                     float* lse) {
+  __shared__ float sm[8][32], ss[8][32];
+  const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+  const int slot = r < rows ? slot_of[r] : kIgnored;
+  float m = -INFINITY, s = 0.0f;
+  auto merge = [&](float om, float os) {
+    const float nm = fmaxf(m, om);
+    const float off = nm == -INFINITY ? 0.0f : nm * kLog2e;
+    // an empty side has s = 0 and m = -inf: its factor is 2^-inf = 0
+    s = s * ex2(fmaf(m, kLog2e, -off)) + os * ex2(fmaf(om, kLog2e, -off));
+    m = nm;
+  };
+  if (slot >= 0)
+    for (int64_t t = part; t < tiles; t += 8) {
+      const float2 q = records[t * rec_stride + slot];
+      merge(q.x, q.y);
+    }
+  sm[part][lane] = m;
+  ss[part][lane] = s;
+  __syncthreads();
+  if (part == 0 && r < rows) {
+    for (int i = 1; i < 8; ++i) merge(sm[i][lane], ss[i][lane]);
+    if (slot >= 0) {
+      const float l = m + logf(s);
+      lse[r] = l;
+      loss[r] = l - label_logit[slot];
+    } else {
+      const float q = slot == kIgnored ? 0.0f : __int_as_float(0x7fffffff);
+      lse[r] = q;
+      loss[r] = q;
+    }
+  }
+}
+
+// dh of every row: the splits' partial sums in ascending order, 16 bits; zero
+// for an ignored row, NaN for a label that is no token
+template <typename T>
+__global__ void __launch_bounds__(256)
+    head_dhidden_kernel(const float* partial, const int* slot_of, const int* count,
+                        int64_t hidden, const uint32_t* top,
+                        T* out) {
+  const int64_t r = blockIdx.x;
+  const int slot = slot_of[r];
+  const int64_t n = *count;
+  const int64_t mt = ((n > 0 ? n : 1) + kBM - 1) / kBM, nt = (hidden + kBN - 1) / kBN;
+  const int splits = count[2];
+  const float inv = 1.0f / coef_scale(top);
+  for (int64_t c = threadIdx.x * 8; c < hidden; c += blockDim.x * 8) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = slot == kBadLabel ? __int_as_float(0x7fffffff) : 0.0f;
+    if (slot >= 0) {
+      const int64_t tile = (slot / kBM) * nt + c / kBN;
+      const float* q = partial + tile * (kBM * kBN) + (slot % kBM) * kBN + c % kBN;
+      for (int s = 0; s < splits; ++s, q += mt * nt * (kBM * kBN)) {
+        const float4 x = reinterpret_cast<const float4*>(q)[0];
+        const float4 y = reinterpret_cast<const float4*>(q)[1];
+        v[0] += x.x;
+        v[1] += x.y;
+        v[2] += x.z;
+        v[3] += x.w;
+        v[4] += y.x;
+        v[5] += y.y;
+        v[6] += y.z;
+        v[7] += y.w;
+      }
+    }
+    uint4 o;
+    o.x = pack2<T>(v[0] * inv, v[1] * inv);
+    o.y = pack2<T>(v[2] * inv, v[3] * inv);
+    o.z = pack2<T>(v[4] * inv, v[5] * inv);
+    o.w = pack2<T>(v[6] * inv, v[7] * inv);
+    *reinterpret_cast<uint4*>(out + r * hidden + c) = o;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------
+
+constexpr int64_t kMaxLossRows = INT32_MAX - 2 * kBM;
+
+int64_t round_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
+
+// Vocabulary columns of a piece of the backward: d of 64 MB stays in L2
+// between the kernel that writes it and the two that read it, and no fewer
+// than 4096 columns, below which a piece has too few tiles for the SMs.
+int64_t piece_cols(int64_t rows, int64_t vocab) {
+  constexpr int64_t kPieceBytes = 64 << 20;
+  int64_t c = kPieceBytes / (2 * round_up(rows, kBM)) / kBN * kBN;
+  if (c < 4096) c = 4096;
+  const int64_t all = round_up(vocab, kBN);
+  return c < all ? c : all;
+}
+
+// Byte offsets of the workspace's parts.
+struct Layout {
+  size_t count, slot_of, plabel, plse, pa, pb, label_logit, packed, records, d, partial, bytes;
+};
+
+Layout layout(int64_t rows, int64_t hidden, int64_t vocab, bool backward) {
+  Layout l = {};
+  size_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const size_t here = at;
+    at += static_cast<size_t>(round_up(bytes, 1024));
+    return here;
+  };
+  const int64_t padded = round_up(rows, kBM);
+  l.count = take(16);  // count, top, splits
+  l.slot_of = take(rows * 4);
+  l.plabel = take(padded * 4);
+  l.packed = take(padded * hidden * 2);
+  if (!backward) {
+    l.label_logit = take(padded * 4);
+    l.records = take((vocab + kBN - 1) / kBN * padded * 8);
+  } else {
+    l.plse = take(padded * 4);
+    l.pa = take(padded * 4);
+    l.pb = take(padded * 4);
+    l.d = take(padded * piece_cols(rows, vocab) * 2);
+    const int64_t tiles = padded / kBM * ((hidden + kBN - 1) / kBN);
+    l.partial = take((tiles > kSplitUnits ? tiles : kSplitUnits) * kBM * kBN * 4);
+  }
+  l.bytes = at;
+  return l;
+}
+
+bool loss_extents_ok(int64_t rows, int64_t hidden, int64_t vocab) {
+  int64_t n = 0;
+  return rows >= 0 && rows <= kMaxLossRows && hidden > 0 && hidden % 8 == 0 &&
+         hidden <= INT32_MAX - kBN && vocab > 0 && vocab <= INT32_MAX - kBN &&
+         count_ok(rows, hidden, &n) && n <= kMaxCount && count_ok(vocab, hidden, &n) &&
+         n <= kMaxCount && count_ok((vocab + kBN - 1) / kBN, rows, &n) && n <= kMaxCount;
+}
+
+template <typename T, Mode kMode>
+int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const Params& p, int64_t grid,
+                cudaStream_t stream) {
+  const cudaError_t e = cudaFuncSetAttribute(head_gemm_kernel<T, kMode>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             static_cast<int>(kSmemBytes));
+  if (e != cudaSuccess) return record_cuda_error(e);
+  head_gemm_kernel<T, kMode>
+      <<<static_cast<unsigned>(grid), kThreads, kSmemBytes, stream>>>(a, b, p);
+  return launch_result();
+}
+
+struct Call {
+  cid_dtype_t dtype;
+  const void* hidden;
+  int64_t rows, dim;
+  const void* weight;
+  int64_t vocab;
+  const int64_t* labels;
+  int64_t ignore;
+  unsigned char* ws;
+  uint32_t* status;
+  cudaStream_t stream;
+};
+
+int launch_prepare(const Call& c, const Layout& l, const float* lse, const float* grad_loss,
+                   const float* grad_lse, bool scaled) {
+  PrepParams q = {};
+  q.hidden = static_cast<const uint4*>(c.hidden);
+  q.rows = c.rows;
+  q.vecs = c.dim / 8;
+  q.labels = c.labels;
+  q.ignore = c.ignore;
+  q.vocab = c.vocab;
+  q.lse = lse;
+  q.grad_loss = grad_loss;
+  q.grad_lse = grad_lse;
+  q.packed = reinterpret_cast<uint4*>(c.ws + l.packed);
+  q.slot_of = reinterpret_cast<int*>(c.ws + l.slot_of);
+  q.plabel = reinterpret_cast<int*>(c.ws + l.plabel);
+  q.plse = reinterpret_cast<float*>(c.ws + l.plse);
+  q.pa = reinterpret_cast<float*>(c.ws + l.pa);
+  q.pb = reinterpret_cast<float*>(c.ws + l.pb);
+  q.count = reinterpret_cast<int*>(c.ws + l.count);
+  q.piece_slices = static_cast<int>(piece_cols(c.rows, c.vocab) / kBK);
+  q.sms = sm_count();
+  q.status = c.status;
+  if (scaled) {
+    q.top = reinterpret_cast<uint32_t*>(c.ws + l.count) + 1;
+    const cudaError_t e = cudaMemsetAsync(q.top, 0, 4, c.stream);
+    if (e != cudaSuccess) return record_cuda_error(e);
+  }
+  const int64_t blocks = (c.rows + kPrepRows - 1) / kPrepRows;
+  head_prepare_kernel<<<static_cast<unsigned>(blocks), 32 * kPrepRows, 0, c.stream>>>(q);
+  return launch_result();
+}
+
+template <typename T>
+int run_loss(const Call& c, float* loss, float* lse) {
+  const Layout l = layout(c.rows, c.dim, c.vocab, false);
+  const int64_t padded = round_up(c.rows, kBM);
+  int rc = launch_prepare(c, l, nullptr, nullptr, nullptr, false);
+  if (rc != CID_OK) return rc;
+  CUtensorMap map_a, map_b;
+  rc = make_map_sw128(&map_a, c.dtype, c.ws + l.packed, c.dim, padded, c.dim, kBK, kBM);
+  if (rc == CID_OK)
+    rc = make_map_sw128(&map_b, c.dtype, c.weight, c.dim, c.vocab, c.dim, kBK, kBN);
+  if (rc != CID_OK) return rc;
+  Params p = {};
+  p.count = reinterpret_cast<const int*>(c.ws + l.count);
+  p.hidden = c.dim;
+  p.cols = c.vocab;
+  p.labels = reinterpret_cast<const int*>(c.ws + l.plabel);
+  p.records = reinterpret_cast<float2*>(c.ws + l.records);
+  p.label_logit = reinterpret_cast<float*>(c.ws + l.label_logit);
+  p.rec_stride = padded;
+  p.status = c.status;
+  const int64_t tiles = (c.vocab + kBN - 1) / kBN;
+  const int64_t units = padded / kBM * tiles;
+  rc = launch_gemm<T, kLoss>(map_a, map_b, p, units < sm_count() ? units : sm_count(), c.stream);
+  if (rc != CID_OK) return rc;
+  head_loss_kernel<<<static_cast<unsigned>((c.rows + 31) / 32), 256, 0, c.stream>>>(
+      p.records, tiles, padded, p.label_logit, reinterpret_cast<const int*>(c.ws + l.slot_of),
+      c.rows, loss, lse);
+  return launch_result();
+}
+
+template <typename T>
+int run_backward(const Call& c, const float* lse, const float* grad_loss, const float* grad_lse,
+                 void* grad_hidden, void* grad_weight) {
+  const Layout l = layout(c.rows, c.dim, c.vocab, true);
+  const int64_t padded = round_up(c.rows, kBM);
+  const int64_t piece = piece_cols(c.rows, c.vocab);
+  const bool scaled = c.dtype == CID_DTYPE_F16;
+  const int sms = sm_count();
+  int rc = launch_prepare(c, l, lse, grad_loss, grad_lse, scaled);
+  if (rc != CID_OK) return rc;
+  CUtensorMap h_k, h_mn, w_k, w_mn, d_k, d_mn;
+  rc = make_map_sw128(&h_k, c.dtype, c.ws + l.packed, c.dim, padded, c.dim, kBK, kBM);
+  if (rc == CID_OK)
+    rc = make_map_sw128(&h_mn, c.dtype, c.ws + l.packed, c.dim, padded, c.dim, 64, kBK);
+  if (rc == CID_OK) rc = make_map_sw128(&w_k, c.dtype, c.weight, c.dim, c.vocab, c.dim, kBK, kBN);
+  if (rc == CID_OK) rc = make_map_sw128(&w_mn, c.dtype, c.weight, c.dim, c.vocab, c.dim, 64, kBK);
+  if (rc == CID_OK) rc = make_map_sw128(&d_k, c.dtype, c.ws + l.d, piece, padded, piece, kBK, kBM);
+  if (rc == CID_OK) rc = make_map_sw128(&d_mn, c.dtype, c.ws + l.d, piece, padded, piece, 64, kBK);
+  if (rc != CID_OK) return rc;
+  Params p = {};
+  p.count = reinterpret_cast<const int*>(c.ws + l.count);
+  p.hidden = c.dim;
+  p.pitch = piece;
+  p.labels = reinterpret_cast<const int*>(c.ws + l.plabel);
+  p.lse = reinterpret_cast<const float*>(c.ws + l.plse);
+  p.ca = reinterpret_cast<const float*>(c.ws + l.pa);
+  p.cb = reinterpret_cast<const float*>(c.ws + l.pb);
+  p.top = scaled ? reinterpret_cast<const uint32_t*>(c.ws + l.count) + 1 : nullptr;
+  p.d = c.ws + l.d;
+  p.grad_weight = grad_weight;
+  p.partial = reinterpret_cast<float*>(c.ws + l.partial);
+  p.status = c.status;
+  const int64_t mt = padded / kBM, ht = (c.dim + kBN - 1) / kBN;
+  for (int64_t c0 = 0; c0 < c.vocab; c0 += piece) {
+    p.col0 = c0;
+    p.cols = c.vocab - c0 < piece ? c.vocab - c0 : piece;
+    p.accumulate = c0 > 0;
+    const int64_t nt = (p.cols + kBN - 1) / kBN;
+    auto grid = [&](int64_t units) { return units < sms ? units : sms; };
+    rc = launch_gemm<T, kDlogits>(h_k, w_k, p, grid(mt * nt), c.stream);
+    if (rc == CID_OK && grad_hidden != nullptr)
+      rc = launch_gemm<T, kDhidden>(d_k, w_mn, p, sms, c.stream);
+    if (rc == CID_OK && grad_weight != nullptr)
+      rc = launch_gemm<T, kDweight>(d_mn, h_mn, p, grid((p.cols + kBM - 1) / kBM * ht), c.stream);
+    if (rc != CID_OK) return rc;
+  }
+  if (grad_hidden == nullptr) return CID_OK;
+  head_dhidden_kernel<T><<<static_cast<unsigned>(c.rows), 256, 0, c.stream>>>(
+      p.partial, reinterpret_cast<const int*>(c.ws + l.slot_of), p.count, c.dim,
+      p.top, static_cast<T*>(grad_hidden));
+  return launch_result();
+}
+
+int check_loss(cid_dtype_t dtype, const void* hidden, int64_t rows, int64_t dim,
+               const void* weight, int64_t vocab, const int64_t* labels, const void* workspace,
+               const uint32_t* status) {
+  if (dtype != CID_DTYPE_BF16 && dtype != CID_DTYPE_F16) return CID_ERR_UNSUPPORTED_DTYPE;
+  if (!loss_extents_ok(rows, dim, vocab)) return CID_ERR_INVALID_ARGUMENT;
+  if (misaligned({{hidden, 16}, {weight, 16}, {labels, 8}, {workspace, 16}, {status, 4}}))
+    return CID_ERR_MISALIGNED;
+  return CID_OK;
+}
+
+}  // namespace
+}  // namespace cid
+
+using namespace cid;
+
+extern "C" size_t cid_lm_head_cross_entropy_workspace_bytes(int64_t rows, int64_t hidden_dim,
+                                                            int64_t vocab, int backward) {
+  if (rows <= 0 || !loss_extents_ok(rows, hidden_dim, vocab)) return 0;
+  return layout(rows, hidden_dim, vocab, backward != 0).bytes;
+}
+
+extern "C" int cid_lm_head_cross_entropy(cid_dtype_t dtype, const void* hidden, int64_t rows,
+                                         int64_t hidden_dim, const void* weight, int64_t vocab,
+                                         const int64_t* labels, int64_t ignore_index, float* loss,
+                                         float* log_sum_exp, void* workspace,
+                                         size_t workspace_bytes, uint32_t* status, void* stream) {
+  const int rc =
+      check_loss(dtype, hidden, rows, hidden_dim, weight, vocab, labels, workspace, status);
+  if (rc != CID_OK) return rc;
+  if (misaligned({{loss, 4}, {log_sum_exp, 4}})) return CID_ERR_MISALIGNED;
+  if (rows == 0) return CID_OK;
+  if (any_null({hidden, weight, labels, loss, log_sum_exp, workspace}))
+    return CID_ERR_INVALID_ARGUMENT;
+  if (workspace_bytes < cid_lm_head_cross_entropy_workspace_bytes(rows, hidden_dim, vocab, 0))
+    return CID_ERR_SCRATCH_LIMIT;
+  const Call c{dtype, hidden,       rows,
+               hidden_dim, weight,  vocab,
+               labels, ignore_index, static_cast<unsigned char*>(workspace),
+               status, as_stream(stream)};
+  return dtype == CID_DTYPE_F16 ? run_loss<__half>(c, loss, log_sum_exp)
+                                : run_loss<__nv_bfloat16>(c, loss, log_sum_exp);
+}
+
+extern "C" int cid_lm_head_cross_entropy_backward(
+    cid_dtype_t dtype, const void* hidden, int64_t rows, int64_t hidden_dim, const void* weight,
+    int64_t vocab, const int64_t* labels, int64_t ignore_index, const float* log_sum_exp,
+    const float* grad_loss, const float* grad_log_sum_exp, void* grad_hidden, void* grad_weight,
+    void* workspace, size_t workspace_bytes, uint32_t* status, void* stream) {
+  const int rc =
+      check_loss(dtype, hidden, rows, hidden_dim, weight, vocab, labels, workspace, status);
+  if (rc != CID_OK) return rc;
+  if (misaligned({{log_sum_exp, 4},
+                  {grad_loss, 4},
+                  {grad_log_sum_exp, 4},
+                  {grad_hidden, 16},
+                  {grad_weight, 16}}))
+    return CID_ERR_MISALIGNED;
+  if (grad_hidden == nullptr && grad_weight == nullptr) return CID_OK;
+  if (rows == 0) {
+    if (grad_weight == nullptr) return CID_OK;
+    return record_cuda_error(cudaMemsetAsync(
+        grad_weight, 0, static_cast<size_t>(vocab) * hidden_dim * 2, as_stream(stream)));
+  }
+  if (any_null({hidden, weight, labels, log_sum_exp, workspace})) return CID_ERR_INVALID_ARGUMENT;
+  if (workspace_bytes < cid_lm_head_cross_entropy_workspace_bytes(rows, hidden_dim, vocab, 1))
+    return CID_ERR_SCRATCH_LIMIT;
+  const Call c{dtype, hidden,       rows,
+               hidden_dim, weight,  vocab,
+               labels, ignore_index, static_cast<unsigned char*>(workspace),
+               status, as_stream(stream)};
+  return dtype == CID_DTYPE_F16
+             ? run_backward<__half>(c, log_sum_exp, grad_loss, grad_log_sum_exp, grad_hidden,
+                                    grad_weight)
+             : run_backward<__nv_bfloat16>(c, log_sum_exp, grad_loss, grad_log_sum_exp,
+                                           grad_hidden, grad_weight);
+}

@@ -340,6 +340,107 @@ at::Tensor lm_head_shard_records(Backend backend, const at::Tensor& token_ids,
 }
 
 // ---------------------------------------------------------------------------
+// lm_head_cross_entropy (additive)
+// ---------------------------------------------------------------------------
+
+namespace {
+
+void check_head_loss(const char* op, const at::Tensor& labels, const at::Tensor& hidden,
+                     const at::Tensor& weight) {
+  TORCH_CHECK(labels.scalar_type() == at::kLong, "labels must use torch.int64");
+  TORCH_CHECK(hidden.dim() >= 1 && hidden.dim() - 1 == labels.dim() &&
+                  hidden.sizes().slice(0, hidden.dim() - 1) == labels.sizes(),
+              "hidden must have shape [*labels.shape, hidden_dim]");
+  TORCH_CHECK(weight.dim() == 2 && weight.size(1) == hidden.size(-1),
+              "weight must have shape [vocab, hidden_dim]");
+  TORCH_CHECK((hidden.scalar_type() == at::kBFloat16 || hidden.scalar_type() == at::kHalf) &&
+                  weight.scalar_type() == hidden.scalar_type(),
+              "hidden and weight must both use torch.bfloat16 or both torch.float16");
+  TORCH_CHECK(weight.size(0) > 0, "weight vocabulary dimension must be non-empty");
+  TORCH_CHECK(hidden.size(-1) > 0 && hidden.size(-1) % 8 == 0,
+              "hidden_dim must be a positive multiple of 8");
+  same_device(op, {&labels, &hidden, &weight});
+}
+
+// Contiguous with a 16-byte-aligned base (TMA): a view that starts elsewhere is copied.
+at::Tensor aligned16(const at::Tensor& t) {
+  auto c = t.contiguous();
+  return reinterpret_cast<std::uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
+}
+
+}  // namespace
+
+std::tuple<at::Tensor, at::Tensor> lm_head_cross_entropy(Backend backend, const at::Tensor& labels,
+                                                         const at::Tensor& hidden,
+                                                         const at::Tensor& weight,
+                                                         std::int64_t ignore_index) {
+  check_head_loss("lm_head_cross_entropy", labels, hidden, weight);
+  const auto f32 = labels.options().dtype(at::kFloat);
+  auto loss = at::empty(labels.sizes(), f32);
+  auto lse = at::empty(labels.sizes(), f32);
+  if (backend == Backend::kMeta) return {loss, lse};
+  if (backend == Backend::kCpu) detail::no_cpu_backend("lm_head_cross_entropy");
+  if (labels.numel() == 0) return {loss, lse};
+  const c10::cuda::CUDAGuard guard(hidden.device());
+  auto h = aligned16(hidden);
+  auto w = aligned16(weight);
+  auto y = labels.contiguous();
+  const size_t bytes =
+      cid_lm_head_cross_entropy_workspace_bytes(y.numel(), h.size(-1), w.size(0), 0);
+  auto ws = at::empty({static_cast<std::int64_t>(bytes)}, hidden.options().dtype(at::kByte));
+  check_result(cid_lm_head_cross_entropy(
+                   dt(h), h.data_ptr(), y.numel(), h.size(-1), w.data_ptr(), w.size(0),
+                   y.data_ptr<std::int64_t>(), ignore_index, loss.data_ptr<float>(),
+                   lse.data_ptr<float>(), ws.data_ptr(), bytes, detail::status_word(h.device()),
+                   stream_of(h)),
+               "lm_head_cross_entropy");
+  return {loss, lse};
+}
+
+std::tuple<at::Tensor, at::Tensor> lm_head_cross_entropy_backward(
+    Backend backend, const std::optional<at::Tensor>& grad_loss,
+    const std::optional<at::Tensor>& grad_log_sum_exp, const at::Tensor& labels,
+    const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& log_sum_exp,
+    std::int64_t ignore_index, bool need_hidden, bool need_weight) {
+  check_head_loss("lm_head_cross_entropy_backward", labels, hidden, weight);
+  TORCH_CHECK(log_sum_exp.sizes() == labels.sizes() && log_sum_exp.scalar_type() == at::kFloat,
+              "log_sum_exp must be the forward's float32 output");
+  for (const auto* g : {&grad_loss, &grad_log_sum_exp})
+    if (g->has_value())
+      TORCH_CHECK((*g)->sizes() == labels.sizes() && (*g)->scalar_type() == at::kFloat,
+                  "output gradients must be float32 of the labels' shape");
+  same_device("lm_head_cross_entropy_backward",
+              {&hidden, &log_sum_exp, grad_loss ? &*grad_loss : nullptr,
+               grad_log_sum_exp ? &*grad_log_sum_exp : nullptr});
+  auto gh = need_hidden ? at::empty(hidden.sizes(), hidden.options())
+                        : at::empty({0}, hidden.options());
+  auto gw = need_weight ? at::empty(weight.sizes(), weight.options())
+                        : at::empty({0}, weight.options());
+  if (backend == Backend::kMeta) return {gh, gw};
+  if (backend == Backend::kCpu) detail::no_cpu_backend("lm_head_cross_entropy_backward");
+  const c10::cuda::CUDAGuard guard(hidden.device());
+  auto h = aligned16(hidden);
+  auto w = aligned16(weight);
+  auto y = labels.contiguous();
+  auto lse = log_sum_exp.contiguous();
+  at::Tensor gl, ge;
+  if (grad_loss) gl = grad_loss->contiguous();
+  if (grad_log_sum_exp) ge = grad_log_sum_exp->contiguous();
+  const size_t bytes =
+      cid_lm_head_cross_entropy_workspace_bytes(y.numel(), h.size(-1), w.size(0), 1);
+  auto ws = at::empty({static_cast<std::int64_t>(bytes)}, hidden.options().dtype(at::kByte));
+  check_result(cid_lm_head_cross_entropy_backward(
+                   dt(h), h.data_ptr(), y.numel(), h.size(-1), w.data_ptr(), w.size(0),
+                   y.data_ptr<std::int64_t>(), ignore_index, lse.data_ptr<float>(),
+                   gl.defined() ? gl.data_ptr<float>() : nullptr,
+                   ge.defined() ? ge.data_ptr<float>() : nullptr,
+                   need_hidden ? gh.data_ptr() : nullptr, need_weight ? gw.data_ptr() : nullptr,
+                   ws.data_ptr(), bytes, detail::status_word(h.device()), stream_of(h)),
+               "lm_head_cross_entropy_backward");
+  return {gh, gw};
+}
+
+// ---------------------------------------------------------------------------
 // live_slot_occupancy — csrc/ops.cpp:12-39
 // ---------------------------------------------------------------------------
 

@@ -102,6 +102,22 @@ at::Tensor lm_head_shard_impl(const at::Tensor& ids, const at::Tensor& hidden,
 }
 
 template <Backend B>
+std::tuple<at::Tensor, at::Tensor> head_loss_impl(const at::Tensor& labels,
+                                                  const at::Tensor& hidden,
+                                                  const at::Tensor& weight, std::int64_t ignore) {
+  return lm_head_cross_entropy(B, labels, hidden, weight, ignore);
+}
+
+template <Backend B>
+std::tuple<at::Tensor, at::Tensor> head_loss_backward_impl(
+    const std::optional<at::Tensor>& gl, const std::optional<at::Tensor>& ge,
+    const at::Tensor& labels, const at::Tensor& hidden, const at::Tensor& weight,
+    const at::Tensor& lse, std::int64_t ignore, bool need_hidden, bool need_weight) {
+  return lm_head_cross_entropy_backward(B, gl, ge, labels, hidden, weight, lse, ignore,
+                                        need_hidden, need_weight);
+}
+
+template <Backend B>
 void register_all(torch::Library& m) {
   m.impl("live_slot_occupancy", TORCH_FN(live_impl<B>));
   m.impl("prefix_allocation_mask", TORCH_FN(prefix_impl<B>));
@@ -119,6 +135,8 @@ void register_all(torch::Library& m) {
   m.impl("display_combine_records", TORCH_FN(combine_records_impl<B>));
   m.impl("lm_head_display_statistics", TORCH_FN(lm_head_impl<B>));
   m.impl("lm_head_shard_records", TORCH_FN(lm_head_shard_impl<B>));
+  m.impl("lm_head_cross_entropy", TORCH_FN(head_loss_impl<B>));
+  m.impl("lm_head_cross_entropy_backward", TORCH_FN(head_loss_backward_impl<B>));
 }
 
 }  // namespace
@@ -188,6 +206,15 @@ TORCH_LIBRARY(cid_engine, m) {
   m.def(
       "lm_head_shard_records(Tensor token_ids, Tensor hidden, Tensor weight_shard, "
       "int vocab_offset, int total_vocab, bool round_bf16=True) -> Tensor");
+  // additive: the loss of the LM head and its gradient (autograd is
+  // registered in Python, cid_engine/head.py)
+  m.def(
+      "lm_head_cross_entropy(Tensor labels, Tensor hidden, Tensor weight, "
+      "int ignore_index=-100) -> (Tensor, Tensor)");
+  m.def(
+      "lm_head_cross_entropy_backward(Tensor? grad_loss, Tensor? grad_log_sum_exp, "
+      "Tensor labels, Tensor hidden, Tensor weight, Tensor log_sum_exp, int ignore_index, "
+      "bool need_hidden, bool need_weight) -> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(cid_engine, CUDA, m) {

@@ -401,6 +401,50 @@ CID_API int cid_lm_head_shard_records(const void* hidden, int64_t rows, int64_t 
                         uint32_t* status, void* stream);
 
 /* ---------------------------------------------------------------------- */
+/* LM head loss (no reference counterpart: the reference's corruption     */
+/* operators, csrc/ops.cpp:292-444, make the labels; the loss is outside  */
+/* it).                                                                   */
+/* ---------------------------------------------------------------------- */
+
+/* Workspace bytes of the two calls below (backward = 0 or 1); 0 for extents
+ * outside their ranges.  They grow with rows, and the backward holds the
+ * logits' gradient of one piece of the vocabulary at a time. */
+CID_API size_t cid_lm_head_cross_entropy_workspace_bytes(int64_t rows, int64_t hidden_dim,
+                        int64_t vocab, int backward);
+
+/* Softmax cross entropy of logits = hidden @ weight^T against `labels`,
+ * without writing the logits:
+ *   log_sum_exp[r] = log sum_v exp logits[r, v]
+ *   loss[r] = log_sum_exp[r] - logits[r, labels[r]]
+ * hidden rows x hidden_dim and weight vocab x hidden_dim of `dtype` (BF16 or
+ * F16), row-major, hidden_dim % 8 == 0, 16-byte aligned (workspace too); f32
+ * accumulation on the tcgen05 tensor cores, logits kept in f32.  A row whose
+ * label is ignore_index has loss and log_sum_exp 0, and its hidden row is not
+ * read.  Any other label outside [0, vocab): NaN in both outputs and
+ * CID_STATUS_TOKEN_ID_OUT_OF_RANGE.  A bounded wait that runs out sets
+ * CID_STATUS_LM_HEAD_TIMEOUT.  The kept rows are counted on the device: calls
+ * can be captured into CUDA graphs and replayed with other labels. */
+CID_API int cid_lm_head_cross_entropy(cid_dtype_t dtype, const void* hidden, int64_t rows,
+                        int64_t hidden_dim, const void* weight, int64_t vocab,
+                        const int64_t* labels, int64_t ignore_index, float* loss,
+                        float* log_sum_exp, void* workspace, size_t workspace_bytes,
+                        uint32_t* status, void* stream);
+
+/* Gradients of cid_lm_head_cross_entropy for the given gradients of its
+ * outputs (rows f32 each; NULL means zero).  log_sum_exp: the forward's
+ * output.  grad_hidden rows x hidden_dim and grad_weight vocab x hidden_dim of
+ * `dtype`, 16-byte aligned, overwritten; either may be NULL when it is not
+ * wanted.  The logits are computed again a piece of the vocabulary at a time.
+ * Rows with ignore_index: zero grad_hidden, no part in grad_weight.  Rows with
+ * another label outside [0, vocab): NaN grad_hidden, no part in grad_weight. */
+CID_API int cid_lm_head_cross_entropy_backward(cid_dtype_t dtype, const void* hidden,
+                        int64_t rows, int64_t hidden_dim, const void* weight, int64_t vocab,
+                        const int64_t* labels, int64_t ignore_index, const float* log_sum_exp,
+                        const float* grad_loss, const float* grad_log_sum_exp,
+                        void* grad_hidden, void* grad_weight, void* workspace,
+                        size_t workspace_bytes, uint32_t* status, void* stream);
+
+/* ---------------------------------------------------------------------- */
 /* Peer record exchange (no reference counterpart: the multi-GPU form of   */
 /* the vocabulary-parallel statistics, csrc/ops.cpp:446-474 sharded).      */
 /* ---------------------------------------------------------------------- */

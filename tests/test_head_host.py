@@ -1,0 +1,126 @@
+"""The LM head's training and 4-bit operators on the host: schemas, refusals,
+shapes on the meta device, autograd, and the C ABI's checks (no GPU)."""
+
+from __future__ import annotations
+
+import ctypes
+from pathlib import Path
+
+import pytest
+import torch
+
+import cid_engine
+
+ROOT = Path(__file__).resolve().parent.parent
+LIB = ROOT / "cid-engine_b200" / "cid_engine" / "libcid_engine_b200.so"
+OK, INVALID, DTYPE, MISALIGNED, SCRATCH = 0, 1, 2, 4, 6
+F32, F16, BF16 = 0, 2, 3
+
+
+@pytest.fixture(scope="module")
+def lib() -> ctypes.CDLL:
+    lib = ctypes.CDLL(str(LIB))
+    lib.cid_lm_head_cross_entropy_workspace_bytes.restype = ctypes.c_size_t
+    return lib
+
+
+def _loss_inputs(device="cpu", dtype=torch.bfloat16, grad=False):
+    y = torch.zeros(3, 5, dtype=torch.long, device=device)
+    h = torch.zeros(3, 5, 64, dtype=dtype, device=device, requires_grad=grad)
+    w = torch.zeros(100, 64, dtype=dtype, device=device, requires_grad=grad)
+    return y, h, w
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_loss_shapes_and_gradients_on_meta(dtype) -> None:
+    y, h, w = _loss_inputs("meta", dtype, grad=True)
+    loss, lse = cid_engine.lm_head_cross_entropy(y, h, w)
+    for t in (loss, lse):
+        assert t.shape == (3, 5) and t.dtype == torch.float32 and t.requires_grad
+    gh, gw = torch.autograd.grad(loss.mean() + (lse**2).mean(), (h, w))
+    assert gh.shape == h.shape and gw.shape == w.shape and gh.dtype == gw.dtype == dtype
+    for ignore in (-100, 7):  # the default and another value take the same path
+        loss, _ = cid_engine.lm_head_cross_entropy(y, h.detach(), w, ignore_index=ignore)
+        (gw,) = torch.autograd.grad(loss.sum(), w)
+        assert gw.shape == w.shape
+    loss, _ = cid_engine.lm_head_cross_entropy(y, h.detach(), w.detach())
+    assert not loss.requires_grad
+
+
+def test_loss_has_no_second_gradient() -> None:
+    y, h, w = _loss_inputs("meta", grad=True)
+    loss, _ = cid_engine.lm_head_cross_entropy(y, h, w)
+    gh, _ = torch.autograd.grad(loss.sum(), (h, w), create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(gh.sum(), h)
+
+
+def test_loss_refusals() -> None:
+    y, h, w = _loss_inputs()
+    f = cid_engine.lm_head_cross_entropy
+    with pytest.raises(RuntimeError, match="CUDA devices only"):
+        f(y, h, w)
+    with pytest.raises(RuntimeError, match="labels must use torch.int64"):
+        f(y.int(), h, w)
+    with pytest.raises(RuntimeError, match=r"\[\*labels.shape, hidden_dim\]"):
+        f(y[:2], h, w)
+    with pytest.raises(RuntimeError, match=r"\[vocab, hidden_dim\]"):
+        f(y, h, w[:, :56])
+    with pytest.raises(RuntimeError, match="both"):
+        f(y, h, w.half())
+    with pytest.raises(RuntimeError, match="both"):
+        f(y, h.float(), w.float())
+    with pytest.raises(RuntimeError, match="non-empty"):
+        f(y, h, w[:0])
+    with pytest.raises(RuntimeError, match="multiple of 8"):
+        f(y, h[..., :60], w[:, :60])
+    with pytest.raises(RuntimeError, match="same device"):
+        f(y.to("meta"), h, w)
+    b = torch.ops.cid_engine.lm_head_cross_entropy_backward
+    g = torch.zeros(3, 5)
+    with pytest.raises(RuntimeError, match="log_sum_exp"):
+        b(g, None, y, h, w, torch.zeros(3), -100, True, True)
+    with pytest.raises(RuntimeError, match="output gradients"):
+        b(g.double(), None, y, h, w, g, -100, True, True)
+    with pytest.raises(RuntimeError, match="CUDA devices only"):
+        b(g, None, y, h, w, g, -100, True, True)
+
+
+def test_loss_c_abi_checks(lib: ctypes.CDLL) -> None:
+    i64, p, null, size = ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p(0), ctypes.c_size_t
+    ws = lib.cid_lm_head_cross_entropy_workspace_bytes
+
+    def need(rows, dim, vocab, backward):
+        return ws(i64(rows), i64(dim), i64(vocab), ctypes.c_int(backward))
+
+    assert 0 < need(4, 64, 300, 0) < need(4, 64, 300, 1)
+    for bad in ((0, 64, 300), (-1, 64, 300), (4, 60, 300), (4, 0, 300), (4, 64, 0), (4, 64, 2**31 - 1),
+                (2**31, 64, 300), (2**30, 2**30, 300)):
+        assert need(*bad, 0) == 0
+
+    def loss(dtype=BF16, rows=4, dim=64, vocab=300, h=0x1000, w=0x2000, y=0x3000, out=0x4000,
+             bytes_=1 << 40):
+        return lib.cid_lm_head_cross_entropy(
+            dtype, p(h), i64(rows), i64(dim), p(w), i64(vocab), p(y), i64(-100), p(out),
+            p(0x5000), p(0x6000), size(bytes_), null, null)
+
+    assert loss(dtype=F32) == DTYPE
+    assert loss(dim=12) == INVALID and loss(rows=-1) == INVALID and loss(vocab=0) == INVALID
+    assert loss(h=0x1008) == MISALIGNED and loss(y=0x3004) == MISALIGNED
+    assert loss(out=0x4002) == MISALIGNED
+    assert loss(rows=0) == OK
+    assert loss(h=0) == INVALID and loss(y=0) == INVALID and loss(out=0) == INVALID
+    assert loss(bytes_=need(4, 64, 300, 0) - 1) == SCRATCH
+
+    def back(dtype=BF16, rows=4, dim=64, lse=0x4000, gl=0x4100, gh=0x5000, gw=0x6000,
+             bytes_=1 << 40):
+        return lib.cid_lm_head_cross_entropy_backward(
+            dtype, p(0x1000), i64(rows), i64(dim), p(0x2000), i64(300), p(0x3000), i64(-100),
+            p(lse), p(gl), null, p(gh), p(gw), p(0x7000), size(bytes_), null, null)
+
+    assert back(dtype=F32) == DTYPE and back(dim=4) == INVALID
+    assert back(gh=0x5008) == MISALIGNED and back(gl=0x4102) == MISALIGNED
+    assert back(gh=0, gw=0) == OK  # nothing wanted
+    assert back(rows=0, gw=0) == OK
+    assert back(lse=0) == INVALID
+    assert back(bytes_=need(4, 64, 300, 1) - 1) == SCRATCH
