@@ -324,7 +324,14 @@ def lm_head_shard_records(
                                                       vocab_offset, total_vocab, round_bf16)
 
 
-from cid_engine.head import lm_head_cross_entropy  # noqa: E402
+from cid_engine.head import (  # noqa: E402
+    QuantizedLMHead,
+    lm_head_cross_entropy,
+    lm_head_dequantize,
+    lm_head_quantize,
+    lm_head_quantized_display_statistics,
+    lm_head_quantized_logits,
+)
 from cid_engine.step import refine_step, refine_step_from_hidden  # noqa: E402
 from cid_engine.loop import DisplayRefineLoop  # noqa: E402
 
@@ -332,6 +339,7 @@ __all__ = [
     "CANN_BACKEND_BUILT",
     "CUDA_BACKEND_BUILT",
     "DisplayRefineLoop",
+    "QuantizedLMHead",
     "ROCM_BACKEND_BUILT",
     "batched_linear_assignment",
     "device_status",
@@ -342,7 +350,11 @@ __all__ = [
     "display_token_statistics_with_repetition",
     "live_slot_occupancy",
     "lm_head_cross_entropy",
+    "lm_head_dequantize",
     "lm_head_display_statistics",
+    "lm_head_quantize",
+    "lm_head_quantized_display_statistics",
+    "lm_head_quantized_logits",
     "lm_head_shard_records",
     "materialize_cell_snapshot",
     "masked_diffusion_corrupt_from_random",

@@ -26,7 +26,8 @@ Without a producer the caller owns the logits ring: step ``s`` reads
 ``logits_buffers[s % len(logits_buffers)]``.  With ``lm_head_weight`` the ring
 holds the display positions' hidden states ``[B, L, H]`` instead, and each
 step runs the LM head fused with the statistics
-(``refine_step_from_hidden``): no ``[B, L, V]`` logits are written at all.
+(``refine_step_from_hidden``): no ``[B, L, V]`` logits are written at all.  A
+``QuantizedLMHead`` as ``lm_head_weight`` runs it from a 4-bit weight.
 """
 
 from __future__ import annotations
@@ -38,6 +39,7 @@ from collections.abc import Callable, Sequence
 import torch
 from torch import Tensor
 
+from cid_engine.head import QuantizedLMHead
 from cid_engine.step import SlotInputs, StepOutputs, refine_step, refine_step_from_hidden
 
 Producer = Callable[[int, Tensor, Tensor], None]
@@ -68,7 +70,7 @@ class DisplayRefineLoop:
         producer: Producer | None = None,
         host_snapshots: int = 4,
         use_graphs: bool = True,
-        lm_head_weight: Tensor | None = None,
+        lm_head_weight: Tensor | QuantizedLMHead | None = None,
     ) -> None:
         if token_ids.device.type != "cuda":
             raise RuntimeError("DisplayRefineLoop runs on CUDA devices only")

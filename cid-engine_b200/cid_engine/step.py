@@ -17,6 +17,8 @@ from dataclasses import dataclass
 import torch
 from torch import Tensor
 
+from cid_engine.head import QuantizedLMHead
+
 
 @dataclass
 class SlotInputs:
@@ -72,7 +74,7 @@ def refine_step(
 def refine_step_from_hidden(
     token_ids: Tensor,
     hidden: Tensor,
-    lm_head_weight: Tensor,
+    lm_head_weight: Tensor | QuantizedLMHead,
     *,
     mask_token_id: int,
     eos_token_id: int | None,
@@ -84,9 +86,15 @@ def refine_step_from_hidden(
 ) -> StepOutputs:
     """The same step from the display positions' hidden states: the LM head
     and the statistics in one kernel (``lm_head_display_statistics``), so no
-    ``[B, L, V]`` logits are written, then the chain of ``refine_step``."""
-    conf, pred, cur = torch.ops.cid_engine.lm_head_display_statistics(
-        token_ids, hidden, lm_head_weight, round_bf16)
+    ``[B, L, V]`` logits are written, then the chain of ``refine_step``.  A
+    ``QuantizedLMHead`` runs the head from its 4-bit weight
+    (``lm_head_quantized_display_statistics``)."""
+    if isinstance(lm_head_weight, QuantizedLMHead):
+        conf, pred, cur = torch.ops.cid_engine.lm_head_quantized_display_statistics(
+            token_ids, hidden, lm_head_weight.packed, lm_head_weight.scales, round_bf16)
+    else:
+        conf, pred, cur = torch.ops.cid_engine.lm_head_display_statistics(
+            token_ids, hidden, lm_head_weight, round_bf16)
     return step_from_statistics(token_ids, conf, pred, cur, mask_token_id=mask_token_id,
                                 eos_token_id=eos_token_id, reveal_fraction=reveal_fraction,
                                 revision_fraction=revision_fraction,

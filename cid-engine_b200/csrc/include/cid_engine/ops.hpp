@@ -127,6 +127,18 @@ std::tuple<at::Tensor, at::Tensor> lm_head_cross_entropy_backward(
     const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& log_sum_exp,
     std::int64_t ignore_index, bool need_hidden, bool need_weight);
 
+// The LM head with 4-bit weights (additive): packed int32 [vocab, hidden / 8]
+// and scales [vocab, hidden / group] (layout in include/cid_engine_b200.h).
+std::tuple<at::Tensor, at::Tensor> lm_head_quantize(Backend backend, const at::Tensor& weight,
+                                                    std::int64_t group_size);
+at::Tensor lm_head_dequantize(Backend backend, const at::Tensor& packed,
+                              const at::Tensor& scales);
+at::Tensor lm_head_quantized_logits(Backend backend, const at::Tensor& hidden,
+                                    const at::Tensor& packed, const at::Tensor& scales);
+Tensor3 lm_head_quantized_display_statistics(Backend backend, const at::Tensor& token_ids,
+                                             const at::Tensor& hidden, const at::Tensor& packed,
+                                             const at::Tensor& scales, bool round_bf16);
+
 // Device status word (CID_STATUS_* bits) of `device`; read() synchronises.
 std::int64_t read_device_status(std::int64_t device, bool reset);
 

@@ -441,6 +441,141 @@ std::tuple<at::Tensor, at::Tensor> lm_head_cross_entropy_backward(
 }
 
 // ---------------------------------------------------------------------------
+// The LM head with 4-bit weights (additive)
+// ---------------------------------------------------------------------------
+
+namespace {
+
+bool is_16_bit_float(const at::Tensor& t) {
+  return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf;
+}
+
+// Group size of a packed weight and its scales.
+std::int64_t check_packed(const at::Tensor& packed, const at::Tensor& scales) {
+  TORCH_CHECK(packed.dim() == 2 && packed.scalar_type() == at::kInt,
+              "packed must be an int32 tensor of shape [vocab, hidden_dim / 8]");
+  TORCH_CHECK(scales.dim() == 2 && is_16_bit_float(scales) && scales.size(0) == packed.size(0),
+              "scales must be a bfloat16 or float16 tensor of shape [vocab, hidden_dim / "
+              "group_size]");
+  TORCH_CHECK(packed.size(0) > 0, "packed vocabulary dimension must be non-empty");
+  const auto dim = packed.size(1) * 8, groups = scales.size(1);
+  const auto group = groups > 0 && dim % groups == 0 ? dim / groups : 0;
+  TORCH_CHECK(group == 32 || group == 64 || group == 128,
+              "packed and scales must have groups of 32, 64 or 128 columns");
+  return group;
+}
+
+}  // namespace
+
+std::tuple<at::Tensor, at::Tensor> lm_head_quantize(Backend backend, const at::Tensor& weight,
+                                                    std::int64_t group_size) {
+  TORCH_CHECK(weight.dim() == 2, "weight must have shape [vocab, hidden_dim]");
+  TORCH_CHECK(is_16_bit_float(weight), "weight must use torch.bfloat16 or torch.float16");
+  TORCH_CHECK(weight.size(0) > 0, "weight vocabulary dimension must be non-empty");
+  TORCH_CHECK(group_size == 32 || group_size == 64 || group_size == 128,
+              "group_size must be 32, 64 or 128");
+  TORCH_CHECK(weight.size(1) > 0 && weight.size(1) % group_size == 0,
+              "hidden_dim must be a positive multiple of group_size");
+  const auto vocab = weight.size(0), dim = weight.size(1);
+  auto packed = at::empty({vocab, dim / 8}, weight.options().dtype(at::kInt));
+  auto scales = at::empty({vocab, dim / group_size}, weight.options());
+  if (backend == Backend::kMeta) return {packed, scales};
+  if (backend == Backend::kCpu) detail::no_cpu_backend("lm_head_quantize");
+  const c10::cuda::CUDAGuard guard(weight.device());
+  auto w = aligned16(weight);
+  check_result(cid_lm_head_quantize(dt(w), w.data_ptr(), vocab, dim,
+                                    static_cast<int>(group_size),
+                                    reinterpret_cast<std::uint32_t*>(packed.data_ptr<int>()),
+                                    scales.data_ptr(), stream_of(w)),
+               "lm_head_quantize");
+  return {packed, scales};
+}
+
+at::Tensor lm_head_dequantize(Backend backend, const at::Tensor& packed,
+                              const at::Tensor& scales) {
+  const auto group = check_packed(packed, scales);
+  same_device("lm_head_dequantize", {&packed, &scales});
+  auto weight = at::empty({packed.size(0), packed.size(1) * 8}, scales.options());
+  if (backend == Backend::kMeta) return weight;
+  if (backend == Backend::kCpu) detail::no_cpu_backend("lm_head_dequantize");
+  const c10::cuda::CUDAGuard guard(packed.device());
+  auto p = aligned16(packed);
+  auto s = scales.contiguous();
+  check_result(cid_lm_head_dequantize(
+                   dt(s), reinterpret_cast<const std::uint32_t*>(p.data_ptr<int>()), s.data_ptr(),
+                   p.size(0), p.size(1) * 8, static_cast<int>(group), weight.data_ptr(),
+                   stream_of(p)),
+               "lm_head_dequantize");
+  return weight;
+}
+
+at::Tensor lm_head_quantized_logits(Backend backend, const at::Tensor& hidden,
+                                    const at::Tensor& packed, const at::Tensor& scales) {
+  const auto group = check_packed(packed, scales);
+  TORCH_CHECK(hidden.dim() >= 1 && hidden.size(-1) == packed.size(1) * 8,
+              "hidden must have shape [*, hidden_dim]");
+  TORCH_CHECK(hidden.scalar_type() == scales.scalar_type(),
+              "hidden and scales must share a dtype");
+  same_device("lm_head_quantized_logits", {&hidden, &packed, &scales});
+  auto sizes = hidden.sizes().vec();
+  sizes.back() = packed.size(0);
+  auto logits = at::empty(sizes, hidden.options());
+  if (backend == Backend::kMeta) return logits;
+  if (backend == Backend::kCpu) detail::no_cpu_backend("lm_head_quantized_logits");
+  if (hidden.numel() == 0) return logits;
+  const c10::cuda::CUDAGuard guard(hidden.device());
+  auto h = aligned16(hidden);
+  auto p = aligned16(packed);
+  auto s = scales.contiguous();
+  const auto dim = h.size(-1);
+  check_result(cid_lm_head_quantized_logits(
+                   dt(h), h.data_ptr(), h.numel() / dim, dim,
+                   reinterpret_cast<const std::uint32_t*>(p.data_ptr<int>()), s.data_ptr(),
+                   static_cast<int>(group), p.size(0), logits.data_ptr(),
+                   detail::status_word(h.device()), stream_of(h)),
+               "lm_head_quantized_logits");
+  return logits;
+}
+
+Tensor3 lm_head_quantized_display_statistics(Backend backend, const at::Tensor& token_ids,
+                                             const at::Tensor& hidden, const at::Tensor& packed,
+                                             const at::Tensor& scales, bool round_bf16) {
+  const auto group = check_packed(packed, scales);
+  TORCH_CHECK(token_ids.scalar_type() == at::kLong, "token_ids must use torch.int64");
+  TORCH_CHECK(hidden.dim() >= 1 && hidden.dim() - 1 == token_ids.dim() &&
+                  hidden.sizes().slice(0, hidden.dim() - 1) == token_ids.sizes() &&
+                  hidden.size(-1) == packed.size(1) * 8,
+              "hidden must have shape [*token_ids.shape, hidden_dim]");
+  TORCH_CHECK(hidden.scalar_type() == scales.scalar_type(),
+              "hidden and scales must share a dtype");
+  same_device("lm_head_quantized_display_statistics", {&token_ids, &hidden, &packed, &scales});
+  const auto f32 = token_ids.options().dtype(at::kFloat);
+  auto confidence = at::empty(token_ids.sizes(), f32);
+  auto predicted = at::empty(token_ids.sizes(), token_ids.options().dtype(at::kLong));
+  auto current = at::empty(token_ids.sizes(), f32);
+  if (backend == Backend::kMeta) return {confidence, predicted, current};
+  if (backend == Backend::kCpu) detail::no_cpu_backend("lm_head_quantized_display_statistics");
+  if (token_ids.numel() == 0) return {confidence, predicted, current};
+  const c10::cuda::CUDAGuard guard(hidden.device());
+  auto h = aligned16(hidden);
+  auto p = aligned16(packed);
+  auto s = scales.contiguous();
+  auto ids = token_ids.contiguous();
+  const auto rows = ids.numel();
+  const size_t bytes = cid_lm_head_quantized_workspace_bytes(rows, p.size(0));
+  auto ws = at::empty({static_cast<std::int64_t>(bytes)}, hidden.options().dtype(at::kByte));
+  check_result(cid_lm_head_quantized_display_statistics(
+                   dt(h), h.data_ptr(), rows, h.size(-1),
+                   reinterpret_cast<const std::uint32_t*>(p.data_ptr<int>()), s.data_ptr(),
+                   static_cast<int>(group), p.size(0), ids.data_ptr<std::int64_t>(),
+                   round_bf16 ? 1 : 0, confidence.data_ptr<float>(),
+                   predicted.data_ptr<std::int64_t>(), current.data_ptr<float>(), ws.data_ptr(),
+                   bytes, detail::status_word(h.device()), stream_of(h)),
+               "lm_head_quantized_display_statistics");
+  return {confidence, predicted, current};
+}
+
+// ---------------------------------------------------------------------------
 // live_slot_occupancy — csrc/ops.cpp:12-39
 // ---------------------------------------------------------------------------
 

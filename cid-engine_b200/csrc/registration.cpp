@@ -118,6 +118,26 @@ std::tuple<at::Tensor, at::Tensor> head_loss_backward_impl(
 }
 
 template <Backend B>
+std::tuple<at::Tensor, at::Tensor> quantize_impl(const at::Tensor& weight, std::int64_t group) {
+  return lm_head_quantize(B, weight, group);
+}
+template <Backend B>
+at::Tensor dequantize_impl(const at::Tensor& packed, const at::Tensor& scales) {
+  return lm_head_dequantize(B, packed, scales);
+}
+template <Backend B>
+at::Tensor quantized_logits_impl(const at::Tensor& hidden, const at::Tensor& packed,
+                                 const at::Tensor& scales) {
+  return lm_head_quantized_logits(B, hidden, packed, scales);
+}
+template <Backend B>
+Tensor3 quantized_stats_impl(const at::Tensor& ids, const at::Tensor& hidden,
+                             const at::Tensor& packed, const at::Tensor& scales,
+                             bool round_bf16) {
+  return lm_head_quantized_display_statistics(B, ids, hidden, packed, scales, round_bf16);
+}
+
+template <Backend B>
 void register_all(torch::Library& m) {
   m.impl("live_slot_occupancy", TORCH_FN(live_impl<B>));
   m.impl("prefix_allocation_mask", TORCH_FN(prefix_impl<B>));
@@ -137,6 +157,10 @@ void register_all(torch::Library& m) {
   m.impl("lm_head_shard_records", TORCH_FN(lm_head_shard_impl<B>));
   m.impl("lm_head_cross_entropy", TORCH_FN(head_loss_impl<B>));
   m.impl("lm_head_cross_entropy_backward", TORCH_FN(head_loss_backward_impl<B>));
+  m.impl("lm_head_quantize", TORCH_FN(quantize_impl<B>));
+  m.impl("lm_head_dequantize", TORCH_FN(dequantize_impl<B>));
+  m.impl("lm_head_quantized_logits", TORCH_FN(quantized_logits_impl<B>));
+  m.impl("lm_head_quantized_display_statistics", TORCH_FN(quantized_stats_impl<B>));
 }
 
 }  // namespace
@@ -215,6 +239,13 @@ TORCH_LIBRARY(cid_engine, m) {
       "lm_head_cross_entropy_backward(Tensor? grad_loss, Tensor? grad_log_sum_exp, "
       "Tensor labels, Tensor hidden, Tensor weight, Tensor log_sum_exp, int ignore_index, "
       "bool need_hidden, bool need_weight) -> (Tensor, Tensor)");
+  // additive: the LM head with 4-bit weights
+  m.def("lm_head_quantize(Tensor weight, int group_size=128) -> (Tensor, Tensor)");
+  m.def("lm_head_dequantize(Tensor packed, Tensor scales) -> Tensor");
+  m.def("lm_head_quantized_logits(Tensor hidden, Tensor packed, Tensor scales) -> Tensor");
+  m.def(
+      "lm_head_quantized_display_statistics(Tensor token_ids, Tensor hidden, Tensor packed, "
+      "Tensor scales, bool round_bf16=True) -> (Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(cid_engine, CUDA, m) {

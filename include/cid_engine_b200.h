@@ -445,6 +445,53 @@ CID_API int cid_lm_head_cross_entropy_backward(cid_dtype_t dtype, const void* hi
                         size_t workspace_bytes, uint32_t* status, void* stream);
 
 /* ---------------------------------------------------------------------- */
+/* LM head with 4-bit weights (no reference counterpart).                 */
+/* ---------------------------------------------------------------------- */
+
+/* A vocab x hidden_dim weight held as codes q in [-8, 7] with one 16-bit scale
+ * for each group of group_size (32, 64 or 128; hidden_dim a multiple of it)
+ * consecutive columns of a row, standing for scale * q:
+ *   packed: vocab x hidden_dim / 8 32-bit words, row-major, 16-byte aligned;
+ *     word j holds q + 8 of column 8 j + 2 i at bits 4 i .. 4 i + 3 and of
+ *     column 8 j + 2 i + 1 at bits 16 + 4 i .. 19 + 4 i, i = 0..3;
+ *   scales: vocab x hidden_dim / group_size of `dtype` (BF16 or F16), row-major.
+ *
+ * quantize: scale = max |w| of the group / 7 rounded to `dtype`, q = w / scale
+ * rounded to nearest (ties to even) and clamped; a group of zeros has scale 0
+ * and codes 0, one with a NaN or infinite weight (or whose scale overflows) that
+ * scale and codes 0.  weight: vocab x hidden_dim of `dtype`, 16-byte aligned. */
+CID_API int cid_lm_head_quantize(cid_dtype_t dtype, const void* weight, int64_t vocab,
+                        int64_t hidden_dim, int group_size, uint32_t* packed, void* scales,
+                        void* stream);
+
+/* weight = scale * q, rounded to `dtype`. */
+CID_API int cid_lm_head_dequantize(cid_dtype_t dtype, const uint32_t* packed, const void* scales,
+                        int64_t vocab, int64_t hidden_dim, int group_size, void* weight,
+                        void* stream);
+
+/* logits = hidden @ (scale * q)^T: hidden rows x hidden_dim of `dtype` (the
+ * scales' type), 16-byte aligned; each group's sum of q * hidden is accumulated
+ * in f32 on the tcgen05 tensor cores and scaled in f32; logits rows x vocab of
+ * `dtype`, rounded once.  Waits inside the kernel are bounded; one that runs
+ * out sets CID_STATUS_LM_HEAD_TIMEOUT. */
+CID_API int cid_lm_head_quantized_logits(cid_dtype_t dtype, const void* hidden, int64_t rows,
+                        int64_t hidden_dim, const uint32_t* packed, const void* scales,
+                        int group_size, int64_t vocab, void* logits, uint32_t* status,
+                        void* stream);
+
+/* Workspace bytes cid_lm_head_quantized_display_statistics needs. */
+CID_API size_t cid_lm_head_quantized_workspace_bytes(int64_t rows, int64_t vocab);
+
+/* cid_display_token_statistics over those logits without writing them: in f32,
+ * each rounded to bf16 first when round_bf16 != 0. */
+CID_API int cid_lm_head_quantized_display_statistics(cid_dtype_t dtype, const void* hidden,
+                        int64_t rows, int64_t hidden_dim, const uint32_t* packed,
+                        const void* scales, int group_size, int64_t vocab,
+                        const int64_t* token_ids, int round_bf16, float* confidence,
+                        int64_t* predicted, float* current_confidence, void* workspace,
+                        size_t workspace_bytes, uint32_t* status, void* stream);
+
+/* ---------------------------------------------------------------------- */
 /* Peer record exchange (no reference counterpart: the multi-GPU form of   */
 /* the vocabulary-parallel statistics, csrc/ops.cpp:446-474 sharded).      */
 /* ---------------------------------------------------------------------- */

@@ -124,3 +124,120 @@ def test_loss_c_abi_checks(lib: ctypes.CDLL) -> None:
     assert back(rows=0, gw=0) == OK
     assert back(lse=0) == INVALID
     assert back(bytes_=need(4, 64, 300, 1) - 1) == SCRATCH
+
+
+def _packed(device="cpu", dtype=torch.bfloat16, vocab=100, dim=128, group=64):
+    return (torch.zeros(vocab, dim // 8, dtype=torch.int32, device=device),
+            torch.zeros(vocab, dim // group, dtype=dtype, device=device))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_int4_shapes_on_meta(dtype, group) -> None:
+    w = torch.zeros(100, 256, dtype=dtype, device="meta")
+    head = cid_engine.lm_head_quantize(w, group_size=group)
+    assert isinstance(head, cid_engine.QuantizedLMHead)
+    assert head.packed.shape == (100, 32) and head.packed.dtype == torch.int32
+    assert head.scales.shape == (100, 256 // group) and head.scales.dtype == dtype
+    assert cid_engine.lm_head_dequantize(*head).shape == (100, 256)
+    h = torch.zeros(3, 5, 256, dtype=dtype, device="meta")
+    z = cid_engine.lm_head_quantized_logits(h, *head)
+    assert z.shape == (3, 5, 100) and z.dtype == dtype
+    ids = torch.zeros(3, 5, dtype=torch.long, device="meta")
+    c, p, u = cid_engine.lm_head_quantized_display_statistics(ids, h, *head)
+    assert c.shape == p.shape == u.shape == (3, 5)
+    assert c.dtype == u.dtype == torch.float32 and p.dtype == torch.int64
+    assert cid_engine.lm_head_quantize(w).scales.shape == (100, 2)
+
+
+def test_int4_refusals() -> None:
+    w = torch.zeros(100, 128, dtype=torch.bfloat16)
+    q = cid_engine.lm_head_quantize
+    with pytest.raises(RuntimeError, match="CUDA devices only"):
+        q(w)
+    with pytest.raises(RuntimeError, match="bfloat16 or torch.float16"):
+        q(w.float())
+    with pytest.raises(RuntimeError, match="32, 64 or 128"):
+        q(w, group_size=16)
+    with pytest.raises(RuntimeError, match="multiple of group_size"):
+        q(w[:, :96], group_size=64)
+    with pytest.raises(RuntimeError, match="non-empty"):
+        q(w[:0])
+    with pytest.raises(RuntimeError, match=r"\[vocab, hidden_dim\]"):
+        q(w[0])
+    packed, scales = _packed()
+    for f in (lambda p, s: cid_engine.lm_head_dequantize(p, s),
+              lambda p, s: cid_engine.lm_head_quantized_logits(
+                  torch.zeros(2, 128, dtype=torch.bfloat16), p, s)):
+        with pytest.raises(RuntimeError, match="CUDA devices only"):
+            f(packed, scales)
+        with pytest.raises(RuntimeError, match="packed must be an int32"):
+            f(packed.long(), scales)
+        with pytest.raises(RuntimeError, match="scales must be"):
+            f(packed, scales.float())
+        with pytest.raises(RuntimeError, match="scales must be"):
+            f(packed, scales[:50])
+        with pytest.raises(RuntimeError, match="groups of 32, 64 or 128"):
+            f(packed, torch.zeros(100, 8, dtype=torch.bfloat16))
+        with pytest.raises(RuntimeError, match="groups of 32, 64 or 128"):
+            f(packed, scales[:, :0])
+        with pytest.raises(RuntimeError, match="non-empty"):
+            f(packed[:0], scales[:0])
+    h = torch.zeros(2, 128, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="share a dtype"):
+        cid_engine.lm_head_quantized_logits(h.half(), packed, scales)
+    with pytest.raises(RuntimeError, match=r"\[\*, hidden_dim\]"):
+        cid_engine.lm_head_quantized_logits(h[:, :64], packed, scales)
+    s = cid_engine.lm_head_quantized_display_statistics
+    ids = torch.zeros(2, dtype=torch.long)
+    with pytest.raises(RuntimeError, match="CUDA devices only"):
+        s(ids, h, packed, scales)
+    with pytest.raises(RuntimeError, match="torch.int64"):
+        s(ids.int(), h, packed, scales)
+    with pytest.raises(RuntimeError, match=r"\[\*token_ids.shape, hidden_dim\]"):
+        s(ids[:1], h, packed, scales)
+
+
+def test_int4_c_abi_checks(lib: ctypes.CDLL) -> None:
+    i64, p, null, size = ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p(0), ctypes.c_size_t
+    lib.cid_lm_head_quantized_workspace_bytes.restype = size
+
+    def quantize(dtype=BF16, w=0x1000, vocab=100, dim=128, group=64, out=0x2000, sc=0x3000):
+        return lib.cid_lm_head_quantize(dtype, p(w), i64(vocab), i64(dim), ctypes.c_int(group),
+                                        p(out), p(sc), null)
+
+    def dequantize(dtype=BF16, w=0x1000, vocab=100, dim=128, group=64, out=0x2000, sc=0x3000):
+        return lib.cid_lm_head_dequantize(dtype, p(out), p(sc), i64(vocab), i64(dim),
+                                          ctypes.c_int(group), p(w), null)
+
+    for f in (quantize, dequantize):
+        assert f(dtype=F32) == DTYPE
+        for bad in (dict(vocab=0), dict(vocab=2**31), dict(dim=0), dict(dim=96), dict(group=16),
+                    dict(group=0), dict(dim=-64), dict(vocab=2**30, dim=2**30)):
+            assert f(**bad) == INVALID, bad
+        assert f(w=0x1008) == MISALIGNED and f(out=0x2004) == MISALIGNED and f(sc=0x3001) == MISALIGNED
+        assert f(w=0) == INVALID and f(out=0) == INVALID and f(sc=0) == INVALID
+
+    def logits(dtype=BF16, rows=2, h=0x1000, dim=128, group=64, vocab=100, out=0x5000):
+        return lib.cid_lm_head_quantized_logits(dtype, p(h), i64(rows), i64(dim), p(0x2000),
+                                                p(0x3000), ctypes.c_int(group), i64(vocab), p(out),
+                                                null, null)
+
+    assert logits(dtype=F32) == DTYPE and logits(rows=-1) == INVALID and logits(dim=100) == INVALID
+    assert logits(rows=2**31) == INVALID and logits(h=0x1002) == MISALIGNED
+    assert logits(out=0x5001) == MISALIGNED and logits(rows=0) == OK
+    assert logits(h=0) == INVALID and logits(out=0) == INVALID
+    need = lib.cid_lm_head_quantized_workspace_bytes(i64(2), i64(300))
+    assert need == 3 * 2 * 16
+    for bad in ((0, 300), (-1, 300), (2, 0), (2, 2**31)):
+        assert lib.cid_lm_head_quantized_workspace_bytes(i64(bad[0]), i64(bad[1])) == 0
+
+    def stats(ids=0x4000, ws=0x6000, bytes_=need, rows=2):
+        return lib.cid_lm_head_quantized_display_statistics(
+            BF16, p(0x1000), i64(rows), i64(128), p(0x2000), p(0x3000), ctypes.c_int(64),
+            i64(300), p(ids), ctypes.c_int(1), p(0x5000), p(0x5100), p(0x5200), p(ws),
+            size(bytes_), null, null)
+
+    assert stats(ids=0x4004) == MISALIGNED and stats(ws=0x6008) == MISALIGNED
+    assert stats(ids=0) == INVALID and stats(ws=0) == INVALID and stats(rows=0) == OK
+    assert stats(bytes_=need - 1) == SCRATCH
