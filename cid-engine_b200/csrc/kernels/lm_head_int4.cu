@@ -22,8 +22,8 @@
 // which tcgen05.mma takes as its A operand; hidden rows are B (N = 16 to 64
 // columns of the accumulator).  q is exact in 16 bits and the scale is applied
 // in f32 to each group's sum when it is read back from TMEM, so nothing is
-// rounded between the inputs and the f32 result.  Two warpgroups take turns:
-// one's MMAs run while the other unpacks.
+// rounded between the inputs and the f32 result.  Unpacking, MMAs and read-back
+// are warpgroups of their own, joined by rings of TMEM buffers.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -37,52 +37,50 @@
 namespace cid {
 namespace {
 
-constexpr int kTileV = 128;       // weight rows of a tile: UMMA M, one a thread
+constexpr int kTileV = 128;       // weight rows of an accumulator: UMMA M, one a thread
 constexpr int kChunk = 128;       // columns a warpgroup unpacks at a time
-constexpr int kStageK = 256;      // columns of a stage: a chunk for each warpgroup
+constexpr int kStageK = 256;      // columns of a stage: two chunks
 constexpr int kUmmaK = 16;
-constexpr uint32_t kStageW = kTileV * kStageK / 2;  // 16 KiB of codes
+constexpr uint32_t kStageW = kTileV * kStageK / 2;  // 16 KiB of codes for 128 weight rows
 constexpr int kChunkCols = kChunk / 2;              // TMEM columns of a chunk of A
 constexpr int kMaxStages = 8;
-constexpr int kThreads = 384;  // warp 0 TMA, warp 1 MMA, warps 2-3 idle, warps 4-11 two warpgroups
 constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kDRegion = kTmemCols - 4 * kChunkCols;  // columns left for accumulators
 constexpr int kMaxParts = 256;  // vocabulary parts of the statistics: record combine limit
+constexpr int kXchPitch = kTileV + 2;  // floats between hidden rows of a transposed tile
+constexpr size_t kSmemLimit = 227 * 1024;
 
 struct Int4Params {
   int64_t rows, vocab;
-  int64_t groups;       // scales a weight row
-  int64_t stages_k;     // stages a tile: ceil(H / kStageK)
-  int64_t tiles;        // weight tiles
-  int64_t parts;        // vocabulary parts, one a CTA
-  int64_t row_blocks;   // blocks of the kernel's N rows
+  int64_t groups;      // scales a weight row
+  int stages_k;        // stages a tile: ceil(H / kStageK)
+  int64_t tiles;       // tiles of R * kTileV weight rows
+  int64_t parts;       // vocabulary parts, one a CTA
+  int64_t row_blocks;  // blocks of the kernel's N rows
   const void* scales;
-  void* out;            // logits [rows][vocab], or NULL
+  void* out;                    // logits [rows][vocab], or NULL
   cid_shard_record_t* records;  // statistics: [parts][rows]
   const int64_t* ids;
   uint32_t* status;
   int round_bf16;
-  int stages;           // shared-memory stages
+  int stages;  // shared-memory stages
 };
 
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 
-// Stores 64 registers to 64 consecutive columns of this thread's TMEM lane.
-__device__ __forceinline__ void tmem_store64(uint32_t taddr, const uint32_t (&r)[64]) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const uint32_t* q = r + 32 * h;
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,"
-        "%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(
-            taddr + 32 * h),
-        "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3]), "r"(q[4]), "r"(q[5]), "r"(q[6]), "r"(q[7]),
-        "r"(q[8]), "r"(q[9]), "r"(q[10]), "r"(q[11]), "r"(q[12]), "r"(q[13]), "r"(q[14]),
-        "r"(q[15]), "r"(q[16]), "r"(q[17]), "r"(q[18]), "r"(q[19]), "r"(q[20]), "r"(q[21]),
-        "r"(q[22]), "r"(q[23]), "r"(q[24]), "r"(q[25]), "r"(q[26]), "r"(q[27]), "r"(q[28]),
-        "r"(q[29]), "r"(q[30]), "r"(q[31])
-        : "memory");
-  }
+// Stores 32 registers to 32 consecutive columns of this thread's TMEM lane.
+__device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t* q) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,"
+      "%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(
+          taddr),
+      "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3]), "r"(q[4]), "r"(q[5]), "r"(q[6]), "r"(q[7]),
+      "r"(q[8]), "r"(q[9]), "r"(q[10]), "r"(q[11]), "r"(q[12]), "r"(q[13]), "r"(q[14]),
+      "r"(q[15]), "r"(q[16]), "r"(q[17]), "r"(q[18]), "r"(q[19]), "r"(q[20]), "r"(q[21]),
+      "r"(q[22]), "r"(q[23]), "r"(q[24]), "r"(q[25]), "r"(q[26]), "r"(q[27]), "r"(q[28]),
+      "r"(q[29]), "r"(q[30]), "r"(q[31])
+      : "memory");
 }
 
 __device__ __forceinline__ void tmem_wait_store() {
@@ -111,6 +109,15 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
       : "memory");
 }
 
+// {a0, a1} += {x0, x1} * {b, b}
+__device__ __forceinline__ void scale_add2(float& a0, float& a1, uint32_t x0, uint32_t x1,
+                                           float b) {
+  asm("{\n .reg .b64 ra, rx, rb;\n mov.b64 ra, {%0, %1};\n mov.b64 rx, {%2, %3};\n"
+      " mov.b64 rb, {%4, %4};\n fma.rn.f32x2 ra, rx, rb, ra;\n mov.b64 {%0, %1}, ra;\n}"
+      : "+f"(a0), "+f"(a1)
+      : "r"(x0), "r"(x1), "f"(b));
+}
+
 // The four pairs of columns of a word of codes as 16-bit pairs.
 template <typename T>
 __device__ __forceinline__ void unpack8(uint32_t w, uint32_t* out) {
@@ -132,62 +139,88 @@ __device__ __forceinline__ void unpack8(uint32_t w, uint32_t* out) {
   }
 }
 
-// Running statistics of one hidden row over the columns a lane has seen.
-struct LaneState {
+// Running statistics of one hidden row over the columns a thread has seen.
+struct RowStats {
   float m, s;
-  int where, nan;
+  int where, nan;  // first column of the maximum, first NaN column; -1: none
 };
 
-__device__ __forceinline__ void lane_merge(LaneState& a, float m, float s, int where, int nan) {
-  if (m > a.m || (m == a.m && where >= 0 && (a.where < 0 || where < a.where))) a.where = where;
-  const float nm = fmaxf(a.m, m);
-  const float off = nm == -INFINITY ? 0.0f : nm * kLog2e;
-  a.s = a.s * ex2(fmaf(a.m, kLog2e, -off)) + s * ex2(fmaf(m, kLog2e, -off));
-  a.m = nm;
-  if (nan >= 0 && (a.nan < 0 || nan < a.nan)) a.nan = nan;
+__device__ __forceinline__ void merge_stats(RowStats& a, const RowStats& b) {
+  if (b.m > a.m || (b.m == a.m && b.where >= 0 && (a.where < 0 || b.where < a.where)))
+    a.where = b.where;
+  const float m = fmaxf(a.m, b.m);
+  if (m == -INFINITY) {
+    a.s += b.s;  // nothing, or NaN
+  } else {
+    // the difference first: a side that keeps its maximum keeps its sum exactly
+    a.s = a.s * ex2((a.m - m) * kLog2e) + b.s * ex2((b.m - m) * kLog2e);
+  }
+  a.m = m;
+  if (b.nan >= 0 && (a.nan < 0 || b.nan < a.nan)) a.nan = b.nan;
 }
 
+// Roles of a CTA: warps 0-3 control (0 TMA, 1 MMA), then R warpgroups that read
+// the accumulators back, then two that unpack.
+__host__ __device__ constexpr int int4_threads(int r) { return 128 * (3 + r); }
+
 // N: hidden rows of a pass (accumulator columns); S: groups in a chunk of 128
-// columns, each with an accumulator of its own.
-template <typename T, int N, int S>
-__global__ void __launch_bounds__(kThreads, 1)
+// columns, each with an accumulator of its own; R: blocks of 128 weight rows a
+// tile; kResident: the hidden rows stay in shared memory for the whole pass
+// (otherwise their slices travel with the codes).
+//
+// Chunks are numbered q along the CTA's work: for every stage its two halves of
+// 128 columns, and for each the tile's R row blocks.  Unpacking warpgroup q & 1
+// fills A buffer (q & 1, (q >> 1) & 1); the accumulators form a ring.
+template <typename T, int N, int S, int R, bool kResident>
+__global__ void __launch_bounds__(int4_threads(R), 1)
     int4_head_kernel(const __grid_constant__ CUtensorMap map_w,
                      const __grid_constant__ CUtensorMap map_h, Int4Params p) {
   constexpr int kDCols = N * S;
-  constexpr int kDBufs = kDCols <= 64 ? 2 : 1;  // accumulators of a warpgroup
-  static_assert(kDCols <= 128 && 2 * 2 * kChunkCols + 2 * kDBufs * kDCols <= int(kTmemCols),
-                "A chunks and accumulators share TMEM");
-  constexpr uint32_t kStageH = N * kStageK * 2;
-  constexpr uint32_t kStage = kStageW + kStageH;
+  constexpr int kDBufs = int(kDRegion) / kDCols < 4 ? int(kDRegion) / kDCols : 4;
+  static_assert(kDBufs == 4 || kDBufs == 2, "the accumulator ring is a power of two");
+  constexpr uint32_t kStage = R * kStageW + (kResident ? 0u : uint32_t(N) * kStageK * 2);
   constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   constexpr uint32_t kDesc = (1u << 4) | (kType << 7) | (kType << 10) |
                              (uint32_t(N >> 3) << 17) | (uint32_t(kTileV >> 4) << 24);
+  constexpr int kPer = kTileV / N;  // threads of a warpgroup that keep one hidden row's statistics
 
   extern __shared__ unsigned char smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   unsigned char* smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
   const int stages = p.stages;
   unsigned char* stage0 = smem;
-  float* xch = reinterpret_cast<float*>(smem + stages * kStage);  // [N][kTileV]
-  uint64_t* full = reinterpret_cast<uint64_t*>(xch + N * kTileV);
+  unsigned char* resident = smem + stages * kStage;  // [2 * chunks][N][64] of the hidden rows
+  float* xch = reinterpret_cast<float*>(
+      resident + (kResident ? size_t(p.stages_k) * (N * kStageK * 2) : 0));  // [R][N][kXchPitch]
+  uint64_t* full = reinterpret_cast<uint64_t*>(xch + R * N * kXchPitch);
   uint64_t* empty = full + kMaxStages;
-  uint64_t* a_full = empty + kMaxStages;  // [2 warpgroups][2]
-  uint64_t* d_full = a_full + 4;          // [2 warpgroups][2]
-  uint64_t* joined = d_full + 4;          // the eight unpacking warps meet
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(joined + 1);
+  uint64_t* a_full = empty + kMaxStages;  // [warpgroup][2]
+  uint64_t* a_empty = a_full + 4;
+  uint64_t* d_full = a_empty + 4;         // [kDBufs]
+  uint64_t* d_empty = d_full + 4;
+  uint64_t* h_full = d_empty + 4;
+  uint64_t* h_empty = h_full + 1;
+  uint64_t* joined = h_empty + 1;         // [R]: a read-back warpgroup's warps meet
+  uint64_t* joined_all = joined + 2;      // all of them
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(joined_all + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 2 * 4 + 1);  // the unpacking warps' reads and the MMAs'
+      mbar_init(&empty[s], kResident ? 8 : 9);  // the unpacking warps', and the MMAs' of hidden
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&a_full[i], 4);
+      mbar_init(&a_empty[i], 1);
       mbar_init(&d_full[i], 1);
+      mbar_init(&d_empty[i], 4);
     }
-    mbar_init(joined, 8);
+    mbar_init(h_full, 1);
+    mbar_init(h_empty, 1);
+    for (int i = 0; i < R; ++i) mbar_init(&joined[i], 4);
+    mbar_init(joined_all, 4 * R);
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -206,7 +239,19 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const int64_t part = blockIdx.x;
   const int64_t t0 = part * p.tiles / p.parts, t1 = (part + 1) * p.tiles / p.parts;
-  const int64_t turns = p.row_blocks * (t1 - t0);  // tiles this CTA runs through
+  const int chunks = 2 * p.stages_k;  // of 128 columns, each R row blocks
+
+  // A bounded wait of a whole warp; false when it ran out or another role did.
+  auto warp_wait = [&](uint64_t* bar, uint32_t parity) {
+    const bool got = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, kWaitNs));
+    if (!got && lane == 0 && !*abort) raise_abort(abort, p.status);
+    return got;
+  };
+  auto thread_wait = [&](uint64_t* bar, uint32_t parity) {
+    const bool got = mbar_wait(bar, parity, abort, kWaitNs);
+    if (!got && !*abort) raise_abort(abort, p.status);
+    return got;
+  };
 
   if (warp == 0) {
     if (lane == 0) {
@@ -214,32 +259,45 @@ __global__ void __launch_bounds__(kThreads, 1)
       int s = 0;
       uint32_t ph = 0, issued = 0, issue_par = 0;
       bool ok = true;
-      for (int64_t i = 0; ok && i < turns; ++i) {
-        const int64_t rb = i / (t1 - t0), t = t0 + i % (t1 - t0);
-        for (int64_t k = 0; k < p.stages_k; ++k) {
-          if (!mbar_wait(&empty[s], ph ^ 1u, abort, kWaitNs)) {
-            if (!*abort) raise_abort(abort, p.status);
-            ok = false;
-            break;
-          }
-          mbar_expect_tx(&full[s], kStage);
-          unsigned char* w = stage0 + s * kStage;
-          tma_load_2d(w, &map_w, static_cast<int32_t>(k * (kStageK / 4)),
-                      static_cast<int32_t>(t * kTileV), &full[s]);
-          for (int b = 0; b < kStageK / 64; ++b)
-            tma_load_2d(w + kStageW + b * (N * 128), &map_h,
-                        static_cast<int32_t>(k * kStageK + b * 64), static_cast<int32_t>(rb * N),
-                        &full[s]);
-          issued |= 1u << s;
-          issue_par = (issue_par & ~(1u << s)) | (ph << s);
-          if (++s == stages) {
-            s = 0;
-            ph ^= 1u;
+      int64_t h_loads = 0;
+      for (int64_t rb = 0; ok && rb < p.row_blocks; ++rb) {
+        if (kResident) {
+          if (rb > 0 && !thread_wait(h_empty, static_cast<uint32_t>(rb - 1) & 1u)) break;
+          mbar_expect_tx(h_full, static_cast<uint32_t>(p.stages_k) * (N * kStageK * 2));
+          for (int b = 0; b < p.stages_k * (kStageK / 64); ++b)
+            tma_load_2d(resident + b * (N * 128), &map_h, b * 64, static_cast<int32_t>(rb * N),
+                        h_full);
+          ++h_loads;
+        }
+        for (int64_t t = t0; ok && t < t1; ++t) {
+          for (int k = 0; k < p.stages_k; ++k) {
+            if (!thread_wait(&empty[s], ph ^ 1u)) {
+              ok = false;
+              break;
+            }
+            mbar_expect_tx(&full[s], kStage);
+            unsigned char* w = stage0 + s * kStage;
+            for (int r = 0; r < R; ++r)
+              tma_load_2d(w + r * kStageW, &map_w, k * (kStageK / 4),
+                          static_cast<int32_t>((t * R + r) * kTileV), &full[s]);
+            if (!kResident)
+              for (int b = 0; b < kStageK / 64; ++b)
+                tma_load_2d(w + R * kStageW + b * (N * 128), &map_h, k * kStageK + b * 64,
+                            static_cast<int32_t>(rb * N), &full[s]);
+            issued |= 1u << s;
+            issue_par = (issue_par & ~(1u << s)) | (ph << s);
+            if (++s == stages) {
+              s = 0;
+              ph ^= 1u;
+            }
           }
         }
       }
+      // copies in flight land before the CTA exits (immediate unless aborted)
       for (int i = 0; i < stages; ++i)
         if (issued & (1u << i)) mbar_wait(&full[i], (issue_par >> i) & 1u, nullptr, kDrainNs);
+      if (h_loads > 0)
+        mbar_wait(h_full, static_cast<uint32_t>(h_loads - 1) & 1u, nullptr, kDrainNs);
     }
   } else if (warp == 1) {
     if (lane == 0) {
@@ -249,259 +307,304 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint64_t* last_bar = nullptr;
       uint32_t last_par = 0;
       bool ok = true;
-      int64_t n = 0;  // stages so far: the chunk count of each warpgroup
-      for (int64_t i = 0; ok && i < turns * p.stages_k; ++i, ++n) {
-        const uint32_t b0 = smem_u32(stage0 + s * kStage + kStageW);
-        const int ab = static_cast<int>(n & 1);
-        const uint32_t par = static_cast<uint32_t>(n >> 1) & 1u;
-        if (!mbar_wait(&full[s], ph, abort, kWaitNs)) {
-          if (!*abort) raise_abort(abort, p.status);
-          break;
-        }
-        for (int wg = 0; wg < 2; ++wg) {
-          // the codes of this chunk are in TMEM, and the accumulator it will use
-          // has been read
-          if (!mbar_wait(&a_full[wg * 2 + ab], par, abort, kWaitNs)) {
-            if (!*abort) raise_abort(abort, p.status);
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t a = tmem_base + static_cast<uint32_t>((wg * 2 + ab) * kChunkCols);
-          const uint32_t d =
-              d_base + static_cast<uint32_t>((wg * kDBufs + (kDBufs == 2 ? ab : 0)) * kDCols);
+      uint32_t q = 0;  // chunk number; its barriers' parities need its low bits only
+      for (int64_t rb = 0; ok && rb < p.row_blocks; ++rb) {
+        if (kResident && !thread_wait(h_full, static_cast<uint32_t>(rb) & 1u)) break;
+        for (int64_t t = t0; ok && t < t1; ++t) {
+          for (int k = 0; ok && k < p.stages_k; ++k) {
+            // the codes reach this role through TMEM; with resident hidden rows a
+            // stage is refilled without it and its barrier must not be waited for
+            if (!kResident && !thread_wait(&full[s], ph)) {
+              ok = false;
+              break;
+            }
+            const uint32_t b0 = kResident ? smem_u32(resident + size_t(k) * (N * kStageK * 2))
+                                          : smem_u32(stage0 + s * kStage + R * kStageW);
+            for (int c = 0; c < 2 * R; ++c, ++q) {
+              const uint32_t ab = (q & 1u) * 2 + ((q >> 1) & 1u), db = q % kDBufs;
+              if (!thread_wait(&a_full[ab], (q >> 2) & 1u) ||
+                  !thread_wait(&d_empty[db], (q / kDBufs & 1u) ^ 1u)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+              const uint32_t a = tmem_base + ab * kChunkCols, d = d_base + db * kDCols;
+              const uint32_t bh = b0 + (c / R) * (2 * N * 128);
 #pragma unroll
-          for (int kk = 0; kk < kChunk / kUmmaK; ++kk) {
-            constexpr int per = kChunk / kUmmaK / S;  // MMAs of a group
-            const uint64_t bd = sw128_desc(b0 + (wg * 2 + kk / 4) * (N * 128) + (kk % 4) * 32);
-            umma_f16_ts(d + (kk / per) * N, a + kk * (kUmmaK / 2), bd, kDesc,
-                        kk % per != 0 ? 1u : 0u);
+              for (int kk = 0; kk < kChunk / kUmmaK; ++kk) {
+                constexpr int per = kChunk / kUmmaK / S;  // MMAs of a group
+                umma_f16_ts(d + (kk / per) * N, a + kk * (kUmmaK / 2),
+                            sw128_desc(bh + (kk / 4) * (N * 128) + (kk % 4) * 32), kDesc,
+                            kk % per != 0 ? 1u : 0u);
+              }
+              umma_commit(&a_empty[ab]);
+              umma_commit(&d_full[db]);
+              last_bar = &d_full[db];
+              last_par = q / kDBufs & 1u;
+            }
+            if (!ok) break;
+            if (!kResident) umma_commit(&empty[s]);
+            if (++s == stages) {
+              s = 0;
+              ph ^= 1u;
+            }
           }
-          umma_commit(&d_full[wg * 2 + ab]);
-          last_bar = &d_full[wg * 2 + ab];
-          last_par = par;
         }
-        if (!ok) break;
-        umma_commit(&empty[s]);
-        if (++s == stages) {
-          s = 0;
-          ph ^= 1u;
-        }
+        if (kResident && ok) umma_commit(h_empty);
       }
+      // MMAs in flight finish before the TMEM is freed (immediate unless aborted)
       if (last_bar != nullptr) mbar_wait(last_bar, last_par, nullptr, kDrainNs);
     }
-  } else if (warp >= 4) {
-    // ---------------- two warpgroups: thread = weight row ----------------
-    const int wg = (warp - 4) >> 2, quarter = warp & 3;
+  } else if (warp >= 4 + 4 * R) {
+    // ---------------- unpacking: thread = weight row ----------------
+    const int wg = (warp - 4 - 4 * R) >> 2, quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
-    const T* scales = static_cast<const T*>(p.scales);
     int s = 0;
-    uint32_t ph = 0;
-    int64_t n = 0;  // chunks of this warpgroup so far
+    uint32_t ph = 0, n = 0;  // n: chunks of this warpgroup so far, q = 2 n + wg
     bool ok = true;
-    constexpr int kOwn = (N + 7) / 8;  // hidden rows whose statistics a warp keeps
-    LaneState st[kOwn];
-    float cur[kOwn];
-
-    float acc[N];
-    // adds the sums of chunk c (stage k of the tile of row v) to acc
-    auto drain = [&](int64_t c, const float (&sc)[S]) {
-      const int ab = static_cast<int>(c & 1);
-      bool got = mbar_wait(&d_full[wg * 2 + ab], static_cast<uint32_t>(c >> 1) & 1u, abort,
-                           kWaitNs);
-      got = __all_sync(0xffffffffu, got);
-      if (!got) {
-        if (lane == 0 && !*abort) raise_abort(abort, p.status);
-        return false;
-      }
-      tc_fence_after();
-      const uint32_t d = d_base + lane_off +
-                         static_cast<uint32_t>((wg * kDBufs + (kDBufs == 2 ? ab : 0)) * kDCols);
+    const int64_t total = p.row_blocks * (t1 - t0) * p.stages_k;
+    for (int64_t i = 0; ok && i < total; ++i) {
+      if (!warp_wait(&full[s], ph)) break;
+      const unsigned char* row = stage0 + s * kStage + (R == 2 ? wg * kStageW : 0) + r * 128;
 #pragma unroll
-      for (int g = 0; g < S; ++g)
+      for (int c = 0; c < R; ++c, ++n) {  // R == 1: half wg of the stage; R == 2: both halves
+        const int half = R == 1 ? wg : c;
+        uint4 w[4];
 #pragma unroll
-        for (int j = 0; j < N; j += 16) {
-          uint32_t x[16];
-          tmem_load16(d + static_cast<uint32_t>(g * N + j), x);
-#pragma unroll
-          for (int q = 0; q < 16; ++q) acc[j + q] = fmaf(__uint_as_float(x[q]), sc[g], acc[j + q]);
+        for (int j = 0; j < 4; ++j)
+          w[j] = *reinterpret_cast<const uint4*>(row + (((half * 4 + j) ^ (r & 7)) << 4));
+        if (c == R - 1) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&empty[s]);
         }
-      tc_fence_before();
-      return true;
-    };
-
-    uint32_t join_par = 0;
-    auto join = [&]() {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(joined);
-      bool got = mbar_wait(joined, join_par, abort, kWaitNs);
-      got = __all_sync(0xffffffffu, got);
-      join_par ^= 1u;
-      if (!got && lane == 0 && !*abort) raise_abort(abort, p.status);
-      return got;
-    };
-
-    for (int64_t i = 0; ok && i < turns; ++i) {
-      const int64_t rb = i / (t1 - t0), ti = i % (t1 - t0), t = t0 + ti;
-      const int64_t v = t * kTileV + r;
-      const bool valid = v < p.vocab;
-      if (ti == 0) {
-#pragma unroll
-        for (int j = 0; j < kOwn; ++j) {
-          st[j] = LaneState{-INFINITY, 0.0f, -1, -1};
-          cur[j] = 0.0f;
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < N; ++j) acc[j] = 0.0f;
-      float sc_prev[S];
-      for (int64_t k = 0; k < p.stages_k; ++k, ++n) {
-        float sc[S];
-#pragma unroll
-        for (int g = 0; g < S; ++g) {
-          const int64_t gi = (k * 2 + wg) * S + g;
-          sc[g] = valid && gi < p.groups ? to_float(scales[v * p.groups + gi]) : 0.0f;
-        }
-        bool got = mbar_wait(&full[s], ph, abort, kWaitNs);
-        got = __all_sync(0xffffffffu, got);
-        if (!got) {
-          if (lane == 0 && !*abort) raise_abort(abort, p.status);
+        const uint32_t ab = static_cast<uint32_t>(wg) * 2 + (n & 1u);
+        if (!warp_wait(&a_empty[ab], (n >> 1 & 1u) ^ 1u)) {
           ok = false;
           break;
         }
-        const unsigned char* row = stage0 + s * kStage + r * 128;
-        uint32_t a[64];
+        tc_fence_after();
+        const uint32_t dst = tmem_base + lane_off + ab * kChunkCols;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const uint4 w =
-              *reinterpret_cast<const uint4*>(row + (((wg * 4 + c) ^ (r & 7)) << 4));
-          unpack8<T>(w.x, a + c * 16);
-          unpack8<T>(w.y, a + c * 16 + 4);
-          unpack8<T>(w.z, a + c * 16 + 8);
-          unpack8<T>(w.w, a + c * 16 + 12);
+        for (int j = 0; j < 2; ++j) {
+          uint32_t a[32];
+          unpack8<T>(w[2 * j].x, a);
+          unpack8<T>(w[2 * j].y, a + 4);
+          unpack8<T>(w[2 * j].z, a + 8);
+          unpack8<T>(w[2 * j].w, a + 12);
+          unpack8<T>(w[2 * j + 1].x, a + 16);
+          unpack8<T>(w[2 * j + 1].y, a + 20);
+          unpack8<T>(w[2 * j + 1].z, a + 24);
+          unpack8<T>(w[2 * j + 1].w, a + 28);
+          tmem_store32(dst + 32 * j, a);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[s]);
-        if (++s == stages) {
-          s = 0;
-          ph ^= 1u;
-        }
-        // A buffer n & 1 was last read by the MMAs of chunk n - 2, whose sums
-        // have been drained; with one accumulator chunk n - 1's must be too
-        if (kDBufs == 1 && k > 0 && !drain(n - 1, sc_prev)) {
-          ok = false;
-          break;
-        }
-        tmem_store64(tmem_base + lane_off + static_cast<uint32_t>((wg * 2 + (n & 1)) * kChunkCols),
-                     a);
         tmem_wait_store();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&a_full[wg * 2 + (n & 1)]);
-        if (kDBufs == 2 && k > 0 && !drain(n - 1, sc_prev)) {
+        if (lane == 0) mbar_arrive(&a_full[ab]);
+      }
+      if (++s == stages) {
+        s = 0;
+        ph ^= 1u;
+      }
+    }
+  } else if (warp >= 4) {
+    // ---------------- read-back: thread = weight row ----------------
+    const int wg = (warp - 4) >> 2, quarter = warp & 3;
+    const int r = quarter * 32 + lane;
+    const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint16_t* scales = static_cast<const uint16_t*>(p.scales);
+    float* tile_xch = xch + wg * (N * kXchPitch);
+    const int own = r / kPer, sub = r % kPer;  // this thread's hidden row and share of columns
+    uint32_t join_par = 0;
+    auto join = [&](uint64_t* bar, uint32_t par) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+      return warp_wait(bar, par);
+    };
+
+    // The scales of four chunks are loaded while the four before are used.
+    constexpr int kAhead = 4;
+    uint16_t next[kAhead * S], now[kAhead * S];
+    auto load_scales = [&](int64_t v, int kc) {
+#pragma unroll
+      for (int i = 0; i < kAhead * S; ++i) {
+        const int64_t g = static_cast<int64_t>(kc) * S + i;
+        next[i] = v < p.vocab && g < p.groups ? scales[v * p.groups + g] : uint16_t{0};
+      }
+    };
+    auto scale_of = [](uint16_t bits) { return to_float(*reinterpret_cast<const T*>(&bits)); };
+
+    uint32_t q = static_cast<uint32_t>(wg);  // R == 2: every other chunk is this warpgroup's
+    bool ok = true;
+    if (t0 < t1) load_scales((t0 * R + wg) * kTileV + r, 0);
+    for (int64_t rb = 0; ok && rb < p.row_blocks; ++rb) {
+      const int64_t row0 = rb * N;
+      RowStats st{-INFINITY, 0.0f, -1, -1};
+      float cur = 0.0f;
+      const bool live = p.out == nullptr && row0 + own < p.rows;
+      const int64_t id = live ? p.ids[row0 + own] : -1;
+      for (int64_t t = t0; ok && t < t1; ++t) {
+        const int64_t v0 = (t * R + wg) * kTileV, v = v0 + r;
+        float acc[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] = 0.0f;
+        for (int kc = 0; ok && kc < chunks; kc += kAhead) {
+#pragma unroll
+          for (int i = 0; i < kAhead * S; ++i) now[i] = next[i];
+          if (kc + kAhead < chunks)
+            load_scales(v, kc + kAhead);
+          else
+            load_scales(t + 1 < t1 ? v + R * kTileV : (t0 * R + wg) * kTileV + r, 0);
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i) {
+            if (kc + i >= chunks) break;
+            const uint32_t db = q % kDBufs;
+            if (!warp_wait(&d_full[db], q / kDBufs & 1u)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t d = d_base + lane_off + db * kDCols;
+#pragma unroll
+            for (int g = 0; g < S; ++g) {
+              const float sc = scale_of(now[i * S + g]);
+              if (N == 16) {
+                uint32_t x[16];
+                tmem_load16(d + g * N, x);
+#pragma unroll
+                for (int e = 0; e < 16; e += 2)
+                  scale_add2(acc[e], acc[e + 1], x[e], x[e + 1], sc);
+              } else {
+#pragma unroll
+                for (int j = 0; j < N; j += 32) {
+                  uint32_t x[32];
+                  tmem_issue32(d + g * N + j, x);
+                  tmem_wait32(x);
+#pragma unroll
+                  for (int e = 0; e < 32; e += 2)
+                    scale_add2(acc[(j + e) % N], acc[(j + e + 1) % N], x[e], x[e + 1], sc);
+                }
+              }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&d_empty[db]);
+            q += R;
+          }
+        }
+        if (!ok) break;
+        // ---- the tile's logits: 128 weight rows x N hidden rows ----
+        if (p.out != nullptr) {
+          if (v < p.vocab) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+              if (row0 + j >= p.rows) break;
+              T* o = static_cast<T*>(p.out) + (row0 + j) * p.vocab + v;
+              if (std::is_same<T, __nv_bfloat16>::value)
+                *reinterpret_cast<__nv_bfloat16*>(o) = __float2bfloat16_rn(acc[j]);
+              else
+                *reinterpret_cast<__half*>(o) = __float2half_rn(acc[j]);
+            }
+          }
+          continue;
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          float z = acc[j];
+          if (p.round_bf16) z = __bfloat162float(__float2bfloat16_rn(z));
+          tile_xch[j * kXchPitch + r] = v < p.vocab ? z : -INFINITY;
+        }
+        if (!join(&joined[wg], join_par)) {
           ok = false;
           break;
         }
-#pragma unroll
-        for (int g = 0; g < S; ++g) sc_prev[g] = sc[g];
-      }
-      if (!ok || !drain(n - 1, sc_prev)) {
-        ok = false;
-        break;
-      }
-      // ---- the tile's sums: warpgroup 1's halves join warpgroup 0's ----
-      if (wg == 1) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) xch[j * kTileV + r] = acc[j];
-      }
-      if (!join()) break;
-      const int64_t row0 = rb * N;
-      if (wg == 0) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-          float z = acc[j] + xch[j * kTileV + r];
-          if (p.out != nullptr) {
-            if (valid && row0 + j < p.rows) {
-              T* o = static_cast<T*>(p.out) + (row0 + j) * p.vocab + v;
-              if (std::is_same<T, __nv_bfloat16>::value)
-                *reinterpret_cast<__nv_bfloat16*>(o) = __float2bfloat16_rn(z);
-              else
-                *reinterpret_cast<__half*>(o) = __float2half_rn(z);
-            }
-          } else {
-            if (p.round_bf16) z = __bfloat162float(__float2bfloat16_rn(z));
-            xch[j * kTileV + r] = valid ? z : -INFINITY;
-          }
-        }
-      }
-      if (!join()) break;
-      if (p.out == nullptr) {
-        const int w = warp - 4;
-#pragma unroll
-        for (int j = 0; j < kOwn; ++j) {
-          const int nrow = w + j * 8;
-          if (nrow >= N || row0 + nrow >= p.rows) break;
-          const float4 q = *reinterpret_cast<const float4*>(xch + nrow * kTileV + lane * 4);
-          const float x[4] = {q.x, q.y, q.z, q.w};
-          const int c0 = static_cast<int>(t * kTileV) + lane * 4;
-          const int64_t rel = p.ids[row0 + nrow] - c0;
-          float cm = -INFINITY;
-          int cw = -1, cn = -1;
-#pragma unroll
-          for (int e = 3; e >= 0; --e) {
-            if (x[e] >= cm && c0 + e < p.vocab) {
-              cm = x[e];
-              cw = c0 + e;
-            }
-            if (x[e] != x[e]) cn = c0 + e;
-            if (rel == e && c0 + e < p.vocab) cur[j] = x[e];
-          }
-          const float off = cm == -INFINITY ? 0.0f : cm * kLog2e;
-          float cs = 0.0f;
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            cs += x[e] == -INFINITY ? 0.0f : ex2(fmaf(x[e], kLog2e, -off));
-          lane_merge(st[j], cm, cs, cw, cn);
-        }
-        if (ti + 1 == t1 - t0) {
-          // ---- the part's record of each row ----
-#pragma unroll
-          for (int j = 0; j < kOwn; ++j) {
-            const int nrow = w + j * 8;
-            if (nrow >= N || row0 + nrow >= p.rows) break;
-            LaneState a = st[j];
-            float c = cur[j];
-#pragma unroll
-            for (int d = 16; d > 0; d >>= 1) {
-              const float om = __shfl_xor_sync(0xffffffffu, a.m, d);
-              const float os = __shfl_xor_sync(0xffffffffu, a.s, d);
-              const int ow = __shfl_xor_sync(0xffffffffu, a.where, d);
-              const int on = __shfl_xor_sync(0xffffffffu, a.nan, d);
-              const float oc = __shfl_xor_sync(0xffffffffu, c, d);
-              lane_merge(a, om, os, ow, on);
-              c += oc;  // one lane at most has seen the token
-            }
-            if (lane == 0) {
-              cid_shard_record_t rec;
-              rec.max_logit = a.m;
-              const bool special = !(a.m > -INFINITY && a.m < INFINITY) || a.s != a.s;
-              const int first = static_cast<int>(t0 * kTileV);
-              if (special) {
-                const int at = a.nan >= 0 ? a.nan : (a.where >= 0 ? a.where : first);
-                rec.sum_exp = a.m == -INFINITY ? 0.0f : __int_as_float(0x7fffffff);
-                rec.index = at | (a.nan >= 0 ? static_cast<int32_t>(0x80000000u) : 0);
-              } else {
-                rec.sum_exp = a.s;
-                rec.index = a.where;
+        join_par ^= 1u;
+        if (live) {
+          // columns sub, sub + kPer, ... of the tile, in two passes: the
+          // maximum, then the exponentials
+          const float* x = tile_xch + own * kXchPitch + sub;
+          RowStats b{-INFINITY, 0.0f, -1, -1};
+          const int c0 = static_cast<int>(v0) + sub;
+#pragma unroll 4
+          for (int e = 0; e < N; ++e) {
+            const float z = x[e * kPer];
+            const int c = c0 + e * kPer;
+            if (c < p.vocab && (z > b.m || b.where < 0)) {
+              // a first -inf is a maximum too; a first NaN is not
+              if (z == z) {
+                b.m = z;
+                b.where = c;
               }
-              rec.current = c;
-              p.records[part * p.rows + row0 + nrow] = rec;
             }
+            if (z != z && b.nan < 0) b.nan = c;
           }
+          const float off = b.m == -INFINITY ? 0.0f : b.m;
+#pragma unroll 4
+          for (int e = 0; e < N; ++e) {
+            const float z = x[e * kPer];
+            b.s += ex2((z - off) * kLog2e);
+          }
+          merge_stats(st, b);
+          const int64_t rel = id - v0;
+          if (rel >= 0 && rel < kTileV && rel % kPer == sub) cur = x[rel - sub];
+        }
+        if (!join(&joined[wg], join_par)) {  // the tile may be overwritten
+          ok = false;
+          break;
+        }
+        join_par ^= 1u;
+      }
+      if (!ok || p.out != nullptr) continue;
+      // ---- the part's record of each row: over the row's threads, then the warpgroups ----
+#pragma unroll
+      for (int d = 1; d < kPer; d <<= 1) {
+        RowStats o;
+        o.m = __shfl_xor_sync(0xffffffffu, st.m, d);
+        o.s = __shfl_xor_sync(0xffffffffu, st.s, d);
+        o.where = __shfl_xor_sync(0xffffffffu, st.where, d);
+        o.nan = __shfl_xor_sync(0xffffffffu, st.nan, d);
+        merge_stats(st, o);
+        cur += __shfl_xor_sync(0xffffffffu, cur, d);  // one thread at most has seen the token
+      }
+      if (R == 2) {
+        float* slot = xch + N * kXchPitch + own * 8;  // the second warpgroup's tile is free
+        if (wg == 1 && sub == 0) {
+          slot[0] = st.m;
+          slot[1] = st.s;
+          slot[2] = __int_as_float(st.where);
+          slot[3] = __int_as_float(st.nan);
+          slot[4] = cur;
+        }
+        if (!join(joined_all, 0)) {
+          ok = false;
+          break;
+        }
+        if (wg == 0) {
+          const RowStats o{slot[0], slot[1], __float_as_int(slot[2]), __float_as_int(slot[3])};
+          merge_stats(st, o);
+          cur += slot[4];
+        }
+        if (!join(joined_all, 1)) {
+          ok = false;
+          break;
         }
       }
-      if (!join()) break;  // xch is free
+      if (live && wg == 0 && sub == 0) {
+        cid_shard_record_t rec;
+        rec.max_logit = st.m;
+        if (!(st.m > -INFINITY && st.m < INFINITY) || st.s != st.s) {
+          const int first = static_cast<int>(t0 * R * kTileV);
+          const int at = st.nan >= 0 ? st.nan : (st.where >= 0 ? st.where : first);
+          rec.sum_exp = st.m == -INFINITY ? 0.0f : __int_as_float(0x7fffffff);
+          rec.index = at | (st.nan >= 0 ? static_cast<int32_t>(0x80000000u) : 0);
+        } else {
+          rec.sum_exp = st.s;
+          rec.index = st.where;
+        }
+        rec.current = cur;
+        p.records[part * p.rows + row0 + own] = rec;
+      }
     }
   }
 
@@ -588,65 +691,96 @@ __global__ void __launch_bounds__(kQuantThreads)
 
 constexpr int64_t kMaxInt4Rows = INT32_MAX - 64;
 
+
 bool int4_weight_ok(int64_t vocab, int64_t dim, int group) {
   int64_t n = 0;
   return (group == 32 || group == 64 || group == 128) && vocab > 0 &&
-         vocab <= INT32_MAX - kTileV && dim > 0 && dim % group == 0 &&
+         vocab <= INT32_MAX - 2 * kTileV && dim > 0 && dim % group == 0 &&
          dim <= INT32_MAX - kStageK && count_ok(vocab, dim, &n) && n <= kMaxCount &&
          n / (8 * kQuantThreads) < INT32_MAX;
 }
 
-int64_t int4_parts(int64_t vocab) {
-  const int64_t tiles = (vocab + kTileV - 1) / kTileV;
-  int64_t parts = sm_count() < kMaxParts ? sm_count() : kMaxParts;
-  return tiles < parts ? tiles : parts;
-}
+// A launch's shape: R blocks of 128 weight rows a tile, its tiles and its parts
+// (one a CTA).
+struct Int4Plan {
+  int n, r;
+  bool resident;
+  int stages;
+  int64_t tiles, parts;
+};
 
-template <typename T, int N, int S>
-int launch_int4(const CUtensorMap& map_w, const CUtensorMap& map_h, Int4Params p,
-                cudaStream_t stream) {
-  constexpr size_t stage = kStageW + size_t{N} * kStageK * 2;
-  constexpr size_t fixed = size_t{N} * kTileV * 4 + 1024 + 512;
-  constexpr size_t fit = (227 * 1024 - fixed) / stage;
-  p.stages = static_cast<int>(fit < kMaxStages ? fit : kMaxStages);
-  p.row_blocks = (p.rows + N - 1) / N;
-  const size_t smem = p.stages * stage + fixed;
-  const cudaError_t e =
-      cudaFuncSetAttribute(int4_head_kernel<T, N, S>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           static_cast<int>(smem));
-  if (e != cudaSuccess) return record_cuda_error(e);
-  int4_head_kernel<T, N, S>
-      <<<static_cast<unsigned>(p.parts), kThreads, smem, stream>>>(map_w, map_h, p);
-  return launch_result();
+size_t int4_smem(int n, int r, bool resident, int stages, int64_t stages_k) {
+  const size_t hidden = static_cast<size_t>(n) * kStageK * 2;
+  return stages * (r * size_t{kStageW} + (resident ? 0 : hidden)) +
+         (resident ? stages_k * hidden : 0) + static_cast<size_t>(r) * n * kXchPitch * 4 + 1024 +
+         512;
 }
 
 // Hidden rows of a pass: the accumulators of a chunk's groups are at most 64
 // columns wide, so a group of 128 takes up to 64 rows a pass, one of 64 up to
-// 32, one of 32 sixteen; more rows read the weight again.
+// 32, one of 32 sixteen; more rows read the weight again.  The hidden rows stay
+// in shared memory where they leave room for four stages of codes; where they
+// do not, their slices are read again for every tile, and tiles of 256 weight
+// rows halve that traffic.
+Int4Plan int4_plan(int64_t rows, int64_t vocab, int64_t dim, int group) {
+  Int4Plan pl;
+  const int most = group / 2;
+  const int64_t stages_k = (dim + kStageK - 1) / kStageK;
+  pl.n = rows > 32 && most >= 64 ? 64 : (rows > 16 && most >= 32 ? 32 : 16);
+  pl.resident = int4_smem(pl.n, 1, true, 4, stages_k) <= kSmemLimit;
+  pl.r = pl.resident ? 1 : 2;
+  pl.stages = kMaxStages;
+  while (int4_smem(pl.n, pl.r, pl.resident, pl.stages, stages_k) > kSmemLimit) --pl.stages;
+  pl.tiles = (vocab + pl.r * kTileV - 1) / (pl.r * kTileV);
+  pl.parts = sm_count() < kMaxParts ? sm_count() : kMaxParts;
+  if (pl.tiles < pl.parts) pl.parts = pl.tiles;
+  return pl;
+}
+
+template <typename T, int N, int S, int R, bool kResident>
+int launch_int4(const CUtensorMap& map_w, const CUtensorMap& map_h, const Int4Params& p,
+                cudaStream_t stream) {
+  const size_t smem = int4_smem(N, R, kResident, p.stages, p.stages_k);
+  const cudaError_t e = cudaFuncSetAttribute(int4_head_kernel<T, N, S, R, kResident>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             static_cast<int>(smem));
+  if (e != cudaSuccess) return record_cuda_error(e);
+  int4_head_kernel<T, N, S, R, kResident>
+      <<<static_cast<unsigned>(p.parts), int4_threads(R), smem, stream>>>(map_w, map_h, p);
+  return launch_result();
+}
+
+template <typename T, int N, int S>
+int launch_int4(const Int4Plan& pl, const CUtensorMap& map_w, const CUtensorMap& map_h,
+                const Int4Params& p, cudaStream_t stream) {
+  return pl.resident ? launch_int4<T, N, S, 1, true>(map_w, map_h, p, stream)
+                     : launch_int4<T, N, S, 2, false>(map_w, map_h, p, stream);
+}
+
 template <typename T>
 int dispatch_int4(cid_dtype_t dtype, const void* hidden, int64_t dim, const void* packed,
-                  int group, Int4Params p, cudaStream_t stream) {
-  const int most = group / 2;
-  const int n = p.rows > 32 && most >= 64 ? 64 : (p.rows > 16 && most >= 32 ? 32 : 16);
+                  int group, Int4Params p, const Int4Plan& pl, cudaStream_t stream) {
   CUtensorMap map_w, map_h;
   // codes copied as 16-bit elements, four columns each
   int rc = make_map_sw128(&map_w, CID_DTYPE_F16, packed, dim / 4, p.vocab, dim / 4, 64, kTileV);
-  if (rc == CID_OK) rc = make_map_sw128(&map_h, dtype, hidden, dim, p.rows, dim, 64, n);
+  if (rc == CID_OK) rc = make_map_sw128(&map_h, dtype, hidden, dim, p.rows, dim, 64, pl.n);
   if (rc != CID_OK) return rc;
   p.groups = dim / group;
-  p.stages_k = (dim + kStageK - 1) / kStageK;
-  p.tiles = (p.vocab + kTileV - 1) / kTileV;
-  p.parts = int4_parts(p.vocab);
+  p.stages_k = static_cast<int>((dim + kStageK - 1) / kStageK);
+  p.row_blocks = (p.rows + pl.n - 1) / pl.n;
+  p.tiles = pl.tiles;
+  p.parts = pl.parts;
+  p.stages = pl.stages;
   switch (group) {
     case 128:
-      return n == 64   ? launch_int4<T, 64, 1>(map_w, map_h, p, stream)
-             : n == 32 ? launch_int4<T, 32, 1>(map_w, map_h, p, stream)
-                       : launch_int4<T, 16, 1>(map_w, map_h, p, stream);
+      return pl.n == 64   ? launch_int4<T, 64, 1>(pl, map_w, map_h, p, stream)
+             : pl.n == 32 ? launch_int4<T, 32, 1>(pl, map_w, map_h, p, stream)
+                          : launch_int4<T, 16, 1>(pl, map_w, map_h, p, stream);
     case 64:
-      return n == 32 ? launch_int4<T, 32, 2>(map_w, map_h, p, stream)
-                     : launch_int4<T, 16, 2>(map_w, map_h, p, stream);
+      return pl.n == 32 ? launch_int4<T, 32, 2>(pl, map_w, map_h, p, stream)
+                        : launch_int4<T, 16, 2>(pl, map_w, map_h, p, stream);
     default:
-      return launch_int4<T, 16, 4>(map_w, map_h, p, stream);
+      return launch_int4<T, 16, 4>(pl, map_w, map_h, p, stream);
   }
 }
 
@@ -723,15 +857,16 @@ extern "C" int cid_lm_head_quantized_logits(cid_dtype_t dtype, const void* hidde
   p.scales = scales;
   p.out = logits;
   p.status = status;
+  const Int4Plan pl = int4_plan(rows, vocab, hidden_dim, group_size);
   return dtype == CID_DTYPE_F16
-             ? dispatch_int4<__half>(dtype, hidden, hidden_dim, packed, group_size, p,
+             ? dispatch_int4<__half>(dtype, hidden, hidden_dim, packed, group_size, p, pl,
                                      as_stream(stream))
-             : dispatch_int4<__nv_bfloat16>(dtype, hidden, hidden_dim, packed, group_size, p,
+             : dispatch_int4<__nv_bfloat16>(dtype, hidden, hidden_dim, packed, group_size, p, pl,
                                             as_stream(stream));
 }
 
 extern "C" size_t cid_lm_head_quantized_workspace_bytes(int64_t rows, int64_t vocab) {
-  if (rows <= 0 || rows > kMaxInt4Rows || vocab <= 0 || vocab > INT32_MAX - kTileV) return 0;
+  if (rows <= 0 || rows > kMaxInt4Rows || vocab <= 0 || vocab > INT32_MAX - 2 * kTileV) return 0;
   const int64_t tiles = (vocab + kTileV - 1) / kTileV;
   return static_cast<size_t>(tiles < kMaxParts ? tiles : kMaxParts) * static_cast<size_t>(rows) *
          sizeof(cid_shard_record_t);
@@ -765,18 +900,19 @@ extern "C" int cid_lm_head_quantized_display_statistics(
   p.ids = token_ids;
   p.status = status;
   p.round_bf16 = round_bf16 ? 1 : 0;
+  const Int4Plan pl = int4_plan(rows, vocab, hidden_dim, group_size);
   rc = dtype == CID_DTYPE_F16
-           ? dispatch_int4<__half>(dtype, hidden, hidden_dim, packed, group_size, p,
+           ? dispatch_int4<__half>(dtype, hidden, hidden_dim, packed, group_size, p, pl,
                                    as_stream(stream))
-           : dispatch_int4<__nv_bfloat16>(dtype, hidden, hidden_dim, packed, group_size, p,
+           : dispatch_int4<__nv_bfloat16>(dtype, hidden, hidden_dim, packed, group_size, p, pl,
                                           as_stream(stream));
   if (rc != CID_OK) return rc;
   // merge the parts of every row (ascending column ranges) into its statistics
   int64_t offsets[kMaxParts + 1];
-  const int64_t parts = int4_parts(vocab), tiles = (vocab + kTileV - 1) / kTileV;
-  for (int64_t i = 0; i < parts; ++i) offsets[i] = i * tiles / parts * kTileV;
-  offsets[parts] = vocab;
+  for (int64_t i = 0; i < pl.parts; ++i)
+    offsets[i] = i * pl.tiles / pl.parts * (pl.r * kTileV);
+  offsets[pl.parts] = vocab;
   return cid_display_combine_records(static_cast<const cid_shard_record_t*>(workspace),
-                                     static_cast<int>(parts), offsets, token_ids, rows,
+                                     static_cast<int>(pl.parts), offsets, token_ids, rows,
                                      confidence, predicted, current_confidence, status, stream);
 }

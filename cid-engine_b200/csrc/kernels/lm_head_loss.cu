@@ -624,9 +624,12 @@ __global__ void __launch_bounds__(256)
   float m = -INFINITY, s = 0.0f;
   auto merge = [&](float om, float os) {
     const float nm = fmaxf(m, om);
-    const float off = nm == -INFINITY ? 0.0f : nm * kLog2e;
-    // an empty side has s = 0 and m = -inf: its factor is 2^-inf = 0
-    s = s * ex2(fmaf(m, kLog2e, -off)) + os * ex2(fmaf(om, kLog2e, -off));
+    // the difference first: a side that keeps its maximum keeps its sum exactly;
+    // an empty side has s = 0 and m = -inf
+    if (nm == -INFINITY)
+      s += os;
+    else
+      s = s * ex2((m - nm) * kLog2e) + os * ex2((om - nm) * kLog2e);
     m = nm;
   };
   if (slot >= 0)

@@ -156,6 +156,10 @@ SIZES = [
     (130, 2049, 512, 128),  # three passes of 64 rows
     (50, 1500, 1600, 32),   # four passes of 16
     (5, 20000, 2048, 64),   # more tiles than SMs
+    (70, 40000, 512, 128),  # several tiles and passes a CTA
+    (20, 40000, 4096, 128), # hidden rows too many for shared memory
+    (64, 80000, 1536, 128), # the same, several tiles of 256 weight rows a CTA
+    (16, 3000, 8192, 32),
 ]
 
 
