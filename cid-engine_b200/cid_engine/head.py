@@ -105,7 +105,8 @@ def lm_head_quantized_logits(hidden: Tensor, packed: Tensor, scales: Tensor) -> 
     hidden's dtype (the scales' dtype too).  Each group's sum is accumulated
     and scaled in float32; the logits are rounded once.  Made for few rows, up
     to some hundred: the weight is read once for every 64 of them (32 with
-    groups of 64, 16 with groups of 32).  Not differentiable."""
+    groups of 64, 16 with groups of 32).  H is at most 32768.  A hidden row with
+    a NaN or infinite value has NaN logits.  Not differentiable."""
     return torch.ops.cid_engine.lm_head_quantized_logits(hidden, packed, scales)
 
 

@@ -8,22 +8,29 @@
 //   statistics: max softmax probability, argmax and the current token's
 //               probability over z, without writing z
 //
-// Codes are stored as q + 8, eight to a 32-bit word: column 8 j + 2 i at bits
-// 4 i and column 8 j + 2 i + 1 at bits 16 + 4 i of word j.  One shift and one
-// masked OR then give a pair of neighbouring columns in the halves of a
-// register, with the exponent that makes them 128 + q + 8 (bf16) or 1024 + q + 8
-// (fp16); one subtraction leaves q exactly.
+// Codes are stored as c = q + 8, eight to a 32-bit word: column 8 j + 2 i at bits
+// 4 i and column 8 j + 2 i + 1 at bits 16 + 4 i of word j.  Masked where they
+// stand, a word's nibbles 0 and 1 of each half are fp16 numbers as they are:
+// c and 16 c times the smallest subnormal 2^-24.  One shift by 8 brings the
+// other two there, so eight columns cost five integer instructions.
+//
+// The MMAs therefore run in fp16 whatever the hidden rows' type: a first kernel
+// turns each hidden row into fp16 times a power of two that brings its largest
+// value to [2^14, 2^15), with the columns that meet 16 c divided by 16.  A bf16
+// value keeps its 8 bits in fp16's 11 unless it is below 2^-24 of its row's
+// largest (2^-28 where not divided), and then loses less than 2^-35 of that
+// largest, far under the f32 sum's own rounding.  The same kernel leaves 8 sum h
+// of every group, which read-back subtracts: sum c h - 8 sum h = sum q h.
 //
 // Product kernel.  The weight's bytes bound it up to some 64 rows (128256 x
 // 4096: 270 MB, 42 us at the copy peak), so every SM streams weight tiles of
 // 128 rows with TMA, whatever the number of hidden rows.  The contraction runs
-// on the tensor cores with the weight as A: a thread owns one weight row, turns
-// 128 of its codes into 64 registers of 16-bit pairs and stores them to TMEM,
-// which tcgen05.mma takes as its A operand; hidden rows are B (N = 16 to 64
-// columns of the accumulator).  q is exact in 16 bits and the scale is applied
-// in f32 to each group's sum when it is read back from TMEM, so nothing is
-// rounded between the inputs and the f32 result.  Unpacking, MMAs and read-back
-// are warpgroups of their own, joined by rings of TMEM buffers.
+// on the tensor cores with the weight as A: a thread owns one weight row, masks
+// 128 of its codes into 64 registers and stores them to TMEM, which tcgen05.mma
+// takes as its A operand; hidden rows are B (N = 16 to 64 columns of the
+// accumulator).  The scale is applied in f32 to each group's sum when it is read
+// back from TMEM.  Unpacking, MMAs and read-back are warps of their own, joined
+// by rings of TMEM buffers.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -58,6 +65,8 @@ struct Int4Params {
   int64_t parts;       // vocabulary parts, one a CTA
   int64_t row_blocks;  // blocks of the kernel's N rows
   const void* scales;
+  const float* sums;       // 8 sum h: [row blocks][groups][N]
+  const float* row_scale;  // what undoes a hidden row's power of two: [row blocks][N]
   void* out;                    // logits [rows][vocab], or NULL
   cid_shard_record_t* records;  // statistics: [parts][rows]
   const int64_t* ids;
@@ -109,34 +118,23 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
       : "memory");
 }
 
-// {a0, a1} += {x0, x1} * {b, b}
-__device__ __forceinline__ void scale_add2(float& a0, float& a1, uint32_t x0, uint32_t x1,
-                                           float b) {
-  asm("{\n .reg .b64 ra, rx, rb;\n mov.b64 ra, {%0, %1};\n mov.b64 rx, {%2, %3};\n"
-      " mov.b64 rb, {%4, %4};\n fma.rn.f32x2 ra, rx, rb, ra;\n mov.b64 {%0, %1}, ra;\n}"
+// {a0, a1} += ({x0, x1} 2^24 - {s0, s1}) b
+__device__ __forceinline__ void group_add2(float& a0, float& a1, uint32_t x0, uint32_t x1,
+                                           float s0, float s1, float b) {
+  asm("{\n .reg .b64 ra, rx, rb, rs, rk;\n mov.b64 ra, {%0, %1};\n mov.b64 rx, {%2, %3};\n"
+      " mov.b64 rs, {%4, %5};\n mov.b64 rb, {%6, %6};\n mov.b64 rk, {%7, %7};\n"
+      " fma.rn.f32x2 rx, rx, rk, rs;\n fma.rn.f32x2 ra, rx, rb, ra;\n"
+      " mov.b64 {%0, %1}, ra;\n}"
       : "+f"(a0), "+f"(a1)
-      : "r"(x0), "r"(x1), "f"(b));
+      : "r"(x0), "r"(x1), "f"(s0), "f"(s1), "f"(b), "f"(16777216.0f));
 }
 
-// The four pairs of columns of a word of codes as 16-bit pairs.
-template <typename T>
+// The four pairs of columns of a word of codes, c 2^-24 and 16 c 2^-24 in fp16.
 __device__ __forceinline__ void unpack8(uint32_t w, uint32_t* out) {
-  constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
-  constexpr uint32_t magic = bf ? 0x43004300u : 0x64006400u;  // 128 or 1024 in both halves
-  constexpr uint32_t bias = bf ? 0x43084308u : 0x64086408u;   // 136 or 1032
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t t = ((w >> (4 * i)) & 0x000f000fu) | magic;
-    if (bf) {
-      const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&t),
-                                       *reinterpret_cast<const __nv_bfloat162*>(&bias));
-      out[i] = *reinterpret_cast<const uint32_t*>(&v);
-    } else {
-      const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&t),
-                                *reinterpret_cast<const __half2*>(&bias));
-      out[i] = *reinterpret_cast<const uint32_t*>(&v);
-    }
-  }
+  out[0] = w & 0x000f000fu;
+  out[1] = w & 0x00f000f0u;
+  out[2] = (w >> 8) & 0x000f000fu;
+  out[3] = (w >> 8) & 0x00f000f0u;
 }
 
 // Running statistics of one hidden row over the columns a thread has seen.
@@ -159,7 +157,7 @@ __device__ __forceinline__ void merge_stats(RowStats& a, const RowStats& b) {
   if (b.nan >= 0 && (a.nan < 0 || b.nan < a.nan)) a.nan = b.nan;
 }
 
-// Roles of a CTA: warps 0-3 control (0 TMA, 1 MMA), then R warpgroups that read
+// Roles of a CTA: warps 0-3 control (0 codes' TMA, 1 and 2 MMA, 3 hidden rows' TMA), then R warpgroups that read
 // the accumulators back, then two that unpack.
 __host__ __device__ constexpr int int4_threads(int r) { return 128 * (3 + r); }
 
@@ -179,9 +177,9 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
   constexpr int kDBufs = int(kDRegion) / kDCols < 4 ? int(kDRegion) / kDCols : 4;
   static_assert(kDBufs == 4 || kDBufs == 2, "the accumulator ring is a power of two");
   constexpr uint32_t kStage = R * kStageW + (kResident ? 0u : uint32_t(N) * kStageK * 2);
-  constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-  constexpr uint32_t kDesc = (1u << 4) | (kType << 7) | (kType << 10) |
-                             (uint32_t(N >> 3) << 17) | (uint32_t(kTileV >> 4) << 24);
+  // D f32, A and B fp16 (0), both K-major, N >> 3 at bit 17, M >> 4 at bit 24
+  constexpr uint32_t kDesc =
+      (1u << 4) | (uint32_t(N >> 3) << 17) | (uint32_t(kTileV >> 4) << 24);
   constexpr int kPer = kTileV / N;  // threads of a warpgroup that keep one hidden row's statistics
 
   extern __shared__ unsigned char smem_raw[];
@@ -192,7 +190,9 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
   unsigned char* resident = smem + stages * kStage;  // [2 * chunks][N][64] of the hidden rows
   float* xch = reinterpret_cast<float*>(
       resident + (kResident ? size_t(p.stages_k) * (N * kStageK * 2) : 0));  // [R][N][kXchPitch]
-  uint64_t* full = reinterpret_cast<uint64_t*>(xch + R * N * kXchPitch);
+  float* sums = xch + R * N * kXchPitch;  // [groups][N] of -8 sum h, then [N] row scales
+  const int64_t group_slots = static_cast<int64_t>(p.stages_k) * 2 * S;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sums + group_slots * N + N);
   uint64_t* empty = full + kMaxStages;
   uint64_t* a_full = empty + kMaxStages;  // [warpgroup][2]
   uint64_t* a_empty = a_full + 4;
@@ -201,15 +201,16 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
   uint64_t* h_full = d_empty + 4;
   uint64_t* h_empty = h_full + 1;
   uint64_t* joined = h_empty + 1;         // [R]: a read-back warpgroup's warps meet
-  uint64_t* joined_all = joined + 2;      // all of them
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(joined_all + 1);
+  uint64_t* joined_all = joined + 2;      // all of the read-back warps
+  uint64_t* mma_done = joined_all + 1;    // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 2);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], kResident ? 8 : 9);  // the unpacking warps', and the MMAs' of hidden
+      mbar_init(&empty[s], kResident ? 8 : 10);  // the unpacking warps', and the MMA warps' of hidden
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&a_full[i], 4);
@@ -218,7 +219,8 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
       mbar_init(&d_empty[i], 4);
     }
     mbar_init(h_full, 1);
-    mbar_init(h_empty, 1);
+    mbar_init(h_empty, 2);
+    for (int i = 0; i < 2; ++i) mbar_init(&mma_done[i], 1);
     for (int i = 0; i < R; ++i) mbar_init(&joined[i], 4);
     mbar_init(joined_all, 4 * R);
     *abort = 0;
@@ -242,10 +244,14 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
   const int chunks = 2 * p.stages_k;  // of 128 columns, each R row blocks
 
   // A bounded wait of a whole warp; false when it ran out or another role did.
+  // One lane polls: thirty-two take turns at the barrier and slow every role.
   auto warp_wait = [&](uint64_t* bar, uint32_t parity) {
-    const bool got = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, kWaitNs));
-    if (!got && lane == 0 && !*abort) raise_abort(abort, p.status);
-    return got;
+    bool got = true;
+    if (lane == 0) {
+      got = mbar_wait(bar, parity, abort, kWaitNs);
+      if (!got && !*abort) raise_abort(abort, p.status);
+    }
+    return __shfl_sync(0xffffffffu, static_cast<int>(got), 0) != 0;
   };
   auto thread_wait = [&](uint64_t* bar, uint32_t parity) {
     const bool got = mbar_wait(bar, parity, abort, kWaitNs);
@@ -256,19 +262,11 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
   if (warp == 0) {
     if (lane == 0) {
       // ---------------- TMA producer ----------------
+      // codes are in flight before the kernel that prepares the hidden rows ends
       int s = 0;
       uint32_t ph = 0, issued = 0, issue_par = 0;
-      bool ok = true;
-      int64_t h_loads = 0;
+      bool ok = true, prepared = false;
       for (int64_t rb = 0; ok && rb < p.row_blocks; ++rb) {
-        if (kResident) {
-          if (rb > 0 && !thread_wait(h_empty, static_cast<uint32_t>(rb - 1) & 1u)) break;
-          mbar_expect_tx(h_full, static_cast<uint32_t>(p.stages_k) * (N * kStageK * 2));
-          for (int b = 0; b < p.stages_k * (kStageK / 64); ++b)
-            tma_load_2d(resident + b * (N * 128), &map_h, b * 64, static_cast<int32_t>(rb * N),
-                        h_full);
-          ++h_loads;
-        }
         for (int64_t t = t0; ok && t < t1; ++t) {
           for (int k = 0; k < p.stages_k; ++k) {
             if (!thread_wait(&empty[s], ph ^ 1u)) {
@@ -280,10 +278,13 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
             for (int r = 0; r < R; ++r)
               tma_load_2d(w + r * kStageW, &map_w, k * (kStageK / 4),
                           static_cast<int32_t>((t * R + r) * kTileV), &full[s]);
-            if (!kResident)
+            if (!kResident) {
+              if (!prepared) pdl_wait();
+              prepared = true;
               for (int b = 0; b < kStageK / 64; ++b)
                 tma_load_2d(w + R * kStageW + b * (N * 128), &map_h, k * kStageK + b * 64,
                             static_cast<int32_t>(rb * N), &full[s]);
+            }
             issued |= 1u << s;
             issue_par = (issue_par & ~(1u << s)) | (ph << s);
             if (++s == stages) {
@@ -296,65 +297,84 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
       // copies in flight land before the CTA exits (immediate unless aborted)
       for (int i = 0; i < stages; ++i)
         if (issued & (1u << i)) mbar_wait(&full[i], (issue_par >> i) & 1u, nullptr, kDrainNs);
-      if (h_loads > 0)
-        mbar_wait(h_full, static_cast<uint32_t>(h_loads - 1) & 1u, nullptr, kDrainNs);
     }
-  } else if (warp == 1) {
-    if (lane == 0) {
-      // ---------------- MMA issuer ----------------
-      int s = 0;
-      uint32_t ph = 0;
-      uint64_t* last_bar = nullptr;
-      uint32_t last_par = 0;
-      bool ok = true;
-      uint32_t q = 0;  // chunk number; its barriers' parities need its low bits only
-      for (int64_t rb = 0; ok && rb < p.row_blocks; ++rb) {
-        if (kResident && !thread_wait(h_full, static_cast<uint32_t>(rb) & 1u)) break;
-        for (int64_t t = t0; ok && t < t1; ++t) {
-          for (int k = 0; ok && k < p.stages_k; ++k) {
-            // the codes reach this role through TMEM; with resident hidden rows a
-            // stage is refilled without it and its barrier must not be waited for
-            if (!kResident && !thread_wait(&full[s], ph)) {
+  } else if (warp == 3) {
+    if (kResident && lane == 0) {
+      // ---------------- resident hidden rows: one load a pass ----------------
+      pdl_wait();
+      int64_t loads = 0;
+      for (int64_t rb = 0; rb < p.row_blocks; ++rb, ++loads) {
+        if (rb > 0 && !thread_wait(h_empty, static_cast<uint32_t>(rb - 1) & 1u)) break;
+        mbar_expect_tx(h_full, static_cast<uint32_t>(p.stages_k) * (N * kStageK * 2));
+        for (int b = 0; b < p.stages_k * (kStageK / 64); ++b)
+          tma_load_2d(resident + b * (N * 128), &map_h, b * 64, static_cast<int32_t>(rb * N),
+                      h_full);
+      }
+      if (loads > 0)
+        mbar_wait(h_full, static_cast<uint32_t>(loads - 1) & 1u, nullptr, kDrainNs);
+    }
+  } else if (warp == 1 || warp == 2) {
+    // ---------------- MMA issuers: one for each unpacking warpgroup ----------------
+    // The whole warp runs the loop, so that addresses and descriptors stay
+    // warp-uniform; lane 0 issues.
+    const uint32_t mw = static_cast<uint32_t>(warp) - 1u;
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    uint32_t q = mw;  // chunk number; its barriers' parities need its low bits only
+    for (int64_t rb = 0; ok && rb < p.row_blocks; ++rb) {
+      if (kResident && !warp_wait(h_full, static_cast<uint32_t>(rb) & 1u)) break;
+      for (int64_t t = t0; ok && t < t1; ++t) {
+        for (int k = 0; ok && k < p.stages_k; ++k) {
+          // the codes reach this role through TMEM; with resident hidden rows a
+          // stage is refilled without it and its barrier must not be waited for
+          if (!kResident && !warp_wait(&full[s], ph)) {
+            ok = false;
+            break;
+          }
+          const uint32_t b0 = kResident ? smem_u32(resident + size_t(k) * (N * kStageK * 2))
+                                        : smem_u32(stage0 + s * kStage + R * kStageW);
+          for (int c = static_cast<int>(mw); c < 2 * R; c += 2, q += 2) {
+            const uint32_t ab = (q & 1u) * 2 + ((q >> 1) & 1u), db = q % kDBufs;
+            if (!warp_wait(&a_full[ab], (q >> 2) & 1u) ||
+                !warp_wait(&d_empty[db], (q / kDBufs & 1u) ^ 1u)) {
               ok = false;
               break;
             }
-            const uint32_t b0 = kResident ? smem_u32(resident + size_t(k) * (N * kStageK * 2))
-                                          : smem_u32(stage0 + s * kStage + R * kStageW);
-            for (int c = 0; c < 2 * R; ++c, ++q) {
-              const uint32_t ab = (q & 1u) * 2 + ((q >> 1) & 1u), db = q % kDBufs;
-              if (!thread_wait(&a_full[ab], (q >> 2) & 1u) ||
-                  !thread_wait(&d_empty[db], (q / kDBufs & 1u) ^ 1u)) {
-                ok = false;
-                break;
-              }
-              tc_fence_after();
-              const uint32_t a = tmem_base + ab * kChunkCols, d = d_base + db * kDCols;
-              const uint32_t bh = b0 + (c / R) * (2 * N * 128);
+            tc_fence_after();
+            const uint32_t a = tmem_base + ab * kChunkCols, d = d_base + db * kDCols;
+            const uint64_t bd = sw128_desc(b0 + (c / R) * (2 * N * 128));
+            if (lane == 0) {
 #pragma unroll
               for (int kk = 0; kk < kChunk / kUmmaK; ++kk) {
                 constexpr int per = kChunk / kUmmaK / S;  // MMAs of a group
+                // the descriptor's address field counts 16 bytes
                 umma_f16_ts(d + (kk / per) * N, a + kk * (kUmmaK / 2),
-                            sw128_desc(bh + (kk / 4) * (N * 128) + (kk % 4) * 32), kDesc,
+                            bd + (kk / 4) * (N * 128 / 16) + (kk % 4) * 2, kDesc,
                             kk % per != 0 ? 1u : 0u);
               }
               umma_commit(&a_empty[ab]);
               umma_commit(&d_full[db]);
-              last_bar = &d_full[db];
-              last_par = q / kDBufs & 1u;
             }
-            if (!ok) break;
-            if (!kResident) umma_commit(&empty[s]);
-            if (++s == stages) {
-              s = 0;
-              ph ^= 1u;
-            }
+            __syncwarp();
+          }
+          if (!ok) break;
+          if (!kResident && lane == 0) umma_commit(&empty[s]);
+          if (++s == stages) {
+            s = 0;
+            ph ^= 1u;
           }
         }
-        if (kResident && ok) umma_commit(h_empty);
       }
-      // MMAs in flight finish before the TMEM is freed (immediate unless aborted)
-      if (last_bar != nullptr) mbar_wait(last_bar, last_par, nullptr, kDrainNs);
+      if (kResident && ok && lane == 0) umma_commit(h_empty);
     }
+    // every arrival of this warp's MMAs lands before the CTA may exit and the
+    // TMEM is freed, also those that no one waits for any more
+    if (lane == 0) {
+      umma_commit(&mma_done[mw]);
+      mbar_wait(&mma_done[mw], 0, nullptr, kDrainNs);
+    }
+    __syncwarp();
   } else if (warp >= 4 + 4 * R) {
     // ---------------- unpacking: thread = weight row ----------------
     const int wg = (warp - 4 - 4 * R) >> 2, quarter = warp & 3;
@@ -388,14 +408,14 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           uint32_t a[32];
-          unpack8<T>(w[2 * j].x, a);
-          unpack8<T>(w[2 * j].y, a + 4);
-          unpack8<T>(w[2 * j].z, a + 8);
-          unpack8<T>(w[2 * j].w, a + 12);
-          unpack8<T>(w[2 * j + 1].x, a + 16);
-          unpack8<T>(w[2 * j + 1].y, a + 20);
-          unpack8<T>(w[2 * j + 1].z, a + 24);
-          unpack8<T>(w[2 * j + 1].w, a + 28);
+          unpack8(w[2 * j].x, a);
+          unpack8(w[2 * j].y, a + 4);
+          unpack8(w[2 * j].z, a + 8);
+          unpack8(w[2 * j].w, a + 12);
+          unpack8(w[2 * j + 1].x, a + 16);
+          unpack8(w[2 * j + 1].y, a + 20);
+          unpack8(w[2 * j + 1].z, a + 24);
+          unpack8(w[2 * j + 1].w, a + 28);
           tmem_store32(dst + 32 * j, a);
         }
         tmem_wait_store();
@@ -436,10 +456,19 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
     auto scale_of = [](uint16_t bits) { return to_float(*reinterpret_cast<const T*>(&bits)); };
 
     uint32_t q = static_cast<uint32_t>(wg);  // R == 2: every other chunk is this warpgroup's
+    uint32_t all_par = 0;
     bool ok = true;
-    if (t0 < t1) load_scales((t0 * R + wg) * kTileV + r, 0);
+    load_scales((t0 * R + wg) * kTileV + r, 0);
+    pdl_wait();
     for (int64_t rb = 0; ok && rb < p.row_blocks; ++rb) {
       const int64_t row0 = rb * N;
+      // the group sums and row scales of this pass's hidden rows
+      for (int64_t i = threadIdx.x - 128; i < group_slots * N; i += 128 * R)
+        sums[i] = i < p.groups * N ? -p.sums[rb * p.groups * N + i] : 0.0f;
+      if (threadIdx.x - 128 < N)
+        sums[group_slots * N + threadIdx.x - 128] = p.row_scale[row0 + threadIdx.x - 128];
+      if (!join(joined_all, all_par)) break;
+      all_par ^= 1u;
       RowStats st{-INFINITY, 0.0f, -1, -1};
       float cur = 0.0f;
       const bool live = p.out == nullptr && row0 + own < p.rows;
@@ -466,24 +495,19 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
             }
             tc_fence_after();
             const uint32_t d = d_base + lane_off + db * kDCols;
+            const float* gs = sums + static_cast<int64_t>(kc + i) * (S * N);
 #pragma unroll
             for (int g = 0; g < S; ++g) {
               const float sc = scale_of(now[i * S + g]);
-              if (N == 16) {
+#pragma unroll
+              for (int j = 0; j < N; j += 16) {
                 uint32_t x[16];
-                tmem_load16(d + g * N, x);
+                tmem_load16(d + g * N + j, x);
 #pragma unroll
-                for (int e = 0; e < 16; e += 2)
-                  scale_add2(acc[e], acc[e + 1], x[e], x[e + 1], sc);
-              } else {
-#pragma unroll
-                for (int j = 0; j < N; j += 32) {
-                  uint32_t x[32];
-                  tmem_issue32(d + g * N + j, x);
-                  tmem_wait32(x);
-#pragma unroll
-                  for (int e = 0; e < 32; e += 2)
-                    scale_add2(acc[(j + e) % N], acc[(j + e + 1) % N], x[e], x[e + 1], sc);
+                for (int e = 0; e < 16; e += 4) {
+                  const float4 h8 = *reinterpret_cast<const float4*>(gs + g * N + j + e);
+                  group_add2(acc[j + e], acc[j + e + 1], x[e], x[e + 1], h8.x, h8.y, sc);
+                  group_add2(acc[j + e + 2], acc[j + e + 3], x[e + 2], x[e + 3], h8.z, h8.w, sc);
                 }
               }
             }
@@ -494,6 +518,8 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
           }
         }
         if (!ok) break;
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] *= sums[group_slots * N + j];
         // ---- the tile's logits: 128 weight rows x N hidden rows ----
         if (p.out != nullptr) {
           if (v < p.vocab) {
@@ -555,7 +581,13 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
         }
         join_par ^= 1u;
       }
-      if (!ok || p.out != nullptr) continue;
+      if (!ok) break;
+      if (p.out != nullptr) {
+        // the next pass's sums wait for every reader of these
+        if (!join(joined_all, all_par)) break;
+        all_par ^= 1u;
+        continue;
+      }
       // ---- the part's record of each row: over the row's threads, then the warpgroups ----
 #pragma unroll
       for (int d = 1; d < kPer; d <<= 1) {
@@ -576,20 +608,17 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
           slot[3] = __int_as_float(st.nan);
           slot[4] = cur;
         }
-        if (!join(joined_all, 0)) {
-          ok = false;
-          break;
-        }
+        if (!join(joined_all, all_par)) break;
+        all_par ^= 1u;
         if (wg == 0) {
           const RowStats o{slot[0], slot[1], __float_as_int(slot[2]), __float_as_int(slot[3])};
           merge_stats(st, o);
           cur += slot[4];
         }
-        if (!join(joined_all, 1)) {
-          ok = false;
-          break;
-        }
       }
+      // the next pass overwrites the slots and sums
+      if (!join(joined_all, all_par)) break;
+      all_par ^= 1u;
       if (live && wg == 0 && sub == 0) {
         cid_shard_record_t rec;
         rec.max_logit = st.m;
@@ -614,6 +643,70 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base),
                  "r"(kTmemCols)
                  : "memory");
+  }
+}
+
+// One block turns one hidden row into the fp16 row of the products, its group
+// sums (8 sum h) and its scale 2^-e; rows past the last get zero sums.
+constexpr int kPrepThreads = 256;
+
+template <typename T>
+__global__ void __launch_bounds__(kPrepThreads)
+    int4_prepare_kernel(const uint4* hidden, int64_t rows, int vecs, int lanes, int n,
+                        uint4* out, float* sums, float* row_scale) {
+  __shared__ uint32_t tops[kPrepThreads / 32];
+  const int64_t r = blockIdx.x;
+  const int groups = vecs / lanes;
+  float* my_sums = sums + (r / n * groups) * n + r % n;
+  if (r >= rows) {
+    for (int g = threadIdx.x; g < groups; g += kPrepThreads) my_sums[int64_t{g} * n] = 0.0f;
+    if (threadIdx.x == 0) row_scale[r] = 0.0f;
+    return;
+  }
+  const uint4* src = hidden + r * vecs;
+  uint32_t top = 0;  // |h| compares as its bits
+  for (int i = threadIdx.x; i < vecs; i += kPrepThreads) {
+    const uint4 v = src[i];
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top = max(top, max(u[j] & 0x7fffu, (u[j] >> 16) & 0x7fffu));
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kPrepThreads / 32; ++i) top = max(top, tops[i]);
+  const uint16_t bits = static_cast<uint16_t>(top);
+  const float most = to_float(*reinterpret_cast<const T*>(&bits));
+  // a row of zeros or one that is not finite keeps its values (the latter's
+  // logits are NaN: an infinity times a code, less eight times it)
+  int e = most > 0.0f && most < INFINITY ? 14 - ilogbf(most) : 0;
+  e = e > 126 ? 126 : e;  // |h| < 2^-112
+  const float up = __int_as_float((e + 127) << 23), down = __int_as_float((127 - e) << 23);
+  if (threadIdx.x == 0) row_scale[r] = down;
+  // whole warps step together: a group's lanes share its sum
+  for (int i0 = 0; i0 < vecs; i0 += kPrepThreads) {
+    const int i = i0 + static_cast<int>(threadIdx.x);
+    float sum = 0.0f;
+    if (i < vecs) {
+      const uint4 v = src[i];
+      const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+      uint32_t o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint16_t b0 = static_cast<uint16_t>(u[j]), b1 = static_cast<uint16_t>(u[j] >> 16);
+        // pairs 1 and 3 of a word meet 16 c
+        const float k = j & 1 ? 0.0625f : 1.0f;
+        const __half2 h = __floats2half2_rn(to_float(*reinterpret_cast<const T*>(&b0)) * up * k,
+                                            to_float(*reinterpret_cast<const T*>(&b1)) * up * k);
+        o[j] = *reinterpret_cast<const uint32_t*>(&h);
+        const float2 f = __half22float2(h);
+        sum += (f.x + f.y) * (j & 1 ? 16.0f : 1.0f);
+      }
+      out[r * vecs + i] = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+    for (int d = 1; d < lanes; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if (i < vecs && i % lanes == 0) my_sums[int64_t{i / lanes} * n] = 8.0f * sum;
   }
 }
 
@@ -709,11 +802,11 @@ struct Int4Plan {
   int64_t tiles, parts;
 };
 
-size_t int4_smem(int n, int r, bool resident, int stages, int64_t stages_k) {
+size_t int4_smem(int n, int r, bool resident, int stages, int64_t stages_k, int64_t slots) {
   const size_t hidden = static_cast<size_t>(n) * kStageK * 2;
   return stages * (r * size_t{kStageW} + (resident ? 0 : hidden)) +
-         (resident ? stages_k * hidden : 0) + static_cast<size_t>(r) * n * kXchPitch * 4 + 1024 +
-         512;
+         (resident ? stages_k * hidden : 0) +
+         (static_cast<size_t>(r) * kXchPitch + slots + 1) * n * 4 + 1024 + 512;
 }
 
 // Hidden rows of a pass: the accumulators of a chunk's groups are at most 64
@@ -725,29 +818,57 @@ size_t int4_smem(int n, int r, bool resident, int stages, int64_t stages_k) {
 Int4Plan int4_plan(int64_t rows, int64_t vocab, int64_t dim, int group) {
   Int4Plan pl;
   const int most = group / 2;
-  const int64_t stages_k = (dim + kStageK - 1) / kStageK;
+  const int64_t stages_k = (dim + kStageK - 1) / kStageK, slots = stages_k * kStageK / group;
   pl.n = rows > 32 && most >= 64 ? 64 : (rows > 16 && most >= 32 ? 32 : 16);
-  pl.resident = int4_smem(pl.n, 1, true, 4, stages_k) <= kSmemLimit;
-  pl.r = pl.resident ? 1 : 2;
-  pl.stages = kMaxStages;
-  while (int4_smem(pl.n, pl.r, pl.resident, pl.stages, stages_k) > kSmemLimit) --pl.stages;
+  for (;; pl.n /= 2) {  // the widest hidden rows leave room for 16 of them only
+    pl.resident = int4_smem(pl.n, 1, true, 4, stages_k, slots) <= kSmemLimit;
+    pl.r = pl.resident ? 1 : 2;
+    pl.stages = kMaxStages;
+    while (pl.stages > 1 &&
+           int4_smem(pl.n, pl.r, pl.resident, pl.stages, stages_k, slots) > kSmemLimit)
+      --pl.stages;
+    if (pl.stages > 1 || pl.n == 16) break;
+  }
   pl.tiles = (vocab + pl.r * kTileV - 1) / (pl.r * kTileV);
   pl.parts = sm_count() < kMaxParts ? sm_count() : kMaxParts;
   if (pl.tiles < pl.parts) pl.parts = pl.tiles;
   return pl;
 }
 
+// Workspace: the fp16 rows, the group sums and row scales of whole passes (sized
+// for passes of 64, whatever the launch takes), and the statistics' records.
+struct Int4Layout {
+  size_t hidden, sums, row_scale, records, bytes;
+};
+
+Int4Layout int4_layout(int64_t rows, int64_t dim, int64_t vocab, int group, bool stats) {
+  auto up = [](size_t x) { return (x + 1023) / 1024 * 1024; };
+  const size_t padded = static_cast<size_t>((rows + 63) / 64 * 64);
+  const int64_t tiles = (vocab + kTileV - 1) / kTileV;
+  Int4Layout l;
+  l.hidden = 0;
+  l.sums = up(static_cast<size_t>(rows) * dim * 2);
+  l.row_scale = l.sums + up(padded * (dim / group) * 4);
+  l.records = l.row_scale + up(padded * 4);
+  l.bytes = l.records + (stats ? static_cast<size_t>(tiles < kMaxParts ? tiles : kMaxParts) *
+                                     static_cast<size_t>(rows) * sizeof(cid_shard_record_t)
+                               : 0);
+  return l;
+}
+
 template <typename T, int N, int S, int R, bool kResident>
 int launch_int4(const CUtensorMap& map_w, const CUtensorMap& map_h, const Int4Params& p,
                 cudaStream_t stream) {
-  const size_t smem = int4_smem(N, R, kResident, p.stages, p.stages_k);
+  const size_t smem =
+      int4_smem(N, R, kResident, p.stages, p.stages_k, static_cast<int64_t>(p.stages_k) * 2 * S);
   const cudaError_t e = cudaFuncSetAttribute(int4_head_kernel<T, N, S, R, kResident>,
                                              cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              static_cast<int>(smem));
   if (e != cudaSuccess) return record_cuda_error(e);
-  int4_head_kernel<T, N, S, R, kResident>
-      <<<static_cast<unsigned>(p.parts), int4_threads(R), smem, stream>>>(map_w, map_h, p);
-  return launch_result();
+  // a programmatic dependent of the kernel that prepares the hidden rows: the
+  // codes start streaming while that one runs
+  return launch_pdl(int4_head_kernel<T, N, S, R, kResident>, dim3(static_cast<unsigned>(p.parts)),
+                    dim3(int4_threads(R)), smem, stream, map_w, map_h, p);
 }
 
 template <typename T, int N, int S>
@@ -758,19 +879,29 @@ int launch_int4(const Int4Plan& pl, const CUtensorMap& map_w, const CUtensorMap&
 }
 
 template <typename T>
-int dispatch_int4(cid_dtype_t dtype, const void* hidden, int64_t dim, const void* packed,
-                  int group, Int4Params p, const Int4Plan& pl, cudaStream_t stream) {
-  CUtensorMap map_w, map_h;
-  // codes copied as 16-bit elements, four columns each
-  int rc = make_map_sw128(&map_w, CID_DTYPE_F16, packed, dim / 4, p.vocab, dim / 4, 64, kTileV);
-  if (rc == CID_OK) rc = make_map_sw128(&map_h, dtype, hidden, dim, p.rows, dim, 64, pl.n);
-  if (rc != CID_OK) return rc;
+int dispatch_int4(const void* hidden, int64_t dim, const void* packed, int group, Int4Params p,
+                  const Int4Plan& pl, unsigned char* ws, const Int4Layout& l,
+                  cudaStream_t stream) {
   p.groups = dim / group;
   p.stages_k = static_cast<int>((dim + kStageK - 1) / kStageK);
   p.row_blocks = (p.rows + pl.n - 1) / pl.n;
   p.tiles = pl.tiles;
   p.parts = pl.parts;
   p.stages = pl.stages;
+  p.sums = reinterpret_cast<const float*>(ws + l.sums);
+  p.row_scale = reinterpret_cast<const float*>(ws + l.row_scale);
+  CUtensorMap map_w, map_h;
+  // codes copied as 16-bit elements, four columns each
+  int rc = make_map_sw128(&map_w, CID_DTYPE_F16, packed, dim / 4, p.vocab, dim / 4, 64, kTileV);
+  if (rc == CID_OK)
+    rc = make_map_sw128(&map_h, CID_DTYPE_F16, ws + l.hidden, dim, p.rows, dim, 64, pl.n);
+  if (rc != CID_OK) return rc;
+  int4_prepare_kernel<T><<<static_cast<unsigned>(p.row_blocks * pl.n), kPrepThreads, 0, stream>>>(
+      static_cast<const uint4*>(hidden), p.rows, static_cast<int>(dim / 8), group / 8, pl.n,
+      reinterpret_cast<uint4*>(ws + l.hidden), reinterpret_cast<float*>(ws + l.sums),
+      reinterpret_cast<float*>(ws + l.row_scale));
+  rc = launch_result();
+  if (rc != CID_OK) return rc;
   switch (group) {
     case 128:
       return pl.n == 64   ? launch_int4<T, 64, 1>(pl, map_w, map_h, p, stream)
@@ -784,18 +915,35 @@ int dispatch_int4(cid_dtype_t dtype, const void* hidden, int64_t dim, const void
   }
 }
 
+// Widest hidden row of the products: its group sums stay in shared memory.
+constexpr int64_t kMaxInt4Dim = 32768;
+
+bool int4_product_ok(int64_t rows, int64_t dim, int64_t vocab, int group) {
+  int64_t n = 0;
+  return rows >= 0 && rows <= kMaxInt4Rows && int4_weight_ok(vocab, dim, group) &&
+         dim <= kMaxInt4Dim && count_ok(rows, dim, &n) && n <= kMaxCount &&
+         count_ok(rows, vocab, &n) && n <= kMaxCount;
+}
+
 // Checks shared by the two products; rows == 0 is left to the caller.
 int check_int4(cid_dtype_t dtype, const void* hidden, int64_t rows, int64_t dim,
                const uint32_t* packed, const void* scales, int group, int64_t vocab,
-               const uint32_t* status) {
+               const void* workspace, const uint32_t* status) {
   if (dtype != CID_DTYPE_BF16 && dtype != CID_DTYPE_F16) return CID_ERR_UNSUPPORTED_DTYPE;
-  int64_t n = 0;
-  if (rows < 0 || rows > kMaxInt4Rows || !int4_weight_ok(vocab, dim, group) ||
-      !count_ok(rows, dim, &n) || n > kMaxCount || !count_ok(rows, vocab, &n) || n > kMaxCount)
-    return CID_ERR_INVALID_ARGUMENT;
-  if (misaligned({{hidden, 16}, {packed, 16}, {scales, 2}, {status, 4}}))
+  if (!int4_product_ok(rows, dim, vocab, group)) return CID_ERR_INVALID_ARGUMENT;
+  if (misaligned({{hidden, 16}, {packed, 16}, {scales, 2}, {workspace, 16}, {status, 4}}))
     return CID_ERR_MISALIGNED;
   return CID_OK;
+}
+
+int run_int4(cid_dtype_t dtype, const void* hidden, int64_t dim, const void* packed, int group,
+             const Int4Params& p, const Int4Plan& pl, void* workspace, const Int4Layout& l,
+             void* stream) {
+  auto* ws = static_cast<unsigned char*>(workspace);
+  return dtype == CID_DTYPE_F16
+             ? dispatch_int4<__half>(hidden, dim, packed, group, p, pl, ws, l, as_stream(stream))
+             : dispatch_int4<__nv_bfloat16>(hidden, dim, packed, group, p, pl, ws, l,
+                                            as_stream(stream));
 }
 
 }  // namespace
@@ -841,35 +989,35 @@ extern "C" int cid_lm_head_dequantize(cid_dtype_t dtype, const uint32_t* packed,
   return launch_result();
 }
 
+extern "C" size_t cid_lm_head_quantized_workspace_bytes(int64_t rows, int64_t hidden_dim,
+                                                        int64_t vocab, int group_size,
+                                                        int statistics) {
+  if (rows <= 0 || !int4_product_ok(rows, hidden_dim, vocab, group_size)) return 0;
+  return int4_layout(rows, hidden_dim, vocab, group_size, statistics != 0).bytes;
+}
+
 extern "C" int cid_lm_head_quantized_logits(cid_dtype_t dtype, const void* hidden, int64_t rows,
                                             int64_t hidden_dim, const uint32_t* packed,
                                             const void* scales, int group_size, int64_t vocab,
-                                            void* logits, uint32_t* status, void* stream) {
-  const int rc =
-      check_int4(dtype, hidden, rows, hidden_dim, packed, scales, group_size, vocab, status);
+                                            void* logits, void* workspace,
+                                            size_t workspace_bytes, uint32_t* status,
+                                            void* stream) {
+  const int rc = check_int4(dtype, hidden, rows, hidden_dim, packed, scales, group_size, vocab,
+                            workspace, status);
   if (rc != CID_OK) return rc;
   if (misaligned({{logits, 2}})) return CID_ERR_MISALIGNED;
   if (rows == 0) return CID_OK;
-  if (any_null({hidden, packed, scales, logits})) return CID_ERR_INVALID_ARGUMENT;
+  if (any_null({hidden, packed, scales, logits, workspace})) return CID_ERR_INVALID_ARGUMENT;
+  const Int4Layout l = int4_layout(rows, hidden_dim, vocab, group_size, false);
+  if (workspace_bytes < l.bytes) return CID_ERR_SCRATCH_LIMIT;
   Int4Params p = {};
   p.rows = rows;
   p.vocab = vocab;
   p.scales = scales;
   p.out = logits;
   p.status = status;
-  const Int4Plan pl = int4_plan(rows, vocab, hidden_dim, group_size);
-  return dtype == CID_DTYPE_F16
-             ? dispatch_int4<__half>(dtype, hidden, hidden_dim, packed, group_size, p, pl,
-                                     as_stream(stream))
-             : dispatch_int4<__nv_bfloat16>(dtype, hidden, hidden_dim, packed, group_size, p, pl,
-                                            as_stream(stream));
-}
-
-extern "C" size_t cid_lm_head_quantized_workspace_bytes(int64_t rows, int64_t vocab) {
-  if (rows <= 0 || rows > kMaxInt4Rows || vocab <= 0 || vocab > INT32_MAX - 2 * kTileV) return 0;
-  const int64_t tiles = (vocab + kTileV - 1) / kTileV;
-  return static_cast<size_t>(tiles < kMaxParts ? tiles : kMaxParts) * static_cast<size_t>(rows) *
-         sizeof(cid_shard_record_t);
+  return run_int4(dtype, hidden, hidden_dim, packed, group_size, p,
+                  int4_plan(rows, vocab, hidden_dim, group_size), workspace, l, stream);
 }
 
 extern "C" int cid_lm_head_quantized_display_statistics(
@@ -878,41 +1026,37 @@ extern "C" int cid_lm_head_quantized_display_statistics(
     const int64_t* token_ids, int round_bf16, float* confidence, int64_t* predicted,
     float* current_confidence, void* workspace, size_t workspace_bytes, uint32_t* status,
     void* stream) {
-  int rc = check_int4(dtype, hidden, rows, hidden_dim, packed, scales, group_size, vocab, status);
+  int rc = check_int4(dtype, hidden, rows, hidden_dim, packed, scales, group_size, vocab,
+                      workspace, status);
   if (rc != CID_OK) return rc;
-  if (misaligned({{token_ids, 8},
-                  {confidence, 4},
-                  {predicted, 8},
-                  {current_confidence, 4},
-                  {workspace, 16}}))
+  if (misaligned(
+          {{token_ids, 8}, {confidence, 4}, {predicted, 8}, {current_confidence, 4}}))
     return CID_ERR_MISALIGNED;
   if (rows == 0) return CID_OK;
   if (any_null({hidden, packed, scales, token_ids, confidence, predicted, current_confidence,
                 workspace}))
     return CID_ERR_INVALID_ARGUMENT;
-  if (workspace_bytes < cid_lm_head_quantized_workspace_bytes(rows, vocab))
-    return CID_ERR_SCRATCH_LIMIT;
+  const Int4Layout l = int4_layout(rows, hidden_dim, vocab, group_size, true);
+  if (workspace_bytes < l.bytes) return CID_ERR_SCRATCH_LIMIT;
+  auto* records =
+      reinterpret_cast<cid_shard_record_t*>(static_cast<unsigned char*>(workspace) + l.records);
   Int4Params p = {};
   p.rows = rows;
   p.vocab = vocab;
   p.scales = scales;
-  p.records = static_cast<cid_shard_record_t*>(workspace);
+  p.records = records;
   p.ids = token_ids;
   p.status = status;
   p.round_bf16 = round_bf16 ? 1 : 0;
   const Int4Plan pl = int4_plan(rows, vocab, hidden_dim, group_size);
-  rc = dtype == CID_DTYPE_F16
-           ? dispatch_int4<__half>(dtype, hidden, hidden_dim, packed, group_size, p, pl,
-                                   as_stream(stream))
-           : dispatch_int4<__nv_bfloat16>(dtype, hidden, hidden_dim, packed, group_size, p, pl,
-                                          as_stream(stream));
+  rc = run_int4(dtype, hidden, hidden_dim, packed, group_size, p, pl, workspace, l, stream);
   if (rc != CID_OK) return rc;
   // merge the parts of every row (ascending column ranges) into its statistics
   int64_t offsets[kMaxParts + 1];
   for (int64_t i = 0; i < pl.parts; ++i)
     offsets[i] = i * pl.tiles / pl.parts * (pl.r * kTileV);
   offsets[pl.parts] = vocab;
-  return cid_display_combine_records(static_cast<const cid_shard_record_t*>(workspace),
-                                     static_cast<int>(pl.parts), offsets, token_ids, rows,
-                                     confidence, predicted, current_confidence, status, stream);
+  return cid_display_combine_records(records, static_cast<int>(pl.parts), offsets, token_ids,
+                                     rows, confidence, predicted, current_confidence, status,
+                                     stream);
 }

@@ -527,11 +527,15 @@ at::Tensor lm_head_quantized_logits(Backend backend, const at::Tensor& hidden,
   auto h = aligned16(hidden);
   auto p = aligned16(packed);
   auto s = scales.contiguous();
-  const auto dim = h.size(-1);
+  const auto dim = h.size(-1), rows = h.numel() / dim;
+  TORCH_CHECK(dim <= 32768, "hidden_dim must be at most 32768");
+  const size_t bytes = cid_lm_head_quantized_workspace_bytes(rows, dim, p.size(0),
+                                                             static_cast<int>(group), 0);
+  auto ws = at::empty({static_cast<std::int64_t>(bytes)}, hidden.options().dtype(at::kByte));
   check_result(cid_lm_head_quantized_logits(
-                   dt(h), h.data_ptr(), h.numel() / dim, dim,
+                   dt(h), h.data_ptr(), rows, dim,
                    reinterpret_cast<const std::uint32_t*>(p.data_ptr<int>()), s.data_ptr(),
-                   static_cast<int>(group), p.size(0), logits.data_ptr(),
+                   static_cast<int>(group), p.size(0), logits.data_ptr(), ws.data_ptr(), bytes,
                    detail::status_word(h.device()), stream_of(h)),
                "lm_head_quantized_logits");
   return logits;
@@ -562,7 +566,9 @@ Tensor3 lm_head_quantized_display_statistics(Backend backend, const at::Tensor& 
   auto s = scales.contiguous();
   auto ids = token_ids.contiguous();
   const auto rows = ids.numel();
-  const size_t bytes = cid_lm_head_quantized_workspace_bytes(rows, p.size(0));
+  TORCH_CHECK(h.size(-1) <= 32768, "hidden_dim must be at most 32768");
+  const size_t bytes = cid_lm_head_quantized_workspace_bytes(rows, h.size(-1), p.size(0),
+                                                             static_cast<int>(group), 1);
   auto ws = at::empty({static_cast<std::int64_t>(bytes)}, hidden.options().dtype(at::kByte));
   check_result(cid_lm_head_quantized_display_statistics(
                    dt(h), h.data_ptr(), rows, h.size(-1),

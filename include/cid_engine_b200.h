@@ -469,18 +469,21 @@ CID_API int cid_lm_head_dequantize(cid_dtype_t dtype, const uint32_t* packed, co
                         int64_t vocab, int64_t hidden_dim, int group_size, void* weight,
                         void* stream);
 
-/* logits = hidden @ (scale * q)^T: hidden rows x hidden_dim of `dtype` (the
- * scales' type), 16-byte aligned; each group's sum of q * hidden is accumulated
- * in f32 on the tcgen05 tensor cores and scaled in f32; logits rows x vocab of
- * `dtype`, rounded once.  Waits inside the kernel are bounded; one that runs
- * out sets CID_STATUS_LM_HEAD_TIMEOUT. */
+/* Workspace bytes of the two products below (statistics = 0 for the logits, 1
+ * for the display statistics); 0 for extents outside their ranges. */
+CID_API size_t cid_lm_head_quantized_workspace_bytes(int64_t rows, int64_t hidden_dim,
+                        int64_t vocab, int group_size, int statistics);
+
+/* logits = hidden @ (scale * q)^T: hidden rows x hidden_dim (<= 32768) of `dtype`
+ * (the scales' type), 16-byte aligned (workspace too); each group's sum of
+ * q * hidden is accumulated in f32 on the tcgen05 tensor cores and scaled in
+ * f32; logits rows x vocab of `dtype`, rounded once.  A hidden row with a NaN or
+ * infinite value has NaN logits.  Waits inside the kernel are bounded; one that
+ * runs out sets CID_STATUS_LM_HEAD_TIMEOUT. */
 CID_API int cid_lm_head_quantized_logits(cid_dtype_t dtype, const void* hidden, int64_t rows,
                         int64_t hidden_dim, const uint32_t* packed, const void* scales,
-                        int group_size, int64_t vocab, void* logits, uint32_t* status,
-                        void* stream);
-
-/* Workspace bytes cid_lm_head_quantized_display_statistics needs. */
-CID_API size_t cid_lm_head_quantized_workspace_bytes(int64_t rows, int64_t vocab);
+                        int group_size, int64_t vocab, void* logits, void* workspace,
+                        size_t workspace_bytes, uint32_t* status, void* stream);
 
 /* cid_display_token_statistics over those logits without writing them: in f32,
  * each rounded to bf16 first when round_bf16 != 0. */

@@ -21,6 +21,7 @@ F32, F16, BF16 = 0, 2, 3
 def lib() -> ctypes.CDLL:
     lib = ctypes.CDLL(str(LIB))
     lib.cid_lm_head_cross_entropy_workspace_bytes.restype = ctypes.c_size_t
+    lib.cid_lm_head_quantized_workspace_bytes.restype = ctypes.c_size_t
     return lib
 
 
@@ -200,7 +201,6 @@ def test_int4_refusals() -> None:
 
 def test_int4_c_abi_checks(lib: ctypes.CDLL) -> None:
     i64, p, null, size = ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p(0), ctypes.c_size_t
-    lib.cid_lm_head_quantized_workspace_bytes.restype = size
 
     def quantize(dtype=BF16, w=0x1000, vocab=100, dim=128, group=64, out=0x2000, sc=0x3000):
         return lib.cid_lm_head_quantize(dtype, p(w), i64(vocab), i64(dim), ctypes.c_int(group),
@@ -218,21 +218,30 @@ def test_int4_c_abi_checks(lib: ctypes.CDLL) -> None:
         assert f(w=0x1008) == MISALIGNED and f(out=0x2004) == MISALIGNED and f(sc=0x3001) == MISALIGNED
         assert f(w=0) == INVALID and f(out=0) == INVALID and f(sc=0) == INVALID
 
-    def logits(dtype=BF16, rows=2, h=0x1000, dim=128, group=64, vocab=100, out=0x5000):
+    def need(rows, dim, vocab, group, statistics):
+        return lib.cid_lm_head_quantized_workspace_bytes(
+            i64(rows), i64(dim), i64(vocab), ctypes.c_int(group), ctypes.c_int(statistics))
+
+    assert 0 < need(2, 128, 300, 64, 0)
+    assert need(2, 128, 300, 64, 1) == need(2, 128, 300, 64, 0) + 3 * 2 * 16
+    for bad in ((0, 128, 300, 64), (-1, 128, 300, 64), (2, 0, 300, 64), (2, 128, 0, 64),
+                (2, 128, 2**31, 64), (2, 128, 300, 48), (2, 32768 + 128, 300, 64)):
+        assert need(*bad, 1) == 0
+
+    def logits(dtype=BF16, rows=2, h=0x1000, dim=128, group=64, vocab=100, out=0x5000, ws=0x6000,
+               bytes_=1 << 40):
         return lib.cid_lm_head_quantized_logits(dtype, p(h), i64(rows), i64(dim), p(0x2000),
                                                 p(0x3000), ctypes.c_int(group), i64(vocab), p(out),
-                                                null, null)
+                                                p(ws), size(bytes_), null, null)
 
     assert logits(dtype=F32) == DTYPE and logits(rows=-1) == INVALID and logits(dim=100) == INVALID
     assert logits(rows=2**31) == INVALID and logits(h=0x1002) == MISALIGNED
+    assert logits(dim=32768 + 128) == INVALID and logits(ws=0x6008) == MISALIGNED
     assert logits(out=0x5001) == MISALIGNED and logits(rows=0) == OK
-    assert logits(h=0) == INVALID and logits(out=0) == INVALID
-    need = lib.cid_lm_head_quantized_workspace_bytes(i64(2), i64(300))
-    assert need == 3 * 2 * 16
-    for bad in ((0, 300), (-1, 300), (2, 0), (2, 2**31)):
-        assert lib.cid_lm_head_quantized_workspace_bytes(i64(bad[0]), i64(bad[1])) == 0
+    assert logits(h=0) == INVALID and logits(out=0) == INVALID and logits(ws=0) == INVALID
+    assert logits(bytes_=need(2, 128, 100, 64, 0) - 1) == SCRATCH
 
-    def stats(ids=0x4000, ws=0x6000, bytes_=need, rows=2):
+    def stats(ids=0x4000, ws=0x6000, bytes_=1 << 40, rows=2):
         return lib.cid_lm_head_quantized_display_statistics(
             BF16, p(0x1000), i64(rows), i64(128), p(0x2000), p(0x3000), ctypes.c_int(64),
             i64(300), p(ids), ctypes.c_int(1), p(0x5000), p(0x5100), p(0x5200), p(ws),
@@ -240,4 +249,4 @@ def test_int4_c_abi_checks(lib: ctypes.CDLL) -> None:
 
     assert stats(ids=0x4004) == MISALIGNED and stats(ws=0x6008) == MISALIGNED
     assert stats(ids=0) == INVALID and stats(ws=0) == INVALID and stats(rows=0) == OK
-    assert stats(bytes_=need - 1) == SCRATCH
+    assert stats(bytes_=need(2, 128, 300, 64, 1) - 1) == SCRATCH
