@@ -22,15 +22,25 @@
 // largest, far under the f32 sum's own rounding.  The same kernel leaves 8 sum h
 // of every group, which read-back subtracts: sum c h - 8 sum h = sum q h.
 //
-// Product kernel.  The weight's bytes bound it up to some 64 rows (128256 x
-// 4096: 270 MB, 42 us at the copy peak), so every SM streams weight tiles of
-// 128 rows with TMA, whatever the number of hidden rows.  The contraction runs
-// on the tensor cores with the weight as A: a thread owns one weight row, masks
-// 128 of its codes into 64 registers and stores them to TMEM, which tcgen05.mma
-// takes as its A operand; hidden rows are B (N = 16 to 64 columns of the
-// accumulator).  The scale is applied in f32 to each group's sum when it is read
-// back from TMEM.  Unpacking, MMAs and read-back are warps of their own, joined
-// by rings of TMEM buffers.
+// Two product kernels; the weight's bytes bound both up to some 64 rows (128256 x
+// 4096: 270 MB, 42 us at the copy peak).
+//
+// * Up to 16 hidden rows (int4_rows_kernel): every warp multiplies on its own,
+//   with mma.sync (16 weight rows x 16 columns times 8 hidden rows).  A thread's
+//   16 bytes of codes from memory are its A fragments after masking, since the
+//   MMA's columns may be taken in any order that the hidden rows in shared
+//   memory follow.  No buffer changes hands between warps until a tile's sums
+//   meet, and at these sizes the legacy tensor path is fast enough (N = 16:
+//   about 29 us of HMMA beside 42 us of memory).  tcgen05 measured 96 us at 16
+//   rows: its hand-overs (codes to TMEM, MMA, accumulator back, each a barrier)
+//   cost more than the MMAs.
+// * More rows (int4_head_kernel): tcgen05 with the weight as A.  Every SM
+//   streams weight tiles with TMA; a thread owns one weight row, masks 128 of
+//   its codes into 64 registers and stores them to TMEM, which tcgen05.mma takes
+//   as its A operand; hidden rows are B (N = 16 to 64 columns of the
+//   accumulator).  The scale is applied in f32 to each group's sum when it is
+//   read back from TMEM.  Unpacking, MMAs and read-back are warps of their own,
+//   joined by rings of TMEM buffers.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -155,6 +165,23 @@ __device__ __forceinline__ void merge_stats(RowStats& a, const RowStats& b) {
   }
   a.m = m;
   if (b.nan >= 0 && (a.nan < 0 || b.nan < a.nan)) a.nan = b.nan;
+}
+
+// The shard record of merged statistics; `first` is the part's first column.
+__device__ __forceinline__ cid_shard_record_t record_of(const RowStats& a, float current,
+                                                        int first) {
+  cid_shard_record_t rec;
+  rec.max_logit = a.m;
+  if (!(a.m > -INFINITY && a.m < INFINITY) || a.s != a.s) {
+    const int at = a.nan >= 0 ? a.nan : (a.where >= 0 ? a.where : first);
+    rec.sum_exp = a.m == -INFINITY ? 0.0f : __int_as_float(0x7fffffff);
+    rec.index = at | (a.nan >= 0 ? static_cast<int32_t>(0x80000000u) : 0);
+  } else {
+    rec.sum_exp = a.s;
+    rec.index = a.where;
+  }
+  rec.current = current;
+  return rec;
 }
 
 // Roles of a CTA: warps 0-3 control (0 codes' TMA, 1 and 2 MMA, 3 hidden rows' TMA), then R warpgroups that read
@@ -619,21 +646,9 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
       // the next pass overwrites the slots and sums
       if (!join(joined_all, all_par)) break;
       all_par ^= 1u;
-      if (live && wg == 0 && sub == 0) {
-        cid_shard_record_t rec;
-        rec.max_logit = st.m;
-        if (!(st.m > -INFINITY && st.m < INFINITY) || st.s != st.s) {
-          const int first = static_cast<int>(t0 * R * kTileV);
-          const int at = st.nan >= 0 ? st.nan : (st.where >= 0 ? st.where : first);
-          rec.sum_exp = st.m == -INFINITY ? 0.0f : __int_as_float(0x7fffffff);
-          rec.index = at | (st.nan >= 0 ? static_cast<int32_t>(0x80000000u) : 0);
-        } else {
-          rec.sum_exp = st.s;
-          rec.index = st.where;
-        }
-        rec.current = cur;
-        p.records[part * p.rows + row0 + own] = rec;
-      }
+      if (live && wg == 0 && sub == 0)
+        p.records[part * p.rows + row0 + own] =
+            record_of(st, cur, static_cast<int>(t0 * R * kTileV));
     }
   }
 
@@ -646,14 +661,300 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
   }
 }
 
-// One block turns one hidden row into the fp16 row of the products, its group
-// sums (8 sum h) and its scale 2^-e; rows past the last get zero sums.
+// ---------------------------------------------------------------------------
+// Up to 16 hidden rows
+// ---------------------------------------------------------------------------
+
+constexpr int kRowsThreads = 512;
+constexpr int kRowsWarps = kRowsThreads / 32;
+constexpr int kRowsPad = 64;  // bytes between hidden rows in shared memory, past whole blocks
+
+struct RowsParams {
+  const uint32_t* packed;
+  const uint16_t* scales;
+  const uint4* hidden;  // prepared, in fragment order: [rows][blocks * 16]
+  const float* sums;    // [groups][N]
+  const float* row_scale;
+  int64_t rows, vocab;
+  int words, groups, blocks;  // a weight row's words, groups and blocks of 128 columns
+  int row_warps;              // 1, 2 or 4 warps along the weight rows, the others along K
+  int64_t tiles, parts;
+  void* out;
+  cid_shard_record_t* records;
+  const int64_t* ids;
+  int round_bf16;
+};
+
+// A thread's codes and scales of 32 weight rows x 128 columns: rows g, g + 8,
+// g + 16, g + 24 (g = lane / 4), in each four words; the scales are those of row
+// g + 8 t (t = lane % 4).
+template <int S>
+struct CodeBlock {
+  uint32_t w[4][4];
+  uint16_t scale[S];
+};
+
+__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                          uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Codes are read once: no line of them stays in L1.
+template <int B>
+__device__ __forceinline__ void load_codes(uint32_t* to, const uint32_t* from) {
+  if (B == 4)
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(to[0]), "=r"(to[1]), "=r"(to[2]), "=r"(to[3])
+                 : "l"(from));
+  else if (B == 2)
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];"
+                 : "=r"(to[0]), "=r"(to[1])
+                 : "l"(from));
+  else
+    asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(to[0]) : "l"(from));
+}
+
+template <typename T, int N, int S>
+__global__ void __launch_bounds__(kRowsThreads, 1) int4_rows_kernel(RowsParams p) {
+  constexpr int kNB = N / 8;     // MMA columns
+  constexpr int kRun = 4 / S;    // consecutive words of a group a thread takes
+  extern __shared__ unsigned char smem[];
+  const int pitch = p.blocks * 256 + kRowsPad;
+  const int rw = p.row_warps, kws = kRowsWarps / rw, tile_rows = 32 * rw;
+  unsigned char* hid = smem;                                     // [N][pitch]
+  float* sums = reinterpret_cast<float*>(smem + N * pitch);      // [blocks * S][N] of -8 sum h
+  float* rscale = sums + p.blocks * S * N;                       // [N]
+  float* red = rscale + N;                                       // [2][kws][N][tile_rows]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int rwi = warp % rw, kw = warp / rw;
+  const int64_t t0 = blockIdx.x * p.tiles / p.parts, t1 = (blockIdx.x + 1) * p.tiles / p.parts;
+  const int per_tile = (p.blocks + kws - 1) / kws;  // blocks of a warp, the last perhaps empty
+  const int64_t total = (t1 - t0) * per_tile;
+
+  int64_t l_tile = t0;  // position of the next load
+  int l_k = 0;
+  auto load = [&](CodeBlock<S>& b) {
+    const int kb = kw + l_k * kws;
+    const int64_t v0 = l_tile * tile_rows + rwi * 32;
+    const bool any = l_tile < t1 && kb < p.blocks;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int64_t v = v0 + g + 8 * r;
+      const uint32_t* row = p.packed + v * p.words + kb * 16;
+#pragma unroll
+      for (int i = 0; i < 4; i += kRun) {
+        // words of a group stand together: group i / kRun, words t * kRun + 0..
+        const int at = (i / kRun) * (4 * kRun) + t * kRun;
+        if (any && v < p.vocab && kb * 16 + at < p.words)
+          load_codes<kRun>(&b.w[r][i], row + at);
+        else
+          for (int j = 0; j < kRun; ++j) b.w[r][i + j] = 0;
+      }
+    }
+    const int64_t v = v0 + g + 8 * t;
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+      const int gi = kb * S + i;
+      b.scale[i] = any && v < p.vocab && gi < p.groups ? p.scales[v * p.groups + gi] : uint16_t{0};
+    }
+    if (++l_k == per_tile) {
+      l_k = 0;
+      ++l_tile;
+    }
+  };
+
+  CodeBlock<S> ring[2];
+  load(ring[0]);
+  load(ring[1]);
+
+  // ---- the hidden rows: from the kernel before ----
+  pdl_wait();
+  for (int i = threadIdx.x; i < N * p.blocks * 16; i += kRowsThreads) {
+    const int n = i / (p.blocks * 16), u = i % (p.blocks * 16);
+    const uint4 h = n < p.rows ? p.hidden[static_cast<int64_t>(n) * (p.blocks * 16) + u]
+                               : make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<uint4*>(hid + n * pitch + u * 16) = h;
+  }
+  for (int i = threadIdx.x; i < p.blocks * S * N; i += kRowsThreads)
+    sums[i] = i < p.groups * N ? -p.sums[i] : 0.0f;
+  if (threadIdx.x < N) rscale[threadIdx.x] = p.row_scale[threadIdx.x];
+  __syncthreads();
+
+  // outputs of this thread: tile row tid % tile_rows, hidden rows tid / tile_rows, + step, ...
+  constexpr int kOwn = 4 * N / 16 > 1 ? 4 * N / 16 : 1;  // at most, with tiles of 128 rows
+  const int orow = threadIdx.x % tile_rows, on = threadIdx.x / tile_rows;
+  const int step = kRowsThreads / tile_rows;
+  RowStats st[kOwn];
+  float cur[kOwn];
+#pragma unroll
+  for (int j = 0; j < kOwn; ++j) {
+    st[j] = RowStats{-INFINITY, 0.0f, -1, -1};
+    cur[j] = 0.0f;
+  }
+
+  float acc[2][kNB][4] = {};
+  int64_t tile = t0;
+  int k = 0, buf = 0;
+  auto compute = [&](const CodeBlock<S>& b) {
+    const int kb = kw + k * kws;
+    if (kb < p.blocks) {
+      const unsigned char* h = hid + g * pitch + kb * 256 + t * 16;
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        float c[2][kNB][4] = {};
+#pragma unroll
+        for (int i = s * kRun; i < (s + 1) * kRun; ++i) {
+          uint32_t a[4][4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) unpack8(b.w[r][i], a[r]);
+#pragma unroll
+          for (int nb = 0; nb < kNB; ++nb) {
+            const uint4 x = *reinterpret_cast<const uint4*>(h + nb * 8 * pitch + i * 64);
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+              mma_16816(c[m][nb], a[2 * m][0], a[2 * m + 1][0], a[2 * m][1], a[2 * m + 1][1], x.x,
+                        x.y);
+              mma_16816(c[m][nb], a[2 * m][2], a[2 * m + 1][2], a[2 * m][3], a[2 * m + 1][3], x.z,
+                        x.w);
+            }
+          }
+        }
+        const float own = to_float(*reinterpret_cast<const T*>(&b.scale[s]));
+        float sc[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sc[r] = __shfl_sync(0xffffffffu, own, (lane & ~3) + r);
+        const float* gs = sums + (kb * S + s) * N + 2 * t;
+#pragma unroll
+        for (int nb = 0; nb < kNB; ++nb) {
+          const float2 h8 = *reinterpret_cast<const float2*>(gs + nb * 8);
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            float* q = acc[m][nb];
+            const float* d = c[m][nb];
+            group_add2(q[0], q[1], __float_as_uint(d[0]), __float_as_uint(d[1]), h8.x, h8.y,
+                       sc[2 * m]);
+            group_add2(q[2], q[3], __float_as_uint(d[2]), __float_as_uint(d[3]), h8.x, h8.y,
+                       sc[2 * m + 1]);
+          }
+        }
+      }
+    }
+    if (++k < per_tile) return;
+    // ---- the tile's sums over the warps along K ----
+    k = 0;
+    float* rb = red + buf * (kws * N * tile_rows);
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int nb = 0; nb < kNB; ++nb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int row = rwi * 32 + m * 16 + (e >> 1) * 8 + g, n = nb * 8 + 2 * t + (e & 1);
+          rb[(kw * N + n) * tile_rows + row] = acc[m][nb][e];
+          acc[m][nb][e] = 0.0f;
+        }
+    __syncthreads();
+    // the other buffer was read before this barrier, this one is before the next
+    const int64_t v = tile * tile_rows + orow;
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) {
+      const int n = on + j * step;
+      if (n < N && n < p.rows) {
+        float z = 0.0f;
+        for (int q = 0; q < kws; ++q) z += rb[(q * N + n) * tile_rows + orow];
+        z *= rscale[n];
+        if (p.out != nullptr) {
+          if (v < p.vocab) {
+            if (std::is_same<T, __nv_bfloat16>::value)
+              static_cast<__nv_bfloat16*>(p.out)[n * p.vocab + v] = __float2bfloat16_rn(z);
+            else
+              static_cast<__half*>(p.out)[n * p.vocab + v] = __float2half_rn(z);
+          }
+        } else if (v < p.vocab) {
+          if (p.round_bf16) z = __bfloat162float(__float2bfloat16_rn(z));
+          const int c = static_cast<int>(v);
+          merge_stats(st[j], z != z ? RowStats{-INFINITY, z, -1, c}
+                                    : RowStats{z, z == INFINITY ? NAN : (z == -INFINITY ? 0.0f : 1.0f),
+                                               c, -1});
+          if (p.ids[n] == v) cur[j] = z;
+        }
+      }
+    }
+    buf ^= 1;
+    ++tile;
+  };
+
+  for (int64_t i = 0; i < total; i += 2) {
+    compute(ring[0]);
+    load(ring[0]);
+    if (i + 1 < total) {
+      compute(ring[1]);
+      load(ring[1]);
+    }
+  }
+  if (p.out != nullptr) return;
+
+  // ---- the part's record of each hidden row: over the tile's rows ----
+  __syncthreads();
+  float* slots = red;  // [N][rw][8]
+#pragma unroll
+  for (int j = 0; j < kOwn; ++j) {
+    const int n = on + j * step;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      RowStats o;
+      o.m = __shfl_xor_sync(0xffffffffu, st[j].m, d);
+      o.s = __shfl_xor_sync(0xffffffffu, st[j].s, d);
+      o.where = __shfl_xor_sync(0xffffffffu, st[j].where, d);
+      o.nan = __shfl_xor_sync(0xffffffffu, st[j].nan, d);
+      merge_stats(st[j], o);
+      cur[j] += __shfl_xor_sync(0xffffffffu, cur[j], d);  // one thread at most has seen the token
+    }
+    if (lane == 0 && n < N) {
+      float* s = slots + (n * rw + orow / 32) * 8;
+      s[0] = st[j].m;
+      s[1] = st[j].s;
+      s[2] = __int_as_float(st[j].where);
+      s[3] = __int_as_float(st[j].nan);
+      s[4] = cur[j];
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < N && threadIdx.x < p.rows) {
+    const int n = threadIdx.x;
+    RowStats a{-INFINITY, 0.0f, -1, -1};
+    float c = 0.0f;
+    for (int q = 0; q < rw; ++q) {
+      const float* s = slots + (n * rw + q) * 8;
+      merge_stats(a, RowStats{s[0], s[1], __float_as_int(s[2]), __float_as_int(s[3])});
+      c += s[4];
+    }
+    p.records[blockIdx.x * p.rows + n] = record_of(a, c, static_cast<int>(t0 * tile_rows));
+  }
+}
+
+// Place of 8 columns (unit u of a block of 128) in the order of the fragments: a
+// quad's thread t takes word i of its codes as columns `first + 8 t'`, see
+// int4_rows_kernel; unit (t, i) goes to 4 i + t.
+__device__ __forceinline__ int fragment_place(int u, int lanes) {
+  if (lanes == 16) return (u & 3) * 4 + (u >> 2);                         // groups of 128
+  if (lanes == 8) return ((u >> 3) * 2 + (u & 1)) * 4 + ((u >> 1) & 3);   // of 64
+  return u;                                                               // of 32
+}
+
+// One block turns one hidden row into the fp16 row of the products (`pitch` units
+// of 8 columns; zeros past the last column), its group sums (8 sum h) and its
+// scale 2^-e; rows past the last get zero sums.
 constexpr int kPrepThreads = 256;
 
 template <typename T>
 __global__ void __launch_bounds__(kPrepThreads)
     int4_prepare_kernel(const uint4* hidden, int64_t rows, int vecs, int lanes, int n,
-                        uint4* out, float* sums, float* row_scale) {
+                        int pitch, bool fragments, uint4* out, float* sums, float* row_scale) {
   __shared__ uint32_t tops[kPrepThreads / 32];
   const int64_t r = blockIdx.x;
   const int groups = vecs / lanes;
@@ -685,9 +986,11 @@ __global__ void __launch_bounds__(kPrepThreads)
   const float up = __int_as_float((e + 127) << 23), down = __int_as_float((127 - e) << 23);
   if (threadIdx.x == 0) row_scale[r] = down;
   // whole warps step together: a group's lanes share its sum
-  for (int i0 = 0; i0 < vecs; i0 += kPrepThreads) {
+  for (int i0 = 0; i0 < pitch; i0 += kPrepThreads) {
     const int i = i0 + static_cast<int>(threadIdx.x);
+    const int64_t to = r * pitch + (fragments ? (i & ~15) + fragment_place(i & 15, lanes) : i);
     float sum = 0.0f;
+    if (i >= vecs && i < pitch) out[to] = make_uint4(0, 0, 0, 0);
     if (i < vecs) {
       const uint4 v = src[i];
       const uint32_t u[4] = {v.x, v.y, v.z, v.w};
@@ -703,7 +1006,7 @@ __global__ void __launch_bounds__(kPrepThreads)
         const float2 f = __half22float2(h);
         sum += (f.x + f.y) * (j & 1 ? 16.0f : 1.0f);
       }
-      out[r * vecs + i] = make_uint4(o[0], o[1], o[2], o[3]);
+      out[to] = make_uint4(o[0], o[1], o[2], o[3]);
     }
     for (int d = 1; d < lanes; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     if (i < vecs && i % lanes == 0) my_sums[int64_t{i / lanes} * n] = 8.0f * sum;
@@ -796,11 +1099,18 @@ bool int4_weight_ok(int64_t vocab, int64_t dim, int group) {
 // A launch's shape: R blocks of 128 weight rows a tile, its tiles and its parts
 // (one a CTA).
 struct Int4Plan {
-  int n, r;
+  int n, r;        // r: 0 for int4_rows_kernel
   bool resident;
   int stages;
+  int row_warps;   // of int4_rows_kernel
+  int tile_rows;
   int64_t tiles, parts;
 };
+
+size_t rows_smem(int n, int row_warps, int64_t blocks, int group) {
+  return n * (blocks * 256 + kRowsPad) + (blocks * (kChunk / group) * n + n) * 4 +
+         size_t{2} * (kRowsWarps / row_warps) * n * (32 * row_warps) * 4;
+}
 
 size_t int4_smem(int n, int r, bool resident, int stages, int64_t stages_k, int64_t slots) {
   const size_t hidden = static_cast<size_t>(n) * kStageK * 2;
@@ -815,8 +1125,35 @@ size_t int4_smem(int n, int r, bool resident, int stages, int64_t stages_k, int6
 // in shared memory where they leave room for four stages of codes; where they
 // do not, their slices are read again for every tile, and tiles of 256 weight
 // rows halve that traffic.
+//
+// Up to 16 hidden rows that fit shared memory beside the sums take
+// int4_rows_kernel.  Its tiles are 32, 64 or 128 weight rows with 16, 8 or 4
+// warps along K: the height whose largest part is smallest, the higher of
+// equals (fewer sums to join).
 Int4Plan int4_plan(int64_t rows, int64_t vocab, int64_t dim, int group) {
   Int4Plan pl;
+  const int64_t blocks = (dim + kChunk - 1) / kChunk;
+  pl.n = rows <= 8 ? 8 : 16;
+  if (rows <= 16 && rows_smem(pl.n, 1, blocks, group) <= kSmemLimit) {
+    const int64_t sms = sm_count() < kMaxParts ? sm_count() : kMaxParts;
+    int64_t best = INT64_MAX;
+    pl.r = 0;
+    pl.resident = true;
+    pl.stages = 0;
+    for (int rw = 4; rw >= 1; rw /= 2) {
+      if (kRowsWarps / rw > blocks && rw < 4) break;
+      const int64_t tiles = (vocab + 32 * rw - 1) / (32 * rw);
+      const int64_t part = (tiles + sms - 1) / sms * rw;
+      if (part < best) {
+        best = part;
+        pl.row_warps = rw;
+        pl.tile_rows = 32 * rw;
+        pl.tiles = tiles;
+        pl.parts = tiles < sms ? tiles : sms;
+      }
+    }
+    return pl;
+  }
   const int most = group / 2;
   const int64_t stages_k = (dim + kStageK - 1) / kStageK, slots = stages_k * kStageK / group;
   pl.n = rows > 32 && most >= 64 ? 64 : (rows > 16 && most >= 32 ? 32 : 16);
@@ -829,7 +1166,9 @@ Int4Plan int4_plan(int64_t rows, int64_t vocab, int64_t dim, int group) {
       --pl.stages;
     if (pl.stages > 1 || pl.n == 16) break;
   }
-  pl.tiles = (vocab + pl.r * kTileV - 1) / (pl.r * kTileV);
+  pl.row_warps = 0;
+  pl.tile_rows = pl.r * kTileV;
+  pl.tiles = (vocab + pl.tile_rows - 1) / pl.tile_rows;
   pl.parts = sm_count() < kMaxParts ? sm_count() : kMaxParts;
   if (pl.tiles < pl.parts) pl.parts = pl.tiles;
   return pl;
@@ -844,10 +1183,10 @@ struct Int4Layout {
 Int4Layout int4_layout(int64_t rows, int64_t dim, int64_t vocab, int group, bool stats) {
   auto up = [](size_t x) { return (x + 1023) / 1024 * 1024; };
   const size_t padded = static_cast<size_t>((rows + 63) / 64 * 64);
-  const int64_t tiles = (vocab + kTileV - 1) / kTileV;
+  const int64_t tiles = (vocab + 31) / 32;  // of the lowest tiles
   Int4Layout l;
   l.hidden = 0;
-  l.sums = up(static_cast<size_t>(rows) * dim * 2);
+  l.sums = up(static_cast<size_t>(rows) * ((dim + kChunk - 1) / kChunk * kChunk) * 2);
   l.row_scale = l.sums + up(padded * (dim / group) * 4);
   l.records = l.row_scale + up(padded * 4);
   l.bytes = l.records + (stats ? static_cast<size_t>(tiles < kMaxParts ? tiles : kMaxParts) *
@@ -878,6 +1217,16 @@ int launch_int4(const Int4Plan& pl, const CUtensorMap& map_w, const CUtensorMap&
                      : launch_int4<T, N, S, 2, false>(map_w, map_h, p, stream);
 }
 
+template <typename T, int N, int S>
+int launch_rows(const RowsParams& p, size_t smem, cudaStream_t stream) {
+  const cudaError_t e =
+      cudaFuncSetAttribute(int4_rows_kernel<T, N, S>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           static_cast<int>(smem));
+  if (e != cudaSuccess) return record_cuda_error(e);
+  return launch_pdl(int4_rows_kernel<T, N, S>, dim3(static_cast<unsigned>(p.parts)),
+                    dim3(kRowsThreads), smem, stream, p);
+}
+
 template <typename T>
 int dispatch_int4(const void* hidden, int64_t dim, const void* packed, int group, Int4Params p,
                   const Int4Plan& pl, unsigned char* ws, const Int4Layout& l,
@@ -890,17 +1239,45 @@ int dispatch_int4(const void* hidden, int64_t dim, const void* packed, int group
   p.stages = pl.stages;
   p.sums = reinterpret_cast<const float*>(ws + l.sums);
   p.row_scale = reinterpret_cast<const float*>(ws + l.row_scale);
-  CUtensorMap map_w, map_h;
-  // codes copied as 16-bit elements, four columns each
-  int rc = make_map_sw128(&map_w, CID_DTYPE_F16, packed, dim / 4, p.vocab, dim / 4, 64, kTileV);
-  if (rc == CID_OK)
-    rc = make_map_sw128(&map_h, CID_DTYPE_F16, ws + l.hidden, dim, p.rows, dim, 64, pl.n);
-  if (rc != CID_OK) return rc;
+  const int64_t blocks = (dim + kChunk - 1) / kChunk;
+  const bool few = pl.r == 0;
   int4_prepare_kernel<T><<<static_cast<unsigned>(p.row_blocks * pl.n), kPrepThreads, 0, stream>>>(
       static_cast<const uint4*>(hidden), p.rows, static_cast<int>(dim / 8), group / 8, pl.n,
-      reinterpret_cast<uint4*>(ws + l.hidden), reinterpret_cast<float*>(ws + l.sums),
-      reinterpret_cast<float*>(ws + l.row_scale));
-  rc = launch_result();
+      static_cast<int>(few ? blocks * 16 : dim / 8), few, reinterpret_cast<uint4*>(ws + l.hidden),
+      reinterpret_cast<float*>(ws + l.sums), reinterpret_cast<float*>(ws + l.row_scale));
+  int rc = launch_result();
+  if (rc != CID_OK) return rc;
+  if (few) {
+    RowsParams q = {};
+    q.packed = static_cast<const uint32_t*>(packed);
+    q.scales = static_cast<const uint16_t*>(p.scales);
+    q.hidden = reinterpret_cast<const uint4*>(ws + l.hidden);
+    q.sums = p.sums;
+    q.row_scale = p.row_scale;
+    q.rows = p.rows;
+    q.vocab = p.vocab;
+    q.words = static_cast<int>(dim / 8);
+    q.groups = static_cast<int>(p.groups);
+    q.blocks = static_cast<int>(blocks);
+    q.row_warps = pl.row_warps;
+    q.tiles = pl.tiles;
+    q.parts = pl.parts;
+    q.out = p.out;
+    q.records = p.records;
+    q.ids = p.ids;
+    q.round_bf16 = p.round_bf16;
+    const size_t smem = rows_smem(pl.n, pl.row_warps, blocks, group);
+    if (group == 128)
+      return pl.n == 8 ? launch_rows<T, 8, 1>(q, smem, stream) : launch_rows<T, 16, 1>(q, smem, stream);
+    if (group == 64)
+      return pl.n == 8 ? launch_rows<T, 8, 2>(q, smem, stream) : launch_rows<T, 16, 2>(q, smem, stream);
+    return pl.n == 8 ? launch_rows<T, 8, 4>(q, smem, stream) : launch_rows<T, 16, 4>(q, smem, stream);
+  }
+  CUtensorMap map_w, map_h;
+  // codes copied as 16-bit elements, four columns each
+  rc = make_map_sw128(&map_w, CID_DTYPE_F16, packed, dim / 4, p.vocab, dim / 4, 64, kTileV);
+  if (rc == CID_OK)
+    rc = make_map_sw128(&map_h, CID_DTYPE_F16, ws + l.hidden, dim, p.rows, dim, 64, pl.n);
   if (rc != CID_OK) return rc;
   switch (group) {
     case 128:
@@ -1054,7 +1431,7 @@ extern "C" int cid_lm_head_quantized_display_statistics(
   // merge the parts of every row (ascending column ranges) into its statistics
   int64_t offsets[kMaxParts + 1];
   for (int64_t i = 0; i < pl.parts; ++i)
-    offsets[i] = i * pl.tiles / pl.parts * (pl.r * kTileV);
+    offsets[i] = i * pl.tiles / pl.parts * pl.tile_rows;
   offsets[pl.parts] = vocab;
   return cid_display_combine_records(records, static_cast<int>(pl.parts), offsets, token_ids,
                                      rows, confidence, predicted, current_confidence, status,
