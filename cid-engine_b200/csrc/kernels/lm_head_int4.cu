@@ -25,15 +25,12 @@
 // Two product kernels; the weight's bytes bound both up to some 64 rows (128256 x
 // 4096: 270 MB, 42 us at the copy peak).
 //
-// * Up to 16 hidden rows (int4_rows_kernel): every warp multiplies on its own,
+// * Up to 8 hidden rows (int4_rows_kernel): every warp multiplies on its own,
 //   with mma.sync (16 weight rows x 16 columns times 8 hidden rows).  A thread's
 //   16 bytes of codes from memory are its A fragments after masking, since the
 //   MMA's columns may be taken in any order that the hidden rows in shared
 //   memory follow.  No buffer changes hands between warps until a tile's sums
-//   meet, and at these sizes the legacy tensor path is fast enough (N = 16:
-//   about 29 us of HMMA beside 42 us of memory).  tcgen05 measured 96 us at 16
-//   rows: its hand-overs (codes to TMEM, MMA, accumulator back, each a barrier)
-//   cost more than the MMAs.
+//   meet, and the legacy tensor path is fast enough for 8 columns.
 // * More rows (int4_head_kernel): tcgen05 with the weight as A.  Every SM
 //   streams weight tiles with TMA; a thread owns one weight row, masks 128 of
 //   its codes into 64 registers and stores them to TMEM, which tcgen05.mma takes
@@ -662,11 +659,15 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
 }
 
 // ---------------------------------------------------------------------------
-// Up to 16 hidden rows
+// Up to 8 hidden rows
 // ---------------------------------------------------------------------------
 
 constexpr int kRowsThreads = 512;
 constexpr int kRowsWarps = kRowsThreads / 32;
+constexpr int kRowsN = 8;  // hidden rows: the MMA's columns
+// Blocks of codes a thread holds ahead.  Measured at 8 rows x 128256 x 4096:
+// groups of 128 70.4 / 66.4 / 64.3 us with 2 / 3 / 4, of 64 94.8 / 94.4 / 103.0 us.
+constexpr int kRowsRing = 3;
 constexpr int kRowsPad = 64;  // bytes between hidden rows in shared memory, past whole blocks
 
 struct RowsParams {
@@ -705,21 +706,21 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
 // Codes are read once: no line of them stays in L1.
 template <int B>
 __device__ __forceinline__ void load_codes(uint32_t* to, const uint32_t* from) {
+  static_assert(B == 4 || B == 2, "16 or 8 bytes");
   if (B == 4)
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                  : "=r"(to[0]), "=r"(to[1]), "=r"(to[2]), "=r"(to[3])
                  : "l"(from));
-  else if (B == 2)
+  else
     asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];"
                  : "=r"(to[0]), "=r"(to[1])
                  : "l"(from));
-  else
-    asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(to[0]) : "l"(from));
 }
 
-template <typename T, int N, int S>
+// kStats: statistics instead of logits (their state costs registers).
+template <typename T, int S, bool kStats>
 __global__ void __launch_bounds__(kRowsThreads, 1) int4_rows_kernel(RowsParams p) {
-  constexpr int kNB = N / 8;     // MMA columns
+  constexpr int N = kRowsN;
   constexpr int kRun = 4 / S;    // consecutive words of a group a thread takes
   extern __shared__ unsigned char smem[];
   const int pitch = p.blocks * 256 + kRowsPad;
@@ -735,41 +736,60 @@ __global__ void __launch_bounds__(kRowsThreads, 1) int4_rows_kernel(RowsParams p
   const int per_tile = (p.blocks + kws - 1) / kws;  // blocks of a warp, the last perhaps empty
   const int64_t total = (t1 - t0) * per_tile;
 
-  int64_t l_tile = t0;  // position of the next load
-  int l_k = 0;
-  auto load = [&](CodeBlock<S>& b) {
-    const int kb = kw + l_k * kws;
-    const int64_t v0 = l_tile * tile_rows + rwi * 32;
-    const bool any = l_tile < t1 && kb < p.blocks;
+  // The load's position: a tile's first row for this thread (row g of the warp's
+  // 32, its words of a group), the bytes from there to rows g + 8 r, and the block
+  // of columns.  Rows and columns past the ends read the last ones instead: such
+  // rows are not stored, such columns meet hidden values of zero.
+  const int words = p.words, groups = p.groups;
+  const int last_word = (words - kRun) * 4;
+  int64_t l_v = t0 * tile_rows + rwi * 32 + g;
+  const unsigned char* l_row = nullptr;
+  const uint16_t* l_scale = nullptr;
+  int l_off[4], l_k = 0, l_kb = kw;
+  int64_t l_tiles = t1 - t0;  // left to load
+  auto seek = [&]() {
+    const int64_t left = p.vocab - 1 - l_v;  // < 0 for a row past the last
+    const int64_t v = left < 0 ? p.vocab - 1 : l_v;
+    l_row = reinterpret_cast<const unsigned char*>(p.packed + v * words) + t * (kRun * 4);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int64_t v = v0 + g + 8 * r;
-      const uint32_t* row = p.packed + v * p.words + kb * 16;
-#pragma unroll
-      for (int i = 0; i < 4; i += kRun) {
-        // words of a group stand together: group i / kRun, words t * kRun + 0..
-        const int at = (i / kRun) * (4 * kRun) + t * kRun;
-        if (any && v < p.vocab && kb * 16 + at < p.words)
-          load_codes<kRun>(&b.w[r][i], row + at);
-        else
-          for (int j = 0; j < kRun; ++j) b.w[r][i + j] = 0;
-      }
+      const int down = left < 8 * r ? (left < 0 ? 0 : static_cast<int>(left)) : 8 * r;
+      l_off[r] = down * words * 4;
     }
-    const int64_t v = v0 + g + 8 * t;
+    const int64_t sv = l_v + 8 * t;
+    l_scale = p.scales + (sv < p.vocab ? sv : p.vocab - 1) * groups;
+  };
+  seek();
+  auto load = [&](CodeBlock<S>& b) {
+    const int kb = l_kb < p.blocks ? l_kb : p.blocks - 1;
+#pragma unroll
+    for (int i = 0; i < 4; i += kRun) {
+      // words of a group stand together: group i / kRun, words t * kRun + 0..
+      const int at = kb * 64 + i * 16;
+      const unsigned char* from = l_row + (at < last_word - t * (kRun * 4) ? at : last_word - t * (kRun * 4));
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        load_codes<kRun>(&b.w[r][i], reinterpret_cast<const uint32_t*>(from + l_off[r]));
+    }
 #pragma unroll
     for (int i = 0; i < S; ++i) {
       const int gi = kb * S + i;
-      b.scale[i] = any && v < p.vocab && gi < p.groups ? p.scales[v * p.groups + gi] : uint16_t{0};
+      b.scale[i] = l_scale[gi < groups ? gi : groups - 1];
     }
+    l_kb += kws;
     if (++l_k == per_tile) {
       l_k = 0;
-      ++l_tile;
+      l_kb = kw;
+      if (--l_tiles > 0) {
+        l_v += tile_rows;
+        seek();
+      }
     }
   };
 
-  CodeBlock<S> ring[2];
-  load(ring[0]);
-  load(ring[1]);
+  CodeBlock<S> ring[kRowsRing];
+#pragma unroll
+  for (int i = 0; i < kRowsRing; ++i) load(ring[i]);
 
   // ---- the hidden rows: from the kernel before ----
   pdl_wait();
@@ -785,7 +805,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) int4_rows_kernel(RowsParams p
   __syncthreads();
 
   // outputs of this thread: tile row tid % tile_rows, hidden rows tid / tile_rows, + step, ...
-  constexpr int kOwn = 4 * N / 16 > 1 ? 4 * N / 16 : 1;  // at most, with tiles of 128 rows
+  constexpr int kOwn = 128 * N / kRowsThreads;  // at most, with tiles of 128 rows
   const int orow = threadIdx.x % tile_rows, on = threadIdx.x / tile_rows;
   const int step = kRowsThreads / tile_rows;
   RowStats st[kOwn];
@@ -796,7 +816,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) int4_rows_kernel(RowsParams p
     cur[j] = 0.0f;
   }
 
-  float acc[2][kNB][4] = {};
+  float acc[2][4] = {};
   int64_t tile = t0;
   int k = 0, buf = 0;
   auto compute = [&](const CodeBlock<S>& b) {
@@ -805,41 +825,29 @@ __global__ void __launch_bounds__(kRowsThreads, 1) int4_rows_kernel(RowsParams p
       const unsigned char* h = hid + g * pitch + kb * 256 + t * 16;
 #pragma unroll
       for (int s = 0; s < S; ++s) {
-        float c[2][kNB][4] = {};
+        const float own = to_float(*reinterpret_cast<const T*>(&b.scale[s]));
+        float c[2][4] = {};
 #pragma unroll
         for (int i = s * kRun; i < (s + 1) * kRun; ++i) {
-          uint32_t a[4][4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) unpack8(b.w[r][i], a[r]);
-#pragma unroll
-          for (int nb = 0; nb < kNB; ++nb) {
-            const uint4 x = *reinterpret_cast<const uint4*>(h + nb * 8 * pitch + i * 64);
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-              mma_16816(c[m][nb], a[2 * m][0], a[2 * m + 1][0], a[2 * m][1], a[2 * m + 1][1], x.x,
-                        x.y);
-              mma_16816(c[m][nb], a[2 * m][2], a[2 * m + 1][2], a[2 * m][3], a[2 * m + 1][3], x.z,
-                        x.w);
-            }
-          }
-        }
-        const float own = to_float(*reinterpret_cast<const T*>(&b.scale[s]));
-        float sc[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) sc[r] = __shfl_sync(0xffffffffu, own, (lane & ~3) + r);
-        const float* gs = sums + (kb * S + s) * N + 2 * t;
-#pragma unroll
-        for (int nb = 0; nb < kNB; ++nb) {
-          const float2 h8 = *reinterpret_cast<const float2*>(gs + nb * 8);
+          const uint4 x = *reinterpret_cast<const uint4*>(h + i * 64);
 #pragma unroll
           for (int m = 0; m < 2; ++m) {
-            float* q = acc[m][nb];
-            const float* d = c[m][nb];
-            group_add2(q[0], q[1], __float_as_uint(d[0]), __float_as_uint(d[1]), h8.x, h8.y,
-                       sc[2 * m]);
-            group_add2(q[2], q[3], __float_as_uint(d[2]), __float_as_uint(d[3]), h8.x, h8.y,
-                       sc[2 * m + 1]);
+            uint32_t a0[4], a1[4];
+            unpack8(b.w[2 * m][i], a0);
+            unpack8(b.w[2 * m + 1][i], a1);
+            mma_16816(c[m], a0[0], a1[0], a0[1], a1[1], x.x, x.y);
+            mma_16816(c[m], a0[2], a1[2], a0[3], a1[3], x.z, x.w);
           }
+        }
+        const float2 h8 = *reinterpret_cast<const float2*>(sums + (kb * S + s) * N + 2 * t);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          const float s0 = __shfl_sync(0xffffffffu, own, (lane & ~3) + 2 * m);
+          const float s1 = __shfl_sync(0xffffffffu, own, (lane & ~3) + 2 * m + 1);
+          group_add2(acc[m][0], acc[m][1], __float_as_uint(c[m][0]), __float_as_uint(c[m][1]),
+                     h8.x, h8.y, s0);
+          group_add2(acc[m][2], acc[m][3], __float_as_uint(c[m][2]), __float_as_uint(c[m][3]),
+                     h8.x, h8.y, s1);
         }
       }
     }
@@ -850,13 +858,11 @@ __global__ void __launch_bounds__(kRowsThreads, 1) int4_rows_kernel(RowsParams p
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int nb = 0; nb < kNB; ++nb)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int row = rwi * 32 + m * 16 + (e >> 1) * 8 + g, n = nb * 8 + 2 * t + (e & 1);
-          rb[(kw * N + n) * tile_rows + row] = acc[m][nb][e];
-          acc[m][nb][e] = 0.0f;
-        }
+      for (int e = 0; e < 4; ++e) {
+        const int row = rwi * 32 + m * 16 + (e >> 1) * 8 + g, n = 2 * t + (e & 1);
+        rb[(kw * N + n) * tile_rows + row] = acc[m][e];
+        acc[m][e] = 0.0f;
+      }
     __syncthreads();
     // the other buffer was read before this barrier, this one is before the next
     const int64_t v = tile * tile_rows + orow;
@@ -867,7 +873,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) int4_rows_kernel(RowsParams p
         float z = 0.0f;
         for (int q = 0; q < kws; ++q) z += rb[(q * N + n) * tile_rows + orow];
         z *= rscale[n];
-        if (p.out != nullptr) {
+        if (!kStats) {
           if (v < p.vocab) {
             if (std::is_same<T, __nv_bfloat16>::value)
               static_cast<__nv_bfloat16*>(p.out)[n * p.vocab + v] = __float2bfloat16_rn(z);
@@ -888,15 +894,15 @@ __global__ void __launch_bounds__(kRowsThreads, 1) int4_rows_kernel(RowsParams p
     ++tile;
   };
 
-  for (int64_t i = 0; i < total; i += 2) {
-    compute(ring[0]);
-    load(ring[0]);
-    if (i + 1 < total) {
-      compute(ring[1]);
-      load(ring[1]);
+  for (int64_t i = 0; i < total; i += kRowsRing) {
+#pragma unroll
+    for (int r = 0; r < kRowsRing; ++r) {
+      if (i + r >= total) break;
+      compute(ring[r]);
+      load(ring[r]);
     }
   }
-  if (p.out != nullptr) return;
+  if (!kStats) return;
 
   // ---- the part's record of each hidden row: over the tile's rows ----
   __syncthreads();
@@ -941,9 +947,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1) int4_rows_kernel(RowsParams p
 // quad's thread t takes word i of its codes as columns `first + 8 t'`, see
 // int4_rows_kernel; unit (t, i) goes to 4 i + t.
 __device__ __forceinline__ int fragment_place(int u, int lanes) {
-  if (lanes == 16) return (u & 3) * 4 + (u >> 2);                         // groups of 128
-  if (lanes == 8) return ((u >> 3) * 2 + (u & 1)) * 4 + ((u >> 1) & 3);   // of 64
-  return u;                                                               // of 32
+  if (lanes == 16) return (u & 3) * 4 + (u >> 2);              // groups of 128
+  return ((u >> 3) * 2 + (u & 1)) * 4 + ((u >> 1) & 3);        // of 64
 }
 
 // One block turns one hidden row into the fp16 row of the products (`pitch` units
@@ -1107,7 +1112,8 @@ struct Int4Plan {
   int64_t tiles, parts;
 };
 
-size_t rows_smem(int n, int row_warps, int64_t blocks, int group) {
+size_t rows_smem(int row_warps, int64_t blocks, int group) {
+  constexpr int n = kRowsN;
   return n * (blocks * 256 + kRowsPad) + (blocks * (kChunk / group) * n + n) * 4 +
          size_t{2} * (kRowsWarps / row_warps) * n * (32 * row_warps) * 4;
 }
@@ -1126,15 +1132,18 @@ size_t int4_smem(int n, int r, bool resident, int stages, int64_t stages_k, int6
 // do not, their slices are read again for every tile, and tiles of 256 weight
 // rows halve that traffic.
 //
-// Up to 16 hidden rows that fit shared memory beside the sums take
-// int4_rows_kernel.  Its tiles are 32, 64 or 128 weight rows with 16, 8 or 4
-// warps along K: the height whose largest part is smallest, the higher of
-// equals (fewer sums to join).
+// Up to 8 hidden rows against groups of 64 or 128 take int4_rows_kernel, where
+// they fit shared memory beside the sums.  Measured at 8 rows x 128256 x 4096, it
+// against the other: groups of 128 70 and 97 us, of 64 95 and 109 us, of 32 (an
+// accumulator and a load for every word) 166 and 130 us; 16 rows of groups of 128
+// 114 and 97 us.  Its tiles are 32, 64 or 128 weight rows with 16, 8 or 4 warps
+// along K: the height whose largest part is smallest, the higher of equals
+// (fewer sums to join).
 Int4Plan int4_plan(int64_t rows, int64_t vocab, int64_t dim, int group) {
   Int4Plan pl;
   const int64_t blocks = (dim + kChunk - 1) / kChunk;
-  pl.n = rows <= 8 ? 8 : 16;
-  if (rows <= 16 && rows_smem(pl.n, 1, blocks, group) <= kSmemLimit) {
+  pl.n = kRowsN;
+  if (rows <= kRowsN && group >= 64 && rows_smem(1, blocks, group) <= kSmemLimit) {
     const int64_t sms = sm_count() < kMaxParts ? sm_count() : kMaxParts;
     int64_t best = INT64_MAX;
     pl.r = 0;
@@ -1217,14 +1226,20 @@ int launch_int4(const Int4Plan& pl, const CUtensorMap& map_w, const CUtensorMap&
                      : launch_int4<T, N, S, 2, false>(map_w, map_h, p, stream);
 }
 
-template <typename T, int N, int S>
+template <typename T, int S, bool kStats>
 int launch_rows(const RowsParams& p, size_t smem, cudaStream_t stream) {
-  const cudaError_t e =
-      cudaFuncSetAttribute(int4_rows_kernel<T, N, S>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           static_cast<int>(smem));
+  const cudaError_t e = cudaFuncSetAttribute(int4_rows_kernel<T, S, kStats>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             static_cast<int>(smem));
   if (e != cudaSuccess) return record_cuda_error(e);
-  return launch_pdl(int4_rows_kernel<T, N, S>, dim3(static_cast<unsigned>(p.parts)),
+  return launch_pdl(int4_rows_kernel<T, S, kStats>, dim3(static_cast<unsigned>(p.parts)),
                     dim3(kRowsThreads), smem, stream, p);
+}
+
+template <typename T, int S>
+int launch_rows(const RowsParams& p, size_t smem, cudaStream_t stream) {
+  return p.out != nullptr ? launch_rows<T, S, false>(p, smem, stream)
+                          : launch_rows<T, S, true>(p, smem, stream);
 }
 
 template <typename T>
@@ -1266,12 +1281,8 @@ int dispatch_int4(const void* hidden, int64_t dim, const void* packed, int group
     q.records = p.records;
     q.ids = p.ids;
     q.round_bf16 = p.round_bf16;
-    const size_t smem = rows_smem(pl.n, pl.row_warps, blocks, group);
-    if (group == 128)
-      return pl.n == 8 ? launch_rows<T, 8, 1>(q, smem, stream) : launch_rows<T, 16, 1>(q, smem, stream);
-    if (group == 64)
-      return pl.n == 8 ? launch_rows<T, 8, 2>(q, smem, stream) : launch_rows<T, 16, 2>(q, smem, stream);
-    return pl.n == 8 ? launch_rows<T, 8, 4>(q, smem, stream) : launch_rows<T, 16, 4>(q, smem, stream);
+    const size_t smem = rows_smem(pl.row_warps, blocks, group);
+    return group == 128 ? launch_rows<T, 1>(q, smem, stream) : launch_rows<T, 2>(q, smem, stream);
   }
   CUtensorMap map_w, map_h;
   // codes copied as 16-bit elements, four columns each
