@@ -14,13 +14,13 @@
 // c and 16 c times the smallest subnormal 2^-24.  One shift by 8 brings the
 // other two there, so eight columns cost five integer instructions.
 //
-// The MMAs therefore run in fp16 whatever the hidden rows' type: a first kernel
-// turns each hidden row into fp16 times a power of two that brings its largest
-// value to [2^14, 2^15), with the columns that meet 16 c divided by 16.  A bf16
-// value keeps its 8 bits in fp16's 11 unless it is below 2^-24 of its row's
-// largest (2^-28 where not divided), and then loses less than 2^-35 of that
-// largest, far under the f32 sum's own rounding.  The same kernel leaves 8 sum h
-// of every group, which read-back subtracts: sum c h - 8 sum h = sum q h.
+// The MMAs therefore run in fp16 whatever the hidden rows' type: each hidden row
+// is first turned into fp16 times a power of two that brings its largest
+// value to [2^14, 2^15), with the columns that meet 16 c divided by 16.  A value
+// keeps all its bits unless it is below 2^-24 of its row's largest, and then
+// loses less than 2^-35 of that largest, far under the f32 sum's own rounding.
+// 8 sum h of every group is kept beside and subtracted from the group's sum:
+// sum c h - 8 sum h = sum q h.
 //
 // Two product kernels; the weight's bytes bound both up to some 64 rows (128256 x
 // 4096: 270 MB, 42 us at the copy peak).
@@ -659,23 +659,65 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
 }
 
 // ---------------------------------------------------------------------------
+// Hidden rows in fp16
+// ---------------------------------------------------------------------------
+
+// Bits of the largest |value| of eight: |h| compares as its bits, NaN above all.
+__device__ __forceinline__ uint32_t top_bits(uint4 v) {
+  const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) top = max(top, max(u[j] & 0x7fffu, (u[j] >> 16) & 0x7fffu));
+  return top;
+}
+
+// e that brings a row's largest value to [2^14, 2^15) by 2^e.  A row of zeros or
+// one that is not finite keeps its values (the latter's logits are NaN: an
+// infinity times a code, less eight times it).
+template <typename T>
+__device__ __forceinline__ int row_exponent(uint32_t top) {
+  const uint16_t bits = static_cast<uint16_t>(top);
+  const float most = to_float(*reinterpret_cast<const T*>(&bits));
+  const int e = most > 0.0f && most < INFINITY ? 14 - ilogbf(most) : 0;
+  return e > 126 ? 126 : e;  // |h| < 2^-112
+}
+
+// Eight columns times `up` in fp16, those that meet 16 c (pairs 1 and 3)
+// divided by 16; adds what the MMAs will see of them to `sum`.
+template <typename T>
+__device__ __forceinline__ uint4 scaled_columns(uint4 v, float up, float& sum) {
+  const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+  uint32_t o[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint16_t b0 = static_cast<uint16_t>(u[j]), b1 = static_cast<uint16_t>(u[j] >> 16);
+    const float k = j & 1 ? 0.0625f : 1.0f;
+    const __half2 h = __floats2half2_rn(to_float(*reinterpret_cast<const T*>(&b0)) * up * k,
+                                        to_float(*reinterpret_cast<const T*>(&b1)) * up * k);
+    o[j] = *reinterpret_cast<const uint32_t*>(&h);
+    const float2 f = __half22float2(h);
+    sum += (f.x + f.y) * (j & 1 ? 16.0f : 1.0f);
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+// ---------------------------------------------------------------------------
 // Up to 8 hidden rows
 // ---------------------------------------------------------------------------
 
 constexpr int kRowsThreads = 512;
 constexpr int kRowsWarps = kRowsThreads / 32;
 constexpr int kRowsN = 8;  // hidden rows: the MMA's columns
-// Blocks of codes a thread holds ahead.  Measured at 8 rows x 128256 x 4096:
-// groups of 128 70.4 / 66.4 / 64.3 us with 2 / 3 / 4, of 64 94.8 / 94.4 / 103.0 us.
-constexpr int kRowsRing = 3;
+// Blocks of codes a thread holds ahead.  Measured at 8 rows x 128256 x 4096 with 2 /
+// 3 / 4: groups of 128 70.4 / 66.7 / 64.3 us, of 64 94.8 / 98.9 / 103.0 us.
+template <int S>
+constexpr int kRowsRing = S == 1 ? 4 : 2;
 constexpr int kRowsPad = 64;  // bytes between hidden rows in shared memory, past whole blocks
 
 struct RowsParams {
   const uint32_t* packed;
   const uint16_t* scales;
-  const uint4* hidden;  // prepared, in fragment order: [rows][blocks * 16]
-  const float* sums;    // [groups][N]
-  const float* row_scale;
+  const uint4* hidden;  // [rows][words]
   int64_t rows, vocab;
   int words, groups, blocks;  // a weight row's words, groups and blocks of 128 columns
   int row_warps;              // 1, 2 or 4 warps along the weight rows, the others along K
@@ -685,6 +727,14 @@ struct RowsParams {
   const int64_t* ids;
   int round_bf16;
 };
+
+// Place of 8 columns (unit u of a block of 128) in the order of the fragments: a
+// quad's thread t takes word i of its codes as columns `first + 8 t'`, see
+// int4_rows_kernel; unit (t, i) goes to 4 i + t.
+__device__ __forceinline__ int fragment_place(int u, int lanes) {
+  if (lanes == 16) return (u & 3) * 4 + (u >> 2);              // groups of 128
+  return ((u >> 3) * 2 + (u & 1)) * 4 + ((u >> 1) & 3);        // of 64
+}
 
 // A thread's codes and scales of 32 weight rows x 128 columns: rows g, g + 8,
 // g + 16, g + 24 (g = lane / 4), in each four words; the scales are those of row
@@ -787,22 +837,40 @@ __global__ void __launch_bounds__(kRowsThreads, 1) int4_rows_kernel(RowsParams p
     }
   };
 
-  CodeBlock<S> ring[kRowsRing];
+  constexpr int kRing = kRowsRing<S>;
+  CodeBlock<S> ring[kRing];
 #pragma unroll
-  for (int i = 0; i < kRowsRing; ++i) load(ring[i]);
+  for (int i = 0; i < kRing; ++i) load(ring[i]);
 
-  // ---- the hidden rows: from the kernel before ----
-  pdl_wait();
-  for (int i = threadIdx.x; i < N * p.blocks * 16; i += kRowsThreads) {
-    const int n = i / (p.blocks * 16), u = i % (p.blocks * 16);
-    const uint4 h = n < p.rows ? p.hidden[static_cast<int64_t>(n) * (p.blocks * 16) + u]
-                               : make_uint4(0, 0, 0, 0);
-    *reinterpret_cast<uint4*>(hid + n * pitch + u * 16) = h;
+  // ---- the hidden rows, two warps each, while the first codes are on their way ----
+  {
+    constexpr int lanes = 16 / S;  // that hold a group's columns
+    const int n = warp >> 1, half = warp & 1, units = p.blocks * 16;
+    uint32_t* tops = reinterpret_cast<uint32_t*>(red);
+    const uint4* src = p.hidden + static_cast<int64_t>(n) * words;
+    uint32_t top = 0;
+    if (n < p.rows)
+      for (int i = half * 32 + lane; i < words; i += 64) top = max(top, top_bits(src[i]));
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) tops[warp] = top;
+    __syncthreads();
+    const int e = row_exponent<T>(max(tops[n * 2], tops[n * 2 + 1]));
+    const float up = __int_as_float((e + 127) << 23);
+    if (half == 0 && lane == 0) rscale[n] = __int_as_float((127 - e) << 23);
+    for (int i0 = half * 32; i0 < units; i0 += 64) {
+      const int i = i0 + lane;
+      float sum = 0.0f;
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (n < p.rows && i < words) x = scaled_columns<T>(src[i], up, sum);
+      if (i < units)
+        *reinterpret_cast<uint4*>(hid + n * pitch +
+                                  ((i & ~15) + fragment_place(i & 15, lanes)) * 16) = x;
+#pragma unroll
+      for (int d = 1; d < lanes; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      if (i < units && i % lanes == 0) sums[i / lanes * N + n] = -8.0f * sum;
+    }
+    __syncthreads();
   }
-  for (int i = threadIdx.x; i < p.blocks * S * N; i += kRowsThreads)
-    sums[i] = i < p.groups * N ? -p.sums[i] : 0.0f;
-  if (threadIdx.x < N) rscale[threadIdx.x] = p.row_scale[threadIdx.x];
-  __syncthreads();
 
   // outputs of this thread: tile row tid % tile_rows, hidden rows tid / tile_rows, + step, ...
   constexpr int kOwn = 128 * N / kRowsThreads;  // at most, with tiles of 128 rows
@@ -894,9 +962,9 @@ __global__ void __launch_bounds__(kRowsThreads, 1) int4_rows_kernel(RowsParams p
     ++tile;
   };
 
-  for (int64_t i = 0; i < total; i += kRowsRing) {
+  for (int64_t i = 0; i < total; i += kRing) {
 #pragma unroll
-    for (int r = 0; r < kRowsRing; ++r) {
+    for (int r = 0; r < kRing; ++r) {
       if (i + r >= total) break;
       compute(ring[r]);
       load(ring[r]);
@@ -943,23 +1011,14 @@ __global__ void __launch_bounds__(kRowsThreads, 1) int4_rows_kernel(RowsParams p
   }
 }
 
-// Place of 8 columns (unit u of a block of 128) in the order of the fragments: a
-// quad's thread t takes word i of its codes as columns `first + 8 t'`, see
-// int4_rows_kernel; unit (t, i) goes to 4 i + t.
-__device__ __forceinline__ int fragment_place(int u, int lanes) {
-  if (lanes == 16) return (u & 3) * 4 + (u >> 2);              // groups of 128
-  return ((u >> 3) * 2 + (u & 1)) * 4 + ((u >> 1) & 3);        // of 64
-}
-
-// One block turns one hidden row into the fp16 row of the products (`pitch` units
-// of 8 columns; zeros past the last column), its group sums (8 sum h) and its
-// scale 2^-e; rows past the last get zero sums.
+// One block turns one hidden row into the fp16 row of the products, its group
+// sums (8 sum h) and its scale 2^-e; rows past the last get zero sums.
 constexpr int kPrepThreads = 256;
 
 template <typename T>
 __global__ void __launch_bounds__(kPrepThreads)
     int4_prepare_kernel(const uint4* hidden, int64_t rows, int vecs, int lanes, int n,
-                        int pitch, bool fragments, uint4* out, float* sums, float* row_scale) {
+                        uint4* out, float* sums, float* row_scale) {
   __shared__ uint32_t tops[kPrepThreads / 32];
   const int64_t r = blockIdx.x;
   const int groups = vecs / lanes;
@@ -970,48 +1029,22 @@ __global__ void __launch_bounds__(kPrepThreads)
     return;
   }
   const uint4* src = hidden + r * vecs;
-  uint32_t top = 0;  // |h| compares as its bits
-  for (int i = threadIdx.x; i < vecs; i += kPrepThreads) {
-    const uint4 v = src[i];
-    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) top = max(top, max(u[j] & 0x7fffu, (u[j] >> 16) & 0x7fffu));
-  }
+  uint32_t top = 0;
+  for (int i = threadIdx.x; i < vecs; i += kPrepThreads) top = max(top, top_bits(src[i]));
   top = __reduce_max_sync(0xffffffffu, top);
   if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kPrepThreads / 32; ++i) top = max(top, tops[i]);
-  const uint16_t bits = static_cast<uint16_t>(top);
-  const float most = to_float(*reinterpret_cast<const T*>(&bits));
-  // a row of zeros or one that is not finite keeps its values (the latter's
-  // logits are NaN: an infinity times a code, less eight times it)
-  int e = most > 0.0f && most < INFINITY ? 14 - ilogbf(most) : 0;
-  e = e > 126 ? 126 : e;  // |h| < 2^-112
+  const int e = row_exponent<T>(top);
   const float up = __int_as_float((e + 127) << 23), down = __int_as_float((127 - e) << 23);
   if (threadIdx.x == 0) row_scale[r] = down;
   // whole warps step together: a group's lanes share its sum
-  for (int i0 = 0; i0 < pitch; i0 += kPrepThreads) {
+  for (int i0 = 0; i0 < vecs; i0 += kPrepThreads) {
     const int i = i0 + static_cast<int>(threadIdx.x);
-    const int64_t to = r * pitch + (fragments ? (i & ~15) + fragment_place(i & 15, lanes) : i);
     float sum = 0.0f;
-    if (i >= vecs && i < pitch) out[to] = make_uint4(0, 0, 0, 0);
     if (i < vecs) {
-      const uint4 v = src[i];
-      const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-      uint32_t o[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint16_t b0 = static_cast<uint16_t>(u[j]), b1 = static_cast<uint16_t>(u[j] >> 16);
-        // pairs 1 and 3 of a word meet 16 c
-        const float k = j & 1 ? 0.0625f : 1.0f;
-        const __half2 h = __floats2half2_rn(to_float(*reinterpret_cast<const T*>(&b0)) * up * k,
-                                            to_float(*reinterpret_cast<const T*>(&b1)) * up * k);
-        o[j] = *reinterpret_cast<const uint32_t*>(&h);
-        const float2 f = __half22float2(h);
-        sum += (f.x + f.y) * (j & 1 ? 16.0f : 1.0f);
-      }
-      out[to] = make_uint4(o[0], o[1], o[2], o[3]);
+      out[r * vecs + i] = scaled_columns<T>(src[i], up, sum);
     }
     for (int d = 1; d < lanes; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     if (i < vecs && i % lanes == 0) my_sums[int64_t{i / lanes} * n] = 8.0f * sum;
@@ -1195,7 +1228,7 @@ Int4Layout int4_layout(int64_t rows, int64_t dim, int64_t vocab, int group, bool
   const int64_t tiles = (vocab + 31) / 32;  // of the lowest tiles
   Int4Layout l;
   l.hidden = 0;
-  l.sums = up(static_cast<size_t>(rows) * ((dim + kChunk - 1) / kChunk * kChunk) * 2);
+  l.sums = up(static_cast<size_t>(rows) * dim * 2);
   l.row_scale = l.sums + up(padded * (dim / group) * 4);
   l.records = l.row_scale + up(padded * 4);
   l.bytes = l.records + (stats ? static_cast<size_t>(tiles < kMaxParts ? tiles : kMaxParts) *
@@ -1232,8 +1265,9 @@ int launch_rows(const RowsParams& p, size_t smem, cudaStream_t stream) {
                                              cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              static_cast<int>(smem));
   if (e != cudaSuccess) return record_cuda_error(e);
-  return launch_pdl(int4_rows_kernel<T, S, kStats>, dim3(static_cast<unsigned>(p.parts)),
-                    dim3(kRowsThreads), smem, stream, p);
+  int4_rows_kernel<T, S, kStats>
+      <<<static_cast<unsigned>(p.parts), kRowsThreads, smem, stream>>>(p);
+  return launch_result();
 }
 
 template <typename T, int S>
@@ -1254,26 +1288,16 @@ int dispatch_int4(const void* hidden, int64_t dim, const void* packed, int group
   p.stages = pl.stages;
   p.sums = reinterpret_cast<const float*>(ws + l.sums);
   p.row_scale = reinterpret_cast<const float*>(ws + l.row_scale);
-  const int64_t blocks = (dim + kChunk - 1) / kChunk;
-  const bool few = pl.r == 0;
-  int4_prepare_kernel<T><<<static_cast<unsigned>(p.row_blocks * pl.n), kPrepThreads, 0, stream>>>(
-      static_cast<const uint4*>(hidden), p.rows, static_cast<int>(dim / 8), group / 8, pl.n,
-      static_cast<int>(few ? blocks * 16 : dim / 8), few, reinterpret_cast<uint4*>(ws + l.hidden),
-      reinterpret_cast<float*>(ws + l.sums), reinterpret_cast<float*>(ws + l.row_scale));
-  int rc = launch_result();
-  if (rc != CID_OK) return rc;
-  if (few) {
+  if (pl.r == 0) {
     RowsParams q = {};
     q.packed = static_cast<const uint32_t*>(packed);
     q.scales = static_cast<const uint16_t*>(p.scales);
-    q.hidden = reinterpret_cast<const uint4*>(ws + l.hidden);
-    q.sums = p.sums;
-    q.row_scale = p.row_scale;
+    q.hidden = static_cast<const uint4*>(hidden);
     q.rows = p.rows;
     q.vocab = p.vocab;
     q.words = static_cast<int>(dim / 8);
     q.groups = static_cast<int>(p.groups);
-    q.blocks = static_cast<int>(blocks);
+    q.blocks = static_cast<int>((dim + kChunk - 1) / kChunk);
     q.row_warps = pl.row_warps;
     q.tiles = pl.tiles;
     q.parts = pl.parts;
@@ -1281,9 +1305,15 @@ int dispatch_int4(const void* hidden, int64_t dim, const void* packed, int group
     q.records = p.records;
     q.ids = p.ids;
     q.round_bf16 = p.round_bf16;
-    const size_t smem = rows_smem(pl.row_warps, blocks, group);
+    const size_t smem = rows_smem(pl.row_warps, q.blocks, group);
     return group == 128 ? launch_rows<T, 1>(q, smem, stream) : launch_rows<T, 2>(q, smem, stream);
   }
+  int4_prepare_kernel<T><<<static_cast<unsigned>(p.row_blocks * pl.n), kPrepThreads, 0, stream>>>(
+      static_cast<const uint4*>(hidden), p.rows, static_cast<int>(dim / 8), group / 8, pl.n,
+      reinterpret_cast<uint4*>(ws + l.hidden), reinterpret_cast<float*>(ws + l.sums),
+      reinterpret_cast<float*>(ws + l.row_scale));
+  int rc = launch_result();
+  if (rc != CID_OK) return rc;
   CUtensorMap map_w, map_h;
   // codes copied as 16-bit elements, four columns each
   rc = make_map_sw128(&map_w, CID_DTYPE_F16, packed, dim / 4, p.vocab, dim / 4, 64, kTileV);
