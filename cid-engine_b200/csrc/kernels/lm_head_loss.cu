@@ -36,25 +36,42 @@
 namespace cid {
 namespace {
 
-constexpr int kBM = 128;  // rows of an output tile
-constexpr int kBN = 256;  // columns of an output tile
-constexpr int kBK = 64;   // K elements a stage: one 128-byte swizzle row
+constexpr int kCtaM = 128;  // rows of an output tile that one CTA holds
+constexpr int kBN = 256;    // columns of an output tile
+constexpr int kBK = 64;     // K elements a stage: one 128-byte swizzle row
 constexpr int kUmmaK = 16;
-constexpr int kStages = 4;
 constexpr int kAccBufs = 2;
 constexpr uint32_t kTmemCols = kAccBufs * kBN;
-constexpr uint32_t kStageA = kBM * kBK * 2;
-constexpr uint32_t kStageB = kBN * kBK * 2;
-constexpr uint32_t kStageBytes = kStageA + kStageB;
 constexpr uint32_t kBlockBytes = 64 * kBK * 2;  // one 64 x 64 block of an MN-major operand
-constexpr size_t kSmemBytes = kStages * size_t{kStageBytes} + 1024 + 256;
+constexpr uint32_t kStageA = kCtaM * kBK * 2;
+// Output leaves through shared memory in boxes of 32 rows x 128 bytes, two for
+// each epilogue warp.
+constexpr uint32_t kBoxBytes = 32 * 128;
+constexpr uint32_t kBoxRegion = 4 * 2 * kBoxBytes;
 constexpr int kThreads = 192;  // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
-constexpr int kRowGroup = 32;  // row blocks that share weight tiles in L2
+constexpr int kRowGroup = 4096;  // rows whose row blocks share weight tiles in L2
 constexpr int kPrepRows = 8;   // rows a prepare block packs, one a warp
 constexpr int kMaxSplits = 64;
 // Units the split of dh aims at: with four waves of 148 SMs the last wave
 // costs little, and the partial tiles stay within 75 MB.
 constexpr int64_t kSplitUnits = 592;
+
+// A CTA pair (cluster of two, tcgen05.mma.cta_group::2) computes 256 x 256
+// tiles: each CTA stages its own 128 rows of A and half of B, so operands cross
+// from L2 into shared memory at two thirds of the rate that a 128 x 256 tile by
+// one CTA needs, and each CTA keeps two accumulators in TMEM.
+template <bool kPair>
+constexpr int kTileM = kPair ? 256 : 128;
+template <bool kPair>
+constexpr uint32_t kStageB = (kPair ? 128 : 256) * kBK * 2;
+template <bool kPair>
+constexpr uint32_t kStageBytes = kStageA + kStageB<kPair>;
+template <bool kPair>
+constexpr int kStages = kPair ? 6 : 4;
+template <bool kPair>
+constexpr size_t kSmemBytes = kStages<kPair> * size_t{kStageBytes<kPair>} + kBoxRegion + 1024 + 512;
+static_assert(kSmemBytes<true> <= 227 * 1024 && kSmemBytes<false> <= 227 * 1024,
+              "shared memory of one CTA");
 
 enum Mode {
   kLoss,     // A = hidden rows, B = weight rows: (max, sum of exp) a row and tile, label logits
@@ -68,7 +85,6 @@ struct Params {
   int64_t hidden;       // H
   int64_t cols;         // vocabulary columns of this piece
   int64_t col0;         // first of them
-  int64_t pitch;        // elements between rows of d
   const int* labels;    // packed rows: label, lse, coefficients
   const float* lse;
   const float* ca;
@@ -77,10 +93,7 @@ struct Params {
   float2* records;      // [tiles][rec_stride]
   float* label_logit;   // [rec_stride]
   int64_t rec_stride;
-  void* d;              // kDlogits output
-  void* grad_weight;    // kDweight output
-  float* partial;       // kDhidden output: [split][tile] blocks of kBM x kBN floats
-  int accumulate;       // add to the partial sums of the pieces before
+  int accumulate;       // kDhidden: add to the partial sums of the pieces before
   uint32_t* status;
 };
 
@@ -103,13 +116,13 @@ struct Grid {
 // smallest.  A unit costs its slices and about kUnitCost slices of epilogue.
 // The count is fixed by a whole piece's slices, so that every piece adds to the
 // same partial tiles.
-__device__ inline int dh_splits(int64_t tiles, int kslices, int sms) {
+__device__ inline int dh_splits(int64_t tiles, int kslices, int workers) {
   constexpr int kUnitCost = 8;
   int best = 1;
   int64_t best_cost = INT64_MAX;
   for (int s = 1; s <= kMaxSplits; ++s) {
     if (s > 1 && (tiles * s > kSplitUnits || s * 8 > kslices)) break;
-    const int64_t waves = (tiles * s + sms - 1) / sms;
+    const int64_t waves = (tiles * s + workers - 1) / workers;
     const int64_t cost = waves * ((kslices + s - 1) / s + kUnitCost);
     if (cost < best_cost) {
       best_cost = cost;
@@ -119,21 +132,21 @@ __device__ inline int dh_splits(int64_t tiles, int kslices, int sms) {
   return best;
 }
 
-__device__ __forceinline__ Grid make_grid(Mode mode, const Params& p, int n) {
+__device__ __forceinline__ Grid make_grid(Mode mode, const Params& p, int n, int tile_m) {
   Grid g;
   const int64_t rows = n > 0 ? n : 1;  // one block of zero rows writes zero gradients
   if (mode == kLoss || mode == kDlogits) {
-    g.mt = (rows + kBM - 1) / kBM;
+    g.mt = (rows + tile_m - 1) / tile_m;
     g.nt = (p.cols + kBN - 1) / kBN;
     g.kslices = (p.hidden + kBK - 1) / kBK;
     g.splits = 1;
   } else if (mode == kDhidden) {
-    g.mt = (rows + kBM - 1) / kBM;
+    g.mt = (rows + tile_m - 1) / tile_m;
     g.nt = (p.hidden + kBN - 1) / kBN;
     g.kslices = (p.cols + kBK - 1) / kBK;
     g.splits = p.count[2];
   } else {
-    g.mt = (p.cols + kBM - 1) / kBM;
+    g.mt = (p.cols + tile_m - 1) / tile_m;
     g.nt = (p.hidden + kBN - 1) / kBN;
     g.kslices = (rows + kBK - 1) / kBK;
     g.splits = 1;
@@ -146,14 +159,15 @@ struct Unit {
   int64_t m, n, split, k0, k1;  // tile coordinates, K slices [k0, k1)
 };
 
-__device__ __forceinline__ Unit unit_at(Mode mode, const Grid& g, int64_t u) {
+__device__ __forceinline__ Unit unit_at(Mode mode, const Grid& g, int64_t u, int tile_m) {
   Unit x;
   if (mode == kLoss || mode == kDlogits) {
-    // groups of kRowGroup row blocks; inside one, the row blocks of a weight
-    // tile run next to each other
-    const int64_t per = kRowGroup * g.nt;
-    const int64_t gi = u / per, first = gi * kRowGroup;
-    const int64_t in = g.mt - first < kRowGroup ? g.mt - first : kRowGroup;
+    // groups of row blocks; inside one, the row blocks of a weight tile run next
+    // to each other
+    const int64_t blocks = kRowGroup / tile_m;
+    const int64_t per = blocks * g.nt;
+    const int64_t gi = u / per, first = gi * blocks;
+    const int64_t in = g.mt - first < blocks ? g.mt - first : blocks;
     const int64_t local = u - gi * per;
     x.m = first + local % in;
     x.n = local / in;
@@ -190,12 +204,12 @@ constexpr bool kBMn = kMode == kDweight || kMode == kDhidden;
 
 // Instruction descriptor of kind::f16: D f32, A and B of type T (0 fp16, 1
 // bf16), bit 15 / 16: A / B with M / N contiguous, N >> 3 at 17, M >> 4 at 24.
-template <typename T, Mode kMode>
+template <typename T, Mode kMode, bool kPair>
 __device__ __forceinline__ uint32_t idesc() {
   constexpr uint32_t t = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   return (1u << 4) | (t << 7) | (t << 10) | ((kAMn<kMode> ? 1u : 0u) << 15) |
          ((kBMn<kMode> ? 1u : 0u) << 16) | (uint32_t(kBN >> 3) << 17) |
-         (uint32_t(kBM >> 4) << 24);
+         (uint32_t(kTileM<kPair> >> 4) << 24);
 }
 
 template <typename T>
@@ -208,78 +222,151 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return r;
 }
 
-// 32 consecutive values of a row of 16-bit elements, columns c0.. of `width`
-// (a multiple of 8), 16-byte aligned.
-template <typename T>
-__device__ __forceinline__ void store32(T* row, int64_t c0, int64_t width, const float (&x)[32]) {
-#pragma unroll
-  for (int j = 0; j < 32; j += 8) {
-    if (c0 + j < width) {
-      uint4 v;
-      v.x = pack2<T>(x[j], x[j + 1]);
-      v.y = pack2<T>(x[j + 2], x[j + 3]);
-      v.z = pack2<T>(x[j + 4], x[j + 5]);
-      v.w = pack2<T>(x[j + 6], x[j + 7]);
-      *reinterpret_cast<uint4*>(row + c0 + j) = v;
-    }
-  }
+// ---- cluster and pair forms of the wrappers ----
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
 }
 
-struct EpiRow {
-  int64_t row;     // row of the output tile's matrix
-  bool valid;
-  int label;
-  float m, s;      // running maximum and sum of exp (kLoss)
-  float lse2, a, b;  // lse in base-2 exponent units, coefficients (kDlogits)
-};
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+}
+
+// The shared::cluster address of `addr` (this CTA's shared memory) in CTA `rank`.
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+
+__device__ __forceinline__ void arrive_at(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// A load into this CTA's shared memory that counts on a barrier of the pair.
+__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, int32_t x,
+                                              int32_t y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      ".cta_group::2 [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+
+template <bool kPair>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t desc,
+                                    uint32_t accumulate) {
+  if (kPair)
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(desc), "r"(accumulate)
+        : "memory");
+  else
+    umma_f16(d, a, b, desc, accumulate);
+}
+
+// Arrives on `bar`, in both CTAs of a pair, once the MMAs issued so far are done.
+template <bool kPair>
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  if (kPair)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+        " [%0], %1;" ::"r"(smem_u32(bar)),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
+  else
+    umma_commit(bar);
+}
+
+// A box from shared memory to the matrix of `map`, or added to it (f32); a group
+// of its own either way, so that waits count boxes.
+__device__ __forceinline__ void box_out(const CUtensorMap* map, int32_t x, int32_t y,
+                                        uint32_t box, bool inside, bool add) {
+  if (!inside) {
+  } else if (add)
+    asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group"
+                 " [%0, {%1, %2}], [%3];" ::"l"(reinterpret_cast<uint64_t>(map)),
+                 "r"(x), "r"(y), "r"(box)
+                 : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group"
+                 " [%0, {%1, %2}], [%3];" ::"l"(reinterpret_cast<uint64_t>(map)),
+                 "r"(x), "r"(y), "r"(box)
+                 : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
 
 // ---------------------------------------------------------------------------
-// The product kernel: one persistent CTA per SM, warp-specialised
+// The product kernel: persistent, warp-specialised, one CTA or one pair a tile
 // ---------------------------------------------------------------------------
+//
+// In a pair, both CTAs load, and read back their half of the rows; the leader
+// (rank 0) counts both CTAs' loads on its `full` barriers and issues the MMAs,
+// whose commits arrive in both.
 
-template <typename T, Mode kMode>
+template <typename T, Mode kMode, bool kPair>
 __global__ void __launch_bounds__(kThreads, 1)
     head_gemm_kernel(const __grid_constant__ CUtensorMap map_a,
-                     const __grid_constant__ CUtensorMap map_b, Params p) {
+                     const __grid_constant__ CUtensorMap map_b,
+                     const __grid_constant__ CUtensorMap map_out, Params p) {
+  constexpr int kS = kStages<kPair>;
+  constexpr int kTM = kTileM<kPair>;
   extern __shared__ unsigned char smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   unsigned char* smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
   unsigned char* stage_a = smem;
-  unsigned char* stage_b = smem + kStages * kStageA;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * kStageBytes);
-  uint64_t* empty = full + kStages;
-  uint64_t* acc_full = empty + kStages;
+  unsigned char* stage_b = smem + kS * kStageA;
+  unsigned char* boxes = smem + kS * kStageBytes<kPair>;
+  uint64_t* full = reinterpret_cast<uint64_t*>(boxes + kBoxRegion);
+  uint64_t* empty = full + kS;
+  uint64_t* acc_full = empty + kS;
   uint64_t* acc_empty = acc_full + kAccBufs;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + kAccBufs);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = kPair ? cluster_rank() : 0;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < kS; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < kAccBufs; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 4);
+      mbar_init(&acc_empty[b], kPair ? 8 : 4);
     }
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                     smem_u32(tmem_slot)),
-                 "r"(kTmemCols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if (kPair) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                       smem_u32(tmem_slot)),
+                   "r"(kTmemCols)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                       smem_u32(tmem_slot)),
+                   "r"(kTmemCols)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   }
   __syncthreads();
+  if (kPair) cluster_sync();  // the peer's barriers are initialised
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const int n = *p.count;
-  const Grid g = make_grid(kMode, p, n);
+  const Grid g = make_grid(kMode, p, n, kTM);
   const int64_t ksteps = (n > 0 ? n + kUmmaK - 1 : kUmmaK) / kUmmaK;  // of kDweight
+  const int64_t first = kPair ? blockIdx.x >> 1 : blockIdx.x;
+  const int64_t stride = kPair ? gridDim.x >> 1 : gridDim.x;
 
   if (warp == 0) {
     if (lane == 0) {
@@ -287,55 +374,65 @@ __global__ void __launch_bounds__(kThreads, 1)
       int s = 0;
       uint32_t ph = 0, issued = 0, issue_par = 0;
       bool ok = true;
-      for (int64_t u = blockIdx.x; ok && u < g.units; u += gridDim.x) {
-        const Unit x = unit_at(kMode, g, u);
+      for (int64_t u = first; ok && u < g.units; u += stride) {
+        const Unit x = unit_at(kMode, g, u, kTM);
+        const int32_t m0 = static_cast<int32_t>(x.m * kTM + rank * kCtaM);
+        const int32_t n0 = static_cast<int32_t>(x.n * kBN + rank * 128);
         for (int64_t k = x.k0; k < x.k1; ++k) {
           if (!mbar_wait(&empty[s], ph ^ 1u, abort, kWaitNs)) {
             if (!*abort) raise_abort(abort, p.status);
             ok = false;
             break;
           }
-          mbar_expect_tx(&full[s], kStageBytes);
+          uint32_t bar = smem_u32(&full[s]);
+          if (rank == 0) mbar_expect_tx(&full[s], (kPair ? 2 : 1) * kStageBytes<kPair>);
+          if (kPair) bar = map_rank(bar, 0);
+          auto load = [&](void* dst, const CUtensorMap* map, int32_t cx, int32_t cy) {
+            if (kPair)
+              tma_load_pair(dst, map, cx, cy, bar);
+            else
+              tma_load_2d(dst, map, cx, cy, &full[s]);
+          };
           unsigned char* a = stage_a + s * kStageA;
-          unsigned char* b = stage_b + s * kStageB;
+          unsigned char* b = stage_b + s * kStageB<kPair>;
           const int32_t kx = static_cast<int32_t>(k * kBK);
-          if (kMode == kDweight) {
-            for (int i = 0; i < kBM / 64; ++i)
-              tma_load_2d(a + i * kBlockBytes, &map_a, static_cast<int32_t>(x.m * kBM + i * 64),
-                          kx, &full[s]);
+          if (kAMn<kMode>) {
+            for (int i = 0; i < 2; ++i) load(a + i * kBlockBytes, &map_a, m0 + i * 64, kx);
           } else {
-            tma_load_2d(a, &map_a, kx, static_cast<int32_t>(x.m * kBM), &full[s]);
+            load(a, &map_a, kx, m0);
           }
           if (kBMn<kMode>) {
             const int32_t row = kx + (kMode == kDhidden ? static_cast<int32_t>(p.col0) : 0);
-            for (int i = 0; i < kBN / 64; ++i)
-              tma_load_2d(b + i * kBlockBytes, &map_b, static_cast<int32_t>(x.n * kBN + i * 64),
-                          row, &full[s]);
+            for (int i = 0; i < (kPair ? 2 : 4); ++i)
+              load(b + i * kBlockBytes, &map_b, n0 + i * 64, row);
           } else {
-            tma_load_2d(b, &map_b, kx, static_cast<int32_t>(p.col0 + x.n * kBN), &full[s]);
+            for (int i = 0; i < (kPair ? 1 : 2); ++i)
+              load(b + i * (128 * kBK * 2), &map_b, kx,
+                   static_cast<int32_t>(p.col0) + n0 + i * 128);
           }
           issued |= 1u << s;
           issue_par = (issue_par & ~(1u << s)) | (ph << s);
-          if (++s == kStages) {
+          if (++s == kS) {
             s = 0;
             ph ^= 1u;
           }
         }
       }
-      // copies in flight land before the CTA exits (immediate unless aborted)
-      for (int i = 0; i < kStages; ++i)
-        if (issued & (1u << i)) mbar_wait(&full[i], (issue_par >> i) & 1u, nullptr, kDrainNs);
+      // what this CTA loaded has been multiplied, and every arrival of the MMAs'
+      // commits on these barriers has landed, before the CTA exits
+      for (int i = 0; i < kS; ++i)
+        if (issued & (1u << i)) mbar_wait(&empty[i], (issue_par >> i) & 1u, nullptr, kDrainNs);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (lane == 0 && rank == 0) {
       // ---------------- MMA issuer ----------------
       int s = 0, buf = 0;
       uint32_t ph = 0, aph = 0;
       uint64_t* last_bar = nullptr;
       uint32_t last_par = 0;
       bool ok = true;
-      for (int64_t u = blockIdx.x; ok && u < g.units; u += gridDim.x) {
-        const Unit x = unit_at(kMode, g, u);
+      for (int64_t u = first; ok && u < g.units; u += stride) {
+        const Unit x = unit_at(kMode, g, u, kTM);
         if (!mbar_wait(&acc_empty[buf], aph ^ 1u, abort, kWaitNs)) {
           if (!*abort) raise_abort(abort, p.status);
           break;
@@ -350,29 +447,25 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           tc_fence_after();
           const uint32_t a0 = smem_u32(stage_a + s * kStageA);
-          const uint32_t b0 = smem_u32(stage_b + s * kStageB);
+          const uint32_t b0 = smem_u32(stage_b + s * kStageB<kPair>);
           // rows past the last step of kDweight are not zero: they are not multiplied
           const int64_t left = kMode == kDweight ? ksteps - k * (kBK / kUmmaK) : kBK / kUmmaK;
 #pragma unroll
           for (int kk = 0; kk < kBK / kUmmaK; ++kk) {
             if (kk >= left) break;
             // K advance: 32 bytes inside a K-major row, two 8-row atoms otherwise
-            const uint64_t ad =
-                kAMn<kMode> ? mn_desc(a0 + kk * 2048) : sw128_desc(a0 + kk * 32);
-            const uint64_t bd =
-                kBMn<kMode> ? mn_desc(b0 + kk * 2048) : sw128_desc(b0 + kk * 32);
-            umma_f16(d, ad, bd, idesc<T, kMode>(), (k > x.k0 || kk > 0) ? 1u : 0u);
+            const uint64_t ad = kAMn<kMode> ? mn_desc(a0 + kk * 2048) : sw128_desc(a0 + kk * 32);
+            const uint64_t bd = kBMn<kMode> ? mn_desc(b0 + kk * 2048) : sw128_desc(b0 + kk * 32);
+            mma<kPair>(d, ad, bd, idesc<T, kMode, kPair>(), (k > x.k0 || kk > 0) ? 1u : 0u);
           }
-          umma_commit(&empty[s]);
-          last_bar = &empty[s];
-          last_par = ph;
-          if (++s == kStages) {
+          commit<kPair>(&empty[s]);
+          if (++s == kS) {
             s = 0;
             ph ^= 1u;
           }
         }
         if (!ok) break;
-        umma_commit(&acc_full[buf]);
+        commit<kPair>(&acc_full[buf]);
         last_bar = &acc_full[buf];
         last_par = aph;
         if (++buf == kAccBufs) {
@@ -387,22 +480,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------- epilogue: thread = tile row, TMEM lane = tile row ----------------
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;
-    const float scale = coef_scale(p.top);
+    const float scale = coef_scale(p.top), inv = 1.0f / scale;
+    const uint32_t box0 = smem_u32(boxes) + static_cast<uint32_t>(quarter) * (2 * kBoxBytes);
+    uint32_t box = 0;  // the next of the warp's two boxes
     int buf = 0;
     uint32_t aph = 0;
-    for (int64_t u = blockIdx.x; u < g.units; u += gridDim.x) {
-      const Unit x = unit_at(kMode, g, u);
-      EpiRow e{};
-      e.row = x.m * kBM + r;
-      e.valid = e.row < (kMode == kDweight ? p.cols : n);
-      e.label = -1;
-      e.m = -INFINITY;
-      if ((kMode == kLoss || kMode == kDlogits) && e.valid) {
-        e.label = p.labels[e.row];
+    for (int64_t u = first; u < g.units; u += stride) {
+      const Unit x = unit_at(kMode, g, u, kTM);
+      const int64_t row0 = x.m * kTM + rank * kCtaM;  // the CTA's first row
+      const int64_t row = row0 + r;
+      const bool valid = row < (kMode == kDweight ? p.cols : n);
+      int label = -1;
+      float lse2 = 0.0f, ca = 0.0f, cb = 0.0f;
+      float top = -INFINITY, sum = 0.0f;
+      if ((kMode == kLoss || kMode == kDlogits) && valid) {
+        label = p.labels[row];
         if (kMode == kDlogits) {
-          e.lse2 = p.lse[e.row] * kLog2e;
-          e.a = p.ca[e.row] * scale;
-          e.b = p.cb[e.row] * scale;
+          lse2 = p.lse[row] * kLog2e;
+          ca = p.ca[row] * scale;
+          cb = p.cb[row] * scale;
         }
       }
       bool got = mbar_wait(&acc_full[buf], aph, abort, kWaitNs);
@@ -414,47 +510,41 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
                              static_cast<uint32_t>(buf * kBN);
-      float* part = nullptr;
-      if (kMode == kDhidden)
-        part = p.partial + ((x.split * g.mt + x.m) * g.nt + x.n) * (kBM * kBN) + r * kBN;
+      const int64_t width = kMode == kLoss || kMode == kDlogits ? p.cols : p.hidden;
+      const bool empty_split = kMode == kDhidden && x.k0 == x.k1;  // no product: zeros
 #pragma unroll 1
       for (int c = 0; c < kBN; c += 32) {
         const int64_t c0 = x.n * kBN + c;  // column of the output tile's matrix
-        const int64_t width = kMode == kLoss || kMode == kDlogits ? p.cols : p.hidden;
         if (c0 >= width && kMode != kDlogits) break;
         uint32_t t[32];
         tmem_issue32(taddr + static_cast<uint32_t>(c), t);
         tmem_wait32(t);
         float v[32];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(t[j]);
-        if (kMode == kDhidden && x.k0 == x.k1) {  // a split without K slices: no product
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = 0.0f;
-        }
+        for (int j = 0; j < 32; ++j) v[j] = empty_split ? 0.0f : __uint_as_float(t[j]);
         if (kMode == kLoss) {
           if (c0 + 32 > width) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
               if (c0 + j >= width) v[j] = -INFINITY;
           }
-          const int64_t rel = e.label - p.col0 - c0;
+          const int64_t rel = label - p.col0 - c0;
           if (rel >= 0 && rel < 32) {
             float at = 0.0f;
 #pragma unroll
             for (int j = 0; j < 32; ++j)
               if (j == rel) at = v[j];
-            p.label_logit[e.row] = at;
+            p.label_logit[row] = at;
           }
           float cm = v[0];
 #pragma unroll
           for (int j = 1; j < 32; ++j) cm = fmaxf(cm, v[j]);
-          if (cm > e.m) {
-            e.s = e.m == -INFINITY ? (e.s != e.s ? e.s : 0.0f) : e.s * ex2((e.m - cm) * kLog2e);
-            e.m = cm;
+          if (cm > top) {
+            sum = top == -INFINITY ? (sum != sum ? sum : 0.0f) : sum * ex2((top - cm) * kLog2e);
+            top = cm;
           }
           // a chunk of -inf alone adds nothing; NaN and +inf make the sum NaN
-          const float off = e.m == -INFINITY ? 0.0f : -e.m * kLog2e;
+          const float off = top == -INFINITY ? 0.0f : -top * kLog2e;
           float a0 = 0.0f, a1 = 0.0f, b0 = 0.0f, b1 = 0.0f;
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
@@ -464,56 +554,93 @@ __global__ void __launch_bounds__(kThreads, 1)
             add2(a0, a1, ex2(x0), ex2(x1));
             add2(b0, b1, ex2(x2), ex2(x3));
           }
-          e.s += (a0 + a1) + (b0 + b1);
-        } else if (kMode == kDlogits) {
-          const int64_t rel = e.label - p.col0 - c0;
+          sum += (a0 + a1) + (b0 + b1);
+          continue;
+        }
+        if (kMode == kDlogits) {
+          const int64_t rel = label - p.col0 - c0;
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
-            float q = e.a * ex2(fmaf(v[j], kLog2e, -e.lse2));
-            if (j == rel) q -= e.b;
-            v[j] = e.valid && c0 + j < width ? q : 0.0f;
+            float q = ca * ex2(fmaf(v[j], kLog2e, -lse2));
+            if (j == rel) q -= cb;
+            v[j] = valid && c0 + j < width ? q : 0.0f;
           }
-          store32<T>(static_cast<T*>(p.d) + e.row * p.pitch, c0, p.pitch, v);
-        } else if (kMode == kDhidden) {
-#pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            float4 o = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-            float4* q = reinterpret_cast<float4*>(part + c + j);
-            if (p.accumulate) {
-              const float4 w = *q;
-              o.x += w.x;
-              o.y += w.y;
-              o.z += w.z;
-              o.w += w.w;
-            }
-            *q = o;
-          }
-        } else if (e.valid) {
-          const float inv = 1.0f / scale;
+        } else if (kMode == kDweight) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] *= inv;
-          store32<T>(static_cast<T*>(p.grad_weight) + (p.col0 + e.row) * p.hidden, c0, p.hidden,
-                     v);
+        }
+        // into the warp's box: 16-byte pieces of a row in the 128-byte swizzle
+        constexpr bool wide = kMode == kDhidden;  // f32: 32 columns a box; 16 bits: 64
+        const bool opens = wide || (c & 32) == 0;
+        if (opens) {  // the store that read this box two boxes ago is done with it
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+          __syncwarp();
+        }
+        const uint32_t dst = box0 + box * kBoxBytes + static_cast<uint32_t>(lane) * 128;
+#pragma unroll
+        for (int j = 0; j < (wide ? 8 : 4); ++j) {
+          const uint32_t piece = wide ? j : (c & 32 ? 4 : 0) + j;
+          const uint32_t to = dst + ((piece ^ (lane & 7u)) << 4);
+          uint32_t o[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            o[e] = wide ? __float_as_uint(v[4 * j + e]) : pack2<T>(v[(8 * j + 2 * e) & 31], v[(8 * j + 2 * e + 1) & 31]);
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(o[0]), "r"(o[1]),
+                       "r"(o[2]), "r"(o[3])
+                       : "memory");
+        }
+        const bool closes = wide || (c & 32) != 0 || (kMode != kDlogits && c0 + 32 >= width);
+        if (closes) {
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            // columns past the matrix are clipped, boxes past its rows not issued
+            int64_t oy = row0 + quarter * 32, ox = c0;
+            if (kMode == kDhidden) {
+              oy = ((x.split * g.mt + x.m) * g.nt + x.n) * kTM + rank * kCtaM + quarter * 32;
+              ox = c;
+            } else {
+              ox = c0 - (c & 32);
+              if (kMode == kDweight) oy += p.col0;
+            }
+            box_out(&map_out, static_cast<int32_t>(ox), static_cast<int32_t>(oy),
+                    box0 + box * kBoxBytes,
+                    kMode != kDweight || row0 + quarter * 32 < p.cols,
+                    kMode == kDhidden && p.accumulate);
+          }
+          box ^= 1u;
         }
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty[buf]);
+      if (lane == 0) {
+        if (kPair)
+          arrive_at(map_rank(smem_u32(&acc_empty[buf]), 0));
+        else
+          mbar_arrive(&acc_empty[buf]);
+      }
       if (++buf == kAccBufs) {
         buf = 0;
         aph ^= 1u;
       }
-      if (kMode == kLoss && e.valid)
-        p.records[x.n * p.rec_stride + e.row] = make_float2(e.m, e.s);
+      if (kMode == kLoss && valid) p.records[x.n * p.rec_stride + row] = make_float2(top, sum);
     }
+    if (kMode != kLoss && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
   }
 
   __syncthreads();
+  if (kPair) cluster_sync();  // no arrival or load for this CTA is under way
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base),
-                 "r"(kTmemCols)
-                 : "memory");
+    if (kPair)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base),
+                   "r"(kTmemCols)
+                   : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base),
+                   "r"(kTmemCols)
+                   : "memory");
   }
 }
 
@@ -540,7 +667,7 @@ struct PrepParams {
   float* pb;
   uint32_t* top;           // fp16 backward: bits of the largest |coefficient|
   int* count;              // [0] kept rows, [2] K splits of dh
-  int piece_slices, sms;   // K slices of a whole piece of dh, SMs
+  int piece_slices, tile_m, workers;  // K slices of a whole piece of dh, rows of a tile, CTAs or pairs
   uint32_t* status;
 };
 
@@ -604,20 +731,23 @@ __global__ void __launch_bounds__(32 * kPrepRows) head_prepare_kernel(PrepParams
     for (int64_t i = n * p.vecs + threadIdx.x; i < pad * p.vecs; i += blockDim.x)
       p.packed[i] = make_uint4(0, 0, 0, 0);
     if (threadIdx.x == 0) {
-      const int64_t mt = ((n > 0 ? n : 1) + kBM - 1) / kBM;
+      const int64_t mt = ((n > 0 ? n : 1) + p.tile_m - 1) / p.tile_m;
       const int64_t nt = (p.vecs * 8 + kBN - 1) / kBN;
       p.count[0] = n;
-      p.count[2] = dh_splits(mt * nt, p.piece_slices, p.sms);
+      p.count[2] = dh_splits(mt * nt, p.piece_slices, p.workers);
     }
   }
 }
 
-// loss and log-sum-exp of 32 rows a block from the tiles' (max, sum of exp)
-__global__ void __launch_bounds__(256)
+// loss and log-sum-exp of 32 rows a block from the tiles' (max, sum of exp), the
+// tiles dealt to kLossParts warps
+constexpr int kLossParts = 32;
+
+__global__ void __launch_bounds__(32 * kLossParts)
     head_loss_kernel(const float2* records, int64_t tiles, int64_t rec_stride,
                      const float* label_logit, const int* slot_of, int64_t rows, float* loss,
                      float* lse) {
-  __shared__ float sm[8][32], ss[8][32];
+  __shared__ float sm[kLossParts][32], ss[kLossParts][32];
   const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
   const int64_t r = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   const int slot = r < rows ? slot_of[r] : kIgnored;
@@ -633,15 +763,20 @@ __global__ void __launch_bounds__(256)
     m = nm;
   };
   if (slot >= 0)
-    for (int64_t t = part; t < tiles; t += 8) {
-      const float2 q = records[t * rec_stride + slot];
-      merge(q.x, q.y);
+    for (int64_t t = part; t < tiles; t += 4 * kLossParts) {
+      float2 q[4];  // four loads in flight
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        q[i] = t + i * kLossParts < tiles ? records[(t + i * kLossParts) * rec_stride + slot]
+                                          : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) merge(q[i].x, q[i].y);
     }
   sm[part][lane] = m;
   ss[part][lane] = s;
   __syncthreads();
   if (part == 0 && r < rows) {
-    for (int i = 1; i < 8; ++i) merge(sm[i][lane], ss[i][lane]);
+    for (int i = 1; i < kLossParts; ++i) merge(sm[i][lane], ss[i][lane]);
     if (slot >= 0) {
       const float l = m + logf(s);
       lse[r] = l;
@@ -659,12 +794,11 @@ __global__ void __launch_bounds__(256)
 template <typename T>
 __global__ void __launch_bounds__(256)
     head_dhidden_kernel(const float* partial, const int* slot_of, const int* count,
-                        int64_t hidden, const uint32_t* top,
-                        T* out) {
+                        int64_t hidden, int tile_m, const uint32_t* top, T* out) {
   const int64_t r = blockIdx.x;
   const int slot = slot_of[r];
   const int64_t n = *count;
-  const int64_t mt = ((n > 0 ? n : 1) + kBM - 1) / kBM, nt = (hidden + kBN - 1) / kBN;
+  const int64_t mt = ((n > 0 ? n : 1) + tile_m - 1) / tile_m, nt = (hidden + kBN - 1) / kBN;
   const int splits = count[2];
   const float inv = 1.0f / coef_scale(top);
   for (int64_t c = threadIdx.x * 8; c < hidden; c += blockDim.x * 8) {
@@ -672,9 +806,9 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = slot == kBadLabel ? __int_as_float(0x7fffffff) : 0.0f;
     if (slot >= 0) {
-      const int64_t tile = (slot / kBM) * nt + c / kBN;
-      const float* q = partial + tile * (kBM * kBN) + (slot % kBM) * kBN + c % kBN;
-      for (int s = 0; s < splits; ++s, q += mt * nt * (kBM * kBN)) {
+      const int64_t tile = (slot / tile_m) * nt + c / kBN, size = tile_m * kBN;
+      const float* q = partial + tile * size + (slot % tile_m) * kBN + c % kBN;
+      for (int s = 0; s < splits; ++s, q += mt * nt * size) {
         const float4 x = reinterpret_cast<const float4*>(q)[0];
         const float4 y = reinterpret_cast<const float4*>(q)[1];
         v[0] += x.x;
@@ -700,16 +834,22 @@ __global__ void __launch_bounds__(256)
 // Host
 // ---------------------------------------------------------------------------
 
-constexpr int64_t kMaxLossRows = INT32_MAX - 2 * kBM;
+constexpr int64_t kMaxLossRows = INT32_MAX - 512;
 
 int64_t round_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
+
+// Rows above which a pair computes a tile: at most 128 rows fill half a pair's
+// tile, and then memory is what counts.
+bool use_pair(int64_t rows) { return rows > kCtaM; }
+
+int64_t padded_rows(int64_t rows) { return round_up(rows, use_pair(rows) ? 256 : 128); }
 
 // Vocabulary columns of a piece of the backward: d of 64 MB stays in L2
 // between the kernel that writes it and the two that read it, and no fewer
 // than 4096 columns, below which a piece has too few tiles for the SMs.
 int64_t piece_cols(int64_t rows, int64_t vocab) {
   constexpr int64_t kPieceBytes = 64 << 20;
-  int64_t c = kPieceBytes / (2 * round_up(rows, kBM)) / kBN * kBN;
+  int64_t c = kPieceBytes / (2 * padded_rows(rows)) / kBN * kBN;
   if (c < 4096) c = 4096;
   const int64_t all = round_up(vocab, kBN);
   return c < all ? c : all;
@@ -718,6 +858,7 @@ int64_t piece_cols(int64_t rows, int64_t vocab) {
 // Byte offsets of the workspace's parts.
 struct Layout {
   size_t count, slot_of, plabel, plse, pa, pb, label_logit, packed, records, d, partial, bytes;
+  int64_t partial_rows;
 };
 
 Layout layout(int64_t rows, int64_t hidden, int64_t vocab, bool backward) {
@@ -728,7 +869,7 @@ Layout layout(int64_t rows, int64_t hidden, int64_t vocab, bool backward) {
     at += static_cast<size_t>(round_up(bytes, 1024));
     return here;
   };
-  const int64_t padded = round_up(rows, kBM);
+  const int64_t padded = padded_rows(rows), tile_m = use_pair(rows) ? 256 : 128;
   l.count = take(16);  // count, top, splits
   l.slot_of = take(rows * 4);
   l.plabel = take(padded * 4);
@@ -741,31 +882,64 @@ Layout layout(int64_t rows, int64_t hidden, int64_t vocab, bool backward) {
     l.pa = take(padded * 4);
     l.pb = take(padded * 4);
     l.d = take(padded * piece_cols(rows, vocab) * 2);
-    const int64_t tiles = padded / kBM * ((hidden + kBN - 1) / kBN);
-    l.partial = take((tiles > kSplitUnits ? tiles : kSplitUnits) * kBM * kBN * 4);
+    const int64_t tiles = padded / tile_m * ((hidden + kBN - 1) / kBN);
+    l.partial_rows = (tiles > kSplitUnits ? tiles : kSplitUnits) * tile_m;
+    l.partial = take(l.partial_rows * kBN * 4);
   }
   l.bytes = at;
   return l;
 }
 
 bool loss_extents_ok(int64_t rows, int64_t hidden, int64_t vocab) {
-  int64_t n = 0;
-  return rows >= 0 && rows <= kMaxLossRows && hidden > 0 && hidden % 8 == 0 &&
-         hidden <= INT32_MAX - kBN && vocab > 0 && vocab <= INT32_MAX - kBN &&
-         count_ok(rows, hidden, &n) && n <= kMaxCount && count_ok(vocab, hidden, &n) &&
-         n <= kMaxCount && count_ok((vocab + kBN - 1) / kBN, rows, &n) && n <= kMaxCount;
+  int64_t n = 0, tiles = 0;
+  if (!(rows >= 0 && rows <= kMaxLossRows && hidden > 0 && hidden % 8 == 0 &&
+        hidden <= INT32_MAX - kBN && vocab > 0 && vocab <= INT32_MAX - kBN &&
+        count_ok(rows, hidden, &n) && n <= kMaxCount && count_ok(vocab, hidden, &n) &&
+        n <= kMaxCount && count_ok((vocab + kBN - 1) / kBN, rows, &n) && n <= kMaxCount))
+    return false;
+  // rows of the partial tiles of dh: a tensor map's extent
+  tiles = (rows + 127) / 128 * ((hidden + kBN - 1) / kBN);
+  return tiles <= INT32_MAX / 512;
 }
 
-template <typename T, Mode kMode>
-int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const Params& p, int64_t grid,
-                cudaStream_t stream) {
-  const cudaError_t e = cudaFuncSetAttribute(head_gemm_kernel<T, kMode>,
+template <typename T, Mode kMode, bool kPair>
+int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out,
+                const Params& p, int64_t units, cudaStream_t stream) {
+  const cudaError_t e = cudaFuncSetAttribute(head_gemm_kernel<T, kMode, kPair>,
                                              cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             static_cast<int>(kSmemBytes));
+                                             static_cast<int>(kSmemBytes<kPair>));
   if (e != cudaSuccess) return record_cuda_error(e);
-  head_gemm_kernel<T, kMode>
-      <<<static_cast<unsigned>(grid), kThreads, kSmemBytes, stream>>>(a, b, p);
-  return launch_result();
+  const int64_t workers = kPair ? sm_count() / 2 : sm_count();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((units < workers ? units : workers) * (kPair ? 2 : 1)));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmemBytes<kPair>;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kPair ? 2 : 1;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return record_cuda_error(
+      cudaLaunchKernelEx(&cfg, head_gemm_kernel<T, kMode, kPair>, a, b, out, p));
+}
+
+// 2-D f32 map of the partial tiles, boxes of 32 x 32.
+int make_partial_map(CUtensorMap* map, void* base, int64_t rows) {
+  auto encode = tensor_map_encoder();
+  if (encode == nullptr) return record_cuda_error(cudaErrorNotSupported);
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(kBN), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(kBN) * 4};
+  cuuint32_t box[2] = {32, 32};
+  cuuint32_t estr[2] = {1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, base, dims, strides, box, estr,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? CID_OK
+             : CID_ERR_INVALID_ARGUMENT;
 }
 
 struct Call {
@@ -801,7 +975,8 @@ int launch_prepare(const Call& c, const Layout& l, const float* lse, const float
   q.pb = reinterpret_cast<float*>(c.ws + l.pb);
   q.count = reinterpret_cast<int*>(c.ws + l.count);
   q.piece_slices = static_cast<int>(piece_cols(c.rows, c.vocab) / kBK);
-  q.sms = sm_count();
+  q.tile_m = use_pair(c.rows) ? 256 : 128;
+  q.workers = use_pair(c.rows) ? sm_count() / 2 : sm_count();
   q.status = c.status;
   if (scaled) {
     q.top = reinterpret_cast<uint32_t*>(c.ws + l.count) + 1;
@@ -813,16 +988,16 @@ int launch_prepare(const Call& c, const Layout& l, const float* lse, const float
   return launch_result();
 }
 
-template <typename T>
+template <typename T, bool kPair>
 int run_loss(const Call& c, float* loss, float* lse) {
   const Layout l = layout(c.rows, c.dim, c.vocab, false);
-  const int64_t padded = round_up(c.rows, kBM);
+  const int64_t padded = padded_rows(c.rows);
   int rc = launch_prepare(c, l, nullptr, nullptr, nullptr, false);
   if (rc != CID_OK) return rc;
   CUtensorMap map_a, map_b;
-  rc = make_map_sw128(&map_a, c.dtype, c.ws + l.packed, c.dim, padded, c.dim, kBK, kBM);
+  rc = make_map_sw128(&map_a, c.dtype, c.ws + l.packed, c.dim, padded, c.dim, kBK, 128);
   if (rc == CID_OK)
-    rc = make_map_sw128(&map_b, c.dtype, c.weight, c.dim, c.vocab, c.dim, kBK, kBN);
+    rc = make_map_sw128(&map_b, c.dtype, c.weight, c.dim, c.vocab, c.dim, kBK, 128);
   if (rc != CID_OK) return rc;
   Params p = {};
   p.count = reinterpret_cast<const int*>(c.ws + l.count);
@@ -834,66 +1009,82 @@ int run_loss(const Call& c, float* loss, float* lse) {
   p.rec_stride = padded;
   p.status = c.status;
   const int64_t tiles = (c.vocab + kBN - 1) / kBN;
-  const int64_t units = padded / kBM * tiles;
-  rc = launch_gemm<T, kLoss>(map_a, map_b, p, units < sm_count() ? units : sm_count(), c.stream);
+  rc = launch_gemm<T, kLoss, kPair>(map_a, map_b, map_a, p, padded / kTileM<kPair> * tiles,
+                                    c.stream);
   if (rc != CID_OK) return rc;
-  head_loss_kernel<<<static_cast<unsigned>((c.rows + 31) / 32), 256, 0, c.stream>>>(
+  head_loss_kernel<<<static_cast<unsigned>((c.rows + 31) / 32), 32 * kLossParts, 0, c.stream>>>(
       p.records, tiles, padded, p.label_logit, reinterpret_cast<const int*>(c.ws + l.slot_of),
       c.rows, loss, lse);
   return launch_result();
 }
 
-template <typename T>
+template <typename T, bool kPair>
 int run_backward(const Call& c, const float* lse, const float* grad_loss, const float* grad_lse,
                  void* grad_hidden, void* grad_weight) {
   const Layout l = layout(c.rows, c.dim, c.vocab, true);
-  const int64_t padded = round_up(c.rows, kBM);
+  const int64_t padded = padded_rows(c.rows);
   const int64_t piece = piece_cols(c.rows, c.vocab);
   const bool scaled = c.dtype == CID_DTYPE_F16;
-  const int sms = sm_count();
   int rc = launch_prepare(c, l, lse, grad_loss, grad_lse, scaled);
   if (rc != CID_OK) return rc;
-  CUtensorMap h_k, h_mn, w_k, w_mn, d_k, d_mn;
-  rc = make_map_sw128(&h_k, c.dtype, c.ws + l.packed, c.dim, padded, c.dim, kBK, kBM);
-  if (rc == CID_OK)
-    rc = make_map_sw128(&h_mn, c.dtype, c.ws + l.packed, c.dim, padded, c.dim, 64, kBK);
-  if (rc == CID_OK) rc = make_map_sw128(&w_k, c.dtype, c.weight, c.dim, c.vocab, c.dim, kBK, kBN);
-  if (rc == CID_OK) rc = make_map_sw128(&w_mn, c.dtype, c.weight, c.dim, c.vocab, c.dim, 64, kBK);
-  if (rc == CID_OK) rc = make_map_sw128(&d_k, c.dtype, c.ws + l.d, piece, padded, piece, kBK, kBM);
-  if (rc == CID_OK) rc = make_map_sw128(&d_mn, c.dtype, c.ws + l.d, piece, padded, piece, 64, kBK);
+  unsigned char* d = c.ws + l.d;
+  CUtensorMap h_k, h_mn, w_k, w_mn, d_k, d_mn, d_out, dw_out, dh_out;
+  auto map = [&](CUtensorMap* m, const void* base, int64_t inner, int64_t outer, int box) {
+    if (rc == CID_OK) rc = make_map_sw128(m, c.dtype, base, inner, outer, inner, 64, box);
+  };
+  map(&h_k, c.ws + l.packed, c.dim, padded, 128);
+  map(&h_mn, c.ws + l.packed, c.dim, padded, kBK);
+  map(&w_k, c.weight, c.dim, c.vocab, 128);
+  map(&w_mn, c.weight, c.dim, c.vocab, kBK);
+  map(&d_k, d, piece, padded, 128);
+  map(&d_mn, d, piece, padded, kBK);
+  map(&d_out, d, piece, padded, 32);
+  if (grad_weight != nullptr) map(&dw_out, grad_weight, c.dim, c.vocab, 32);
+  if (rc == CID_OK) rc = make_partial_map(&dh_out, c.ws + l.partial, l.partial_rows);
   if (rc != CID_OK) return rc;
   Params p = {};
   p.count = reinterpret_cast<const int*>(c.ws + l.count);
   p.hidden = c.dim;
-  p.pitch = piece;
   p.labels = reinterpret_cast<const int*>(c.ws + l.plabel);
   p.lse = reinterpret_cast<const float*>(c.ws + l.plse);
   p.ca = reinterpret_cast<const float*>(c.ws + l.pa);
   p.cb = reinterpret_cast<const float*>(c.ws + l.pb);
   p.top = scaled ? reinterpret_cast<const uint32_t*>(c.ws + l.count) + 1 : nullptr;
-  p.d = c.ws + l.d;
-  p.grad_weight = grad_weight;
-  p.partial = reinterpret_cast<float*>(c.ws + l.partial);
   p.status = c.status;
-  const int64_t mt = padded / kBM, ht = (c.dim + kBN - 1) / kBN;
+  constexpr int kTM = kTileM<kPair>;
+  const int64_t mt = padded / kTM, ht = (c.dim + kBN - 1) / kBN;
   for (int64_t c0 = 0; c0 < c.vocab; c0 += piece) {
     p.col0 = c0;
     p.cols = c.vocab - c0 < piece ? c.vocab - c0 : piece;
     p.accumulate = c0 > 0;
-    const int64_t nt = (p.cols + kBN - 1) / kBN;
-    auto grid = [&](int64_t units) { return units < sms ? units : sms; };
-    rc = launch_gemm<T, kDlogits>(h_k, w_k, p, grid(mt * nt), c.stream);
+    rc = launch_gemm<T, kDlogits, kPair>(h_k, w_k, d_out, p, mt * ((p.cols + kBN - 1) / kBN),
+                                         c.stream);
     if (rc == CID_OK && grad_hidden != nullptr)
-      rc = launch_gemm<T, kDhidden>(d_k, w_mn, p, sms, c.stream);
+      rc = launch_gemm<T, kDhidden, kPair>(d_k, w_mn, dh_out, p, INT32_MAX, c.stream);
     if (rc == CID_OK && grad_weight != nullptr)
-      rc = launch_gemm<T, kDweight>(d_mn, h_mn, p, grid((p.cols + kBM - 1) / kBM * ht), c.stream);
+      rc = launch_gemm<T, kDweight, kPair>(d_mn, h_mn, dw_out, p, (p.cols + kTM - 1) / kTM * ht,
+                                           c.stream);
     if (rc != CID_OK) return rc;
   }
   if (grad_hidden == nullptr) return CID_OK;
   head_dhidden_kernel<T><<<static_cast<unsigned>(c.rows), 256, 0, c.stream>>>(
-      p.partial, reinterpret_cast<const int*>(c.ws + l.slot_of), p.count, c.dim,
-      p.top, static_cast<T*>(grad_hidden));
+      reinterpret_cast<const float*>(c.ws + l.partial),
+      reinterpret_cast<const int*>(c.ws + l.slot_of), p.count, c.dim, kTM, p.top,
+      static_cast<T*>(grad_hidden));
   return launch_result();
+}
+
+template <typename T>
+int run_loss(const Call& c, float* loss, float* lse) {
+  return use_pair(c.rows) ? run_loss<T, true>(c, loss, lse) : run_loss<T, false>(c, loss, lse);
+}
+
+template <typename T>
+int run_backward(const Call& c, const float* lse, const float* grad_loss, const float* grad_lse,
+                 void* grad_hidden, void* grad_weight) {
+  return use_pair(c.rows)
+             ? run_backward<T, true>(c, lse, grad_loss, grad_lse, grad_hidden, grad_weight)
+             : run_backward<T, false>(c, lse, grad_loss, grad_lse, grad_hidden, grad_weight);
 }
 
 int check_loss(cid_dtype_t dtype, const void* hidden, int64_t rows, int64_t dim,
