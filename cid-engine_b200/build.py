@@ -91,7 +91,7 @@ def build(force: bool = False, jobs: int | None = None) -> Path:
         f"-I{tinc / 'torch' / 'csrc' / 'api' / 'include'}", f"-I{CUDA_HOME / 'include'}",
         f"-I{py_inc}",
     ]
-    cpp_sources = [CSRC / n for n in ("ops.cpp", "refine.cpp", "registration.cpp", "bindings.cpp")]
+    cpp_sources = [CSRC / n for n in ("ops.cpp", "refine.cpp", "autograd.cpp", "registration.cpp", "bindings.cpp")]
     cpp_objs = [BUILD / (s.stem + ".cpp.o") for s in cpp_sources]
     todo_cpp = [
         (s, o) for s, o in zip(cpp_sources, cpp_objs) if force or _stale(o, [s, *headers])

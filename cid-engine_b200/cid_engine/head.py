@@ -3,8 +3,8 @@
 * ``lm_head_cross_entropy``: softmax cross entropy over the vocabulary without
   the logits, differentiable.  The reference stops at the corruption that makes
   the labels (``csrc/ops.cpp:292-444`` of fwerkor/cid-engine v1.1.0); the loss
-  over them is the step that follows.  The operators are registered by ``_C``;
-  this module registers their autograd formula.
+  over them is the step that follows.  The operators and their
+  autograd formula are registered by ``_C``.
 * ``QuantizedLMHead`` and the operators on it: the head's weight as 4-bit codes
   with a scale for each group of columns, its logits, and the display
   statistics over them (``csrc/ops.cpp:446-474`` takes materialised logits).
@@ -42,35 +42,6 @@ def lm_head_cross_entropy(
     penalty of the log-sum-exp.  The backward computes the logits again, a
     piece of the vocabulary at a time."""
     return torch.ops.cid_engine.lm_head_cross_entropy(labels, hidden, weight, ignore_index)
-
-
-def _setup(ctx, inputs, output) -> None:
-    labels, hidden, weight, ignore_index = inputs
-    ctx.ignore_index = ignore_index
-    ctx.set_materialize_grads(False)
-    ctx.save_for_backward(labels, hidden, weight, output[1])
-
-
-def _backward(ctx, grad_loss, grad_lse):
-    labels, hidden, weight, lse = ctx.saved_tensors
-    need_hidden, need_weight = ctx.needs_input_grad[1:3]
-    if grad_loss is None and grad_lse is None:
-        return None, None, None, None
-    gh, gw = torch.ops.cid_engine.lm_head_cross_entropy_backward(
-        grad_loss, grad_lse, labels, hidden, weight, lse, ctx.ignore_index,
-        need_hidden, need_weight)
-    return None, gh if need_hidden else None, gw if need_weight else None, None
-
-
-def _no_second_backward(ctx, *grads):
-    raise RuntimeError("cid_engine.lm_head_cross_entropy is differentiable once: "
-                       "its gradient has no gradient")
-
-
-torch.library.register_autograd("cid_engine::lm_head_cross_entropy", _backward,
-                                setup_context=_setup)
-torch.library.register_autograd("cid_engine::lm_head_cross_entropy_backward",
-                                _no_second_backward)
 
 
 class QuantizedLMHead(NamedTuple):

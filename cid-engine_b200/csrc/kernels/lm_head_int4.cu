@@ -85,6 +85,16 @@ struct Int4Params {
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 
+template <typename T>
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
+  uint32_t r;
+  if (std::is_same<T, __nv_bfloat16>::value)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
 // Stores 32 registers to 32 consecutive columns of this thread's TMEM lane.
 __device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t* q) {
   asm volatile(
@@ -1056,67 +1066,102 @@ __global__ void __launch_bounds__(kPrepThreads)
 // ---------------------------------------------------------------------------
 
 constexpr int kQuantThreads = 256;
+constexpr int kQuantWords = 4;  // words a thread, a block apart: loads in flight
+constexpr int64_t kQuantBlock = kQuantThreads * kQuantWords;
+
+// Code of w for scale s and r = 1 / s rounded: rint(w / s), ties to even, without a
+// division.  The sum with 1.5 2^23 rounds w r to an integer q; it can differ from
+// the rounded quotient only where w / s is a tie (no other quotient of two 11-bit
+// numbers is nearer to one than 2^-13), and there the remainder w - q s, exact in
+// f32, is half of s: then an odd q moves to the even neighbour on its side.
+__device__ __forceinline__ uint32_t code_of(float w, float s, float r) {
+  const float t = fmaf(w, r, 12582912.0f);
+  float q = t - 12582912.0f;
+  const float rest = fmaf(-q, s, w);
+  if (2.0f * fabsf(rest) == s && (__float_as_uint(t) & 1u)) q += copysignf(1.0f, rest);
+  // 1.5 2^23 + 8 + q in [0, 15]: the code is the low bits
+  return __float_as_uint(fminf(fmaxf(q, -8.0f), 7.0f) + 12582920.0f) & 15u;
+}
 
 // A lane holds 8 columns (16 bytes) and writes their word; the group's lanes
 // (4, 8 or 16) share the maximum.  |w| compares as its bits, NaN above all, so
 // a NaN or infinite weight leaves its group's scale NaN or infinite.
+// Bound by memory: 2.5 bytes a weight.
 template <typename T>
 __global__ void __launch_bounds__(kQuantThreads)
-    quantize_kernel(const uint4* weight, int64_t words, int lanes, uint32_t* packed, T* scales) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kQuantThreads + threadIdx.x;
-  // words is a multiple of 4, a group's lanes are in range together
-  const uint4 v = i < words ? weight[i] : make_uint4(0, 0, 0, 0);
-  const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-  uint32_t top = 0;
+    quantize_kernel(const uint4* weight, int64_t words, int lanes_log2, uint32_t* packed,
+                    T* scales) {
+  const int64_t first = blockIdx.x * kQuantBlock + threadIdx.x;
+  const int lanes = 1 << lanes_log2;
+  uint4 v[kQuantWords];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) top = max(top, max(u[j] & 0x7fffu, (u[j] >> 16) & 0x7fffu));
-  for (int d = 1; d < lanes; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
-  if (i >= words) return;
-  const uint16_t bits = static_cast<uint16_t>(top);
-  const float amax = to_float(*reinterpret_cast<const T*>(&bits));
-  T scale;
-  if (std::is_same<T, __nv_bfloat16>::value)
-    *reinterpret_cast<__nv_bfloat16*>(&scale) = __float2bfloat16_rn(__fdiv_rn(amax, 7.0f));
-  else
-    *reinterpret_cast<__half*>(&scale) = __float2half_rn(__fdiv_rn(amax, 7.0f));
-  const float s = to_float(scale);
-  uint32_t word = 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint16_t b = static_cast<uint16_t>(u[j] >> (16 * h));
-      float q = 0.0f;
-      if (s > 0.0f && s < INFINITY) {
-        q = rintf(__fdiv_rn(to_float(*reinterpret_cast<const T*>(&b)), s));
-        q = fminf(fmaxf(q, -8.0f), 7.0f);
-      }
-      word |= static_cast<uint32_t>(static_cast<int>(q) + 8) << (4 * j + 16 * h);
-    }
+  for (int k = 0; k < kQuantWords; ++k) {
+    const int64_t i = first + k * kQuantThreads;
+    // words is a multiple of 4, a group's lanes are in range together
+    v[k] = i < words ? __ldcs(weight + i) : make_uint4(0, 0, 0, 0);
   }
-  packed[i] = word;
-  if (i % lanes == 0) scales[i / lanes] = scale;
+#pragma unroll
+  for (int k = 0; k < kQuantWords; ++k) {
+    const int64_t i = first + k * kQuantThreads;
+    const uint32_t u[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+    uint32_t top = top_bits(v[k]);
+    for (int d = 1; d < lanes; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+    if (i >= words) continue;
+    const uint16_t bits = static_cast<uint16_t>(top);
+    const float amax = to_float(*reinterpret_cast<const T*>(&bits));
+    T scale;
+    if (std::is_same<T, __nv_bfloat16>::value)
+      *reinterpret_cast<__nv_bfloat16*>(&scale) = __float2bfloat16_rn(__fdiv_rn(amax, 7.0f));
+    else
+      *reinterpret_cast<__half*>(&scale) = __float2half_rn(__fdiv_rn(amax, 7.0f));
+    float s = to_float(scale);
+    // below 2^-100 the reciprocal could overflow: scale and weights grow alike
+    const float grow = s < 7.9e-31f ? 1.2676506e30f : 1.0f;  // 2^100
+    s *= grow;
+    const bool usable = s > 0.0f && s < INFINITY;
+    const float r = usable ? __frcp_rn(s) : 0.0f;
+    uint32_t word = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint16_t b0 = static_cast<uint16_t>(u[j]), b1 = static_cast<uint16_t>(u[j] >> 16);
+      const float w0 = to_float(*reinterpret_cast<const T*>(&b0)) * grow;
+      const float w1 = to_float(*reinterpret_cast<const T*>(&b1)) * grow;
+      word |= code_of(w0, s, r) << (4 * j) | code_of(w1, s, r) << (4 * j + 16);
+    }
+    packed[i] = usable ? word : 0x88888888u;
+    if ((i & (lanes - 1)) == 0) scales[i >> lanes_log2] = scale;
+  }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kQuantThreads)
-    dequantize_kernel(const uint32_t* packed, const T* scales, int64_t words, int lanes,
+    dequantize_kernel(const uint32_t* packed, const T* scales, int64_t words, int lanes_log2,
                       uint4* weight) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kQuantThreads + threadIdx.x;
-  if (i >= words) return;
-  const uint32_t w = packed[i];
-  const float s = to_float(scales[i / lanes]);
-  uint32_t u[4];
+  const int64_t first = blockIdx.x * kQuantBlock + threadIdx.x;
+  uint32_t w[kQuantWords];
+  float s[kQuantWords];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float lo = s * static_cast<float>(static_cast<int>((w >> (4 * j)) & 15u) - 8);
-    const float hi = s * static_cast<float>(static_cast<int>((w >> (4 * j + 16)) & 15u) - 8);
-    if (std::is_same<T, __nv_bfloat16>::value)
-      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u[j]) : "f"(hi), "f"(lo));
-    else
-      asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(u[j]) : "f"(hi), "f"(lo));
+  for (int k = 0; k < kQuantWords; ++k) {
+    const int64_t i = first + k * kQuantThreads;
+    w[k] = i < words ? packed[i] : 0;
+    s[k] = i < words ? to_float(scales[i >> lanes_log2]) : 0.0f;
   }
-  weight[i] = make_uint4(u[0], u[1], u[2], u[3]);
+#pragma unroll
+  for (int k = 0; k < kQuantWords; ++k) {
+    const int64_t i = first + k * kQuantThreads;
+    if (i >= words) break;
+    uint32_t u[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      // 2^23 + code as float bits, less 2^23 + 8: q
+      const float lo =
+          __uint_as_float(0x4b000000u | ((w[k] >> (4 * j)) & 15u)) - 8388616.0f;
+      const float hi =
+          __uint_as_float(0x4b000000u | ((w[k] >> (4 * j + 16)) & 15u)) - 8388616.0f;
+      u[j] = pack_pair<T>(s[k] * lo, s[k] * hi);
+    }
+    __stcs(weight + i, make_uint4(u[0], u[1], u[2], u[3]));
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -1125,6 +1170,9 @@ __global__ void __launch_bounds__(kQuantThreads)
 
 constexpr int64_t kMaxInt4Rows = INT32_MAX - 64;
 
+
+// log2 of the words, and so lanes, of a group of 32, 64 or 128.
+int lanes_log2(int group) { return group == 32 ? 2 : (group == 64 ? 3 : 4); }
 
 bool int4_weight_ok(int64_t vocab, int64_t dim, int group) {
   int64_t n = 0;
@@ -1377,14 +1425,14 @@ extern "C" int cid_lm_head_quantize(cid_dtype_t dtype, const void* weight, int64
   if (misaligned({{weight, 16}, {packed, 16}, {scales, 2}})) return CID_ERR_MISALIGNED;
   if (any_null({weight, packed, scales})) return CID_ERR_INVALID_ARGUMENT;
   const int64_t words = vocab * (hidden_dim / 8);
-  const unsigned blocks = static_cast<unsigned>((words + kQuantThreads - 1) / kQuantThreads);
+  const unsigned blocks = static_cast<unsigned>((words + kQuantBlock - 1) / kQuantBlock);
   const auto* w = static_cast<const uint4*>(weight);
   if (dtype == CID_DTYPE_F16)
     quantize_kernel<__half><<<blocks, kQuantThreads, 0, as_stream(stream)>>>(
-        w, words, group_size / 8, packed, static_cast<__half*>(scales));
+        w, words, lanes_log2(group_size), packed, static_cast<__half*>(scales));
   else
     quantize_kernel<__nv_bfloat16><<<blocks, kQuantThreads, 0, as_stream(stream)>>>(
-        w, words, group_size / 8, packed, static_cast<__nv_bfloat16*>(scales));
+        w, words, lanes_log2(group_size), packed, static_cast<__nv_bfloat16*>(scales));
   return launch_result();
 }
 
@@ -1396,14 +1444,14 @@ extern "C" int cid_lm_head_dequantize(cid_dtype_t dtype, const uint32_t* packed,
   if (misaligned({{weight, 16}, {packed, 16}, {scales, 2}})) return CID_ERR_MISALIGNED;
   if (any_null({weight, packed, scales})) return CID_ERR_INVALID_ARGUMENT;
   const int64_t words = vocab * (hidden_dim / 8);
-  const unsigned blocks = static_cast<unsigned>((words + kQuantThreads - 1) / kQuantThreads);
+  const unsigned blocks = static_cast<unsigned>((words + kQuantBlock - 1) / kQuantBlock);
   auto* w = static_cast<uint4*>(weight);
   if (dtype == CID_DTYPE_F16)
     dequantize_kernel<__half><<<blocks, kQuantThreads, 0, as_stream(stream)>>>(
-        packed, static_cast<const __half*>(scales), words, group_size / 8, w);
+        packed, static_cast<const __half*>(scales), words, lanes_log2(group_size), w);
   else
     dequantize_kernel<__nv_bfloat16><<<blocks, kQuantThreads, 0, as_stream(stream)>>>(
-        packed, static_cast<const __nv_bfloat16*>(scales), words, group_size / 8, w);
+        packed, static_cast<const __nv_bfloat16*>(scales), words, lanes_log2(group_size), w);
   return launch_result();
 }
 

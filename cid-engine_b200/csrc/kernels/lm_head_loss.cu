@@ -672,7 +672,7 @@ struct PrepParams {
 };
 
 // One block packs kPrepRows rows: it counts the kept rows before its own
-// (reading their labels, 8 bytes each from L2), then a warp copies each row.
+// (reading their labels, 8 bytes each from L2), then copies them.
 // The last block leaves the count and zeroes the rows up to the next multiple
 // of 16, the K step of dW = d^T h.
 __global__ void __launch_bounds__(32 * kPrepRows) head_prepare_kernel(PrepParams p) {
@@ -719,11 +719,21 @@ __global__ void __launch_bounds__(32 * kPrepRows) head_prepare_kernel(PrepParams
     if (lane == 0) total = base + __popc(mask);
   }
   __syncthreads();
-  const int slot = slots[warp];
-  if (slot >= 0) {
-    const uint4* src = p.hidden + (r0 + warp) * p.vecs;
-    uint4* dst = p.packed + slot * p.vecs;
-    for (int64_t i = lane; i < p.vecs; i += 32) dst[i] = src[i];
+  // the block's kept rows, piece by piece: eight loads of a thread in flight
+  constexpr int kFlight = 8;
+  const uint32_t vecs = static_cast<uint32_t>(p.vecs), units = kPrepRows * vecs;
+  for (uint32_t i0 = threadIdx.x; i0 < units; i0 += kFlight * blockDim.x) {
+    uint4 v[kFlight];
+    int to[kFlight];
+#pragma unroll
+    for (int j = 0; j < kFlight; ++j) {
+      const uint32_t i = i0 + j * blockDim.x;
+      to[j] = i < units ? slots[i / vecs] : kIgnored;
+      if (to[j] >= 0) v[j] = p.hidden[r0 * p.vecs + i];
+    }
+#pragma unroll
+    for (int j = 0; j < kFlight; ++j)
+      if (to[j] >= 0) p.packed[to[j] * p.vecs + (i0 + j * blockDim.x) % vecs] = v[j];
   }
   if (r0 + kPrepRows >= p.rows) {
     const int n = total;
@@ -808,6 +818,7 @@ __global__ void __launch_bounds__(256)
     if (slot >= 0) {
       const int64_t tile = (slot / tile_m) * nt + c / kBN, size = tile_m * kBN;
       const float* q = partial + tile * size + (slot % tile_m) * kBN + c % kBN;
+#pragma unroll 4
       for (int s = 0; s < splits; ++s, q += mt * nt * size) {
         const float4 x = reinterpret_cast<const float4*>(q)[0];
         const float4 y = reinterpret_cast<const float4*>(q)[1];
@@ -893,7 +904,7 @@ Layout layout(int64_t rows, int64_t hidden, int64_t vocab, bool backward) {
 bool loss_extents_ok(int64_t rows, int64_t hidden, int64_t vocab) {
   int64_t n = 0, tiles = 0;
   if (!(rows >= 0 && rows <= kMaxLossRows && hidden > 0 && hidden % 8 == 0 &&
-        hidden <= INT32_MAX - kBN && vocab > 0 && vocab <= INT32_MAX - kBN &&
+        hidden <= INT32_MAX / 2 && vocab > 0 && vocab <= INT32_MAX - kBN &&
         count_ok(rows, hidden, &n) && n <= kMaxCount && count_ok(vocab, hidden, &n) &&
         n <= kMaxCount && count_ok((vocab + kBN - 1) / kBN, rows, &n) && n <= kMaxCount))
     return false;

@@ -230,8 +230,8 @@ TORCH_LIBRARY(cid_engine, m) {
   m.def(
       "lm_head_shard_records(Tensor token_ids, Tensor hidden, Tensor weight_shard, "
       "int vocab_offset, int total_vocab, bool round_bf16=True) -> Tensor");
-  // additive: the loss of the LM head and its gradient (autograd is
-  // registered in Python, cid_engine/head.py)
+  // additive: the loss of the LM head and its gradient (their Autograd kernels
+  // are in autograd.cpp)
   m.def(
       "lm_head_cross_entropy(Tensor labels, Tensor hidden, Tensor weight, "
       "int ignore_index=-100) -> (Tensor, Tensor)");
