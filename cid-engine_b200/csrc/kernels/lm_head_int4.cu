@@ -52,22 +52,22 @@ namespace cid {
 namespace {
 
 constexpr int kTileV = 128;       // weight rows of an accumulator: UMMA M, one a thread
-constexpr int kChunk = 128;       // columns a warpgroup unpacks at a time
-constexpr int kStageK = 256;      // columns of a stage: two chunks
+constexpr int kChunk = 128;       // columns of a stage, unpacked by a warpgroup at a time
 constexpr int kUmmaK = 16;
-constexpr uint32_t kStageW = kTileV * kStageK / 2;  // 16 KiB of codes for 128 weight rows
+constexpr uint32_t kStageW = kTileV * kChunk / 2;   // 8 KiB of codes for 128 weight rows
 constexpr int kChunkCols = kChunk / 2;              // TMEM columns of a chunk of A
-constexpr int kMaxStages = 8;
+constexpr int kMaxStages = 16;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kDRegion = kTmemCols - 4 * kChunkCols;  // columns left for accumulators
 constexpr int kMaxParts = 256;  // vocabulary parts of the statistics: record combine limit
-constexpr int kXchPitch = kTileV + 2;  // floats between hidden rows of a transposed tile
+constexpr int kXchRows = 32;           // hidden rows that a tile is transposed in at a time
+constexpr int kXchPitch = kTileV + 2;  // floats between them
 constexpr size_t kSmemLimit = 227 * 1024;
 
 struct Int4Params {
   int64_t rows, vocab;
   int64_t groups;      // scales a weight row
-  int stages_k;        // stages a tile: ceil(H / kStageK)
+  int chunks;          // stages a tile: ceil(H / kChunk)
   int64_t tiles;       // tiles of R * kTileV weight rows
   int64_t parts;       // vocabulary parts, one a CTA
   int64_t row_blocks;  // blocks of the kernel's N rows
@@ -195,14 +195,27 @@ __device__ __forceinline__ cid_shard_record_t record_of(const RowStats& a, float
 // the accumulators back, then two that unpack.
 __host__ __device__ constexpr int int4_threads(int r) { return 128 * (3 + r); }
 
+// With two row blocks (640 threads, 96 registers each at launch) the read-back
+// warps hold 64 accumulators apiece: registers move to them from the others.  The
+// shares add up to no more than the launch's, and on each SM sub-partition (a warp
+// of control, two of read-back, two of unpacking) to 32 x 472 of 16384.
+constexpr int kLaunchRegs = 96;
+constexpr int kCtrlRegs = 40;
+constexpr int kReadRegs = 144;
+constexpr int kUnpackRegs = 72;
+static_assert(128 * kCtrlRegs + 256 * kReadRegs + 256 * kUnpackRegs <=
+                  int4_threads(2) * kLaunchRegs,
+              "setmaxnreg.inc draws only on the registers the CTA was launched with");
+
 // N: hidden rows of a pass (accumulator columns); S: groups in a chunk of 128
 // columns, each with an accumulator of its own; R: blocks of 128 weight rows a
 // tile; kResident: the hidden rows stay in shared memory for the whole pass
 // (otherwise their slices travel with the codes).
 //
-// Chunks are numbered q along the CTA's work: for every stage its two halves of
-// 128 columns, and for each the tile's R row blocks.  Unpacking warpgroup q & 1
-// fills A buffer (q & 1, (q >> 1) & 1); the accumulators form a ring.
+// Chunks are numbered q along the CTA's work: for every stage the tile's R row
+// blocks.  Unpacking warpgroup q & 1 fills A buffer (q & 1, (q >> 1) & 1), so with
+// one row block the warpgroups take turns at the stages; the accumulators form a
+// ring.
 template <typename T, int N, int S, int R, bool kResident>
 __global__ void __launch_bounds__(int4_threads(R), 1)
     int4_head_kernel(const __grid_constant__ CUtensorMap map_w,
@@ -210,11 +223,13 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
   constexpr int kDCols = N * S;
   constexpr int kDBufs = int(kDRegion) / kDCols < 4 ? int(kDRegion) / kDCols : 4;
   static_assert(kDBufs == 4 || kDBufs == 2, "the accumulator ring is a power of two");
-  constexpr uint32_t kStage = R * kStageW + (kResident ? 0u : uint32_t(N) * kStageK * 2);
+  constexpr uint32_t kHidden = uint32_t(N) * kChunk * 2;  // hidden rows of a stage
+  constexpr uint32_t kStage = R * kStageW + (kResident ? 0u : kHidden);
   // D f32, A and B fp16 (0), both K-major, N >> 3 at bit 17, M >> 4 at bit 24
   constexpr uint32_t kDesc =
       (1u << 4) | (uint32_t(N >> 3) << 17) | (uint32_t(kTileV >> 4) << 24);
-  constexpr int kPer = kTileV / N;  // threads of a warpgroup that keep one hidden row's statistics
+  constexpr int kXN = N < kXchRows ? N : kXchRows;
+  constexpr int kPer = kTileV / kXN;  // threads of a warpgroup that keep one hidden row's statistics
 
   extern __shared__ unsigned char smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -223,9 +238,9 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
   unsigned char* stage0 = smem;
   unsigned char* resident = smem + stages * kStage;  // [2 * chunks][N][64] of the hidden rows
   float* xch = reinterpret_cast<float*>(
-      resident + (kResident ? size_t(p.stages_k) * (N * kStageK * 2) : 0));  // [R][N][kXchPitch]
-  float* sums = xch + R * N * kXchPitch;  // [groups][N] of -8 sum h, then [N] row scales
-  const int64_t group_slots = static_cast<int64_t>(p.stages_k) * 2 * S;
+      resident + (kResident ? size_t(p.chunks) * kHidden : 0));  // [R][kXN][kXchPitch]
+  float* sums = xch + R * kXN * kXchPitch;  // [groups][N] of -8 sum h, then [N] row scales
+  const int64_t group_slots = static_cast<int64_t>(p.chunks) * S;
   uint64_t* full = reinterpret_cast<uint64_t*>(sums + group_slots * N + N);
   uint64_t* empty = full + kMaxStages;
   uint64_t* a_full = empty + kMaxStages;  // [warpgroup][2]
@@ -244,7 +259,8 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], kResident ? 8 : 10);  // the unpacking warps', and the MMA warps' of hidden
+      // the warps that unpack the stage, and the MMA warps that use its hidden rows
+      mbar_init(&empty[s], kResident ? 4 * R : 5 * R);
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&a_full[i], 4);
@@ -275,7 +291,7 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
 
   const int64_t part = blockIdx.x;
   const int64_t t0 = part * p.tiles / p.parts, t1 = (part + 1) * p.tiles / p.parts;
-  const int chunks = 2 * p.stages_k;  // of 128 columns, each R row blocks
+  const int chunks = p.chunks;
 
   // A bounded wait of a whole warp; false when it ran out or another role did.
   // One lane polls: thirty-two take turns at the barrier and slow every role.
@@ -293,183 +309,181 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
     return got;
   };
 
-  if (warp == 0) {
-    if (lane == 0) {
-      // ---------------- TMA producer ----------------
-      // codes are in flight before the kernel that prepares the hidden rows ends
+  if (warp < 4) {
+    if (R == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCtrlRegs));
+    if (warp == 0) {
+      if (lane == 0) {
+        // ---------------- TMA producer ----------------
+        // codes are in flight before the kernel that prepares the hidden rows ends
+        int s = 0;
+        uint32_t ph = 0, issued = 0, issue_par = 0;
+        bool ok = true, prepared = false;
+        for (int64_t rb = 0; ok && rb < p.row_blocks; ++rb) {
+          for (int64_t t = t0; ok && t < t1; ++t) {
+            for (int k = 0; k < chunks; ++k) {
+              if (!thread_wait(&empty[s], ph ^ 1u)) {
+                ok = false;
+                break;
+              }
+              mbar_expect_tx(&full[s], kStage);
+              unsigned char* w = stage0 + s * kStage;
+              for (int r = 0; r < R; ++r)
+                tma_load_2d(w + r * kStageW, &map_w, k * (kChunk / 4),
+                            static_cast<int32_t>((t * R + r) * kTileV), &full[s]);
+              if (!kResident) {
+                if (!prepared) pdl_wait();
+                prepared = true;
+                for (int b = 0; b < kChunk / 64; ++b)
+                  tma_load_2d(w + R * kStageW + b * (N * 128), &map_h, k * kChunk + b * 64,
+                              static_cast<int32_t>(rb * N), &full[s]);
+              }
+              issued |= 1u << s;
+              issue_par = (issue_par & ~(1u << s)) | (ph << s);
+              if (++s == stages) {
+                s = 0;
+                ph ^= 1u;
+              }
+            }
+          }
+        }
+        // copies in flight land before the CTA exits (immediate unless aborted)
+        for (int i = 0; i < stages; ++i)
+          if (issued & (1u << i)) mbar_wait(&full[i], (issue_par >> i) & 1u, nullptr, kDrainNs);
+      }
+    } else if (warp == 3) {
+      if (kResident && lane == 0) {
+        // ---------------- resident hidden rows: one load a pass ----------------
+        pdl_wait();
+        int64_t loads = 0;
+        for (int64_t rb = 0; rb < p.row_blocks; ++rb, ++loads) {
+          if (rb > 0 && !thread_wait(h_empty, static_cast<uint32_t>(rb - 1) & 1u)) break;
+          mbar_expect_tx(h_full, static_cast<uint32_t>(chunks) * kHidden);
+          for (int b = 0; b < chunks * (kChunk / 64); ++b)
+            tma_load_2d(resident + b * (N * 128), &map_h, b * 64, static_cast<int32_t>(rb * N),
+                        h_full);
+        }
+        if (loads > 0)
+          mbar_wait(h_full, static_cast<uint32_t>(loads - 1) & 1u, nullptr, kDrainNs);
+      }
+    } else if (warp == 1 || warp == 2) {
+      // ---------------- MMA issuers: one for each unpacking warpgroup ----------------
+      // The whole warp runs the loop, so that addresses and descriptors stay
+      // warp-uniform; lane 0 issues.
+      const uint32_t mw = static_cast<uint32_t>(warp) - 1u;
       int s = 0;
-      uint32_t ph = 0, issued = 0, issue_par = 0;
-      bool ok = true, prepared = false;
+      uint32_t ph = 0;
+      bool ok = true;
+      uint32_t q = mw, turn = 0;  // chunk number (parities need its low bits only), whose stage it is
       for (int64_t rb = 0; ok && rb < p.row_blocks; ++rb) {
+        if (kResident && !warp_wait(h_full, static_cast<uint32_t>(rb) & 1u)) break;
         for (int64_t t = t0; ok && t < t1; ++t) {
-          for (int k = 0; k < p.stages_k; ++k) {
-            if (!thread_wait(&empty[s], ph ^ 1u)) {
-              ok = false;
-              break;
+          for (int k = 0; ok && k < chunks; ++k, turn ^= 1u) {
+            if (R == 2 || turn == mw) {
+              // the codes reach this role through TMEM; with resident hidden rows a
+              // stage is refilled without it and its barrier must not be waited for
+              const uint32_t ab = mw * 2 + ((q >> 1) & 1u), db = q % kDBufs;
+              if ((!kResident && !warp_wait(&full[s], ph)) ||
+                  !warp_wait(&a_full[ab], (q >> 2) & 1u) ||
+                  !warp_wait(&d_empty[db], (q / kDBufs & 1u) ^ 1u)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+              const uint32_t a = tmem_base + ab * kChunkCols, d = d_base + db * kDCols;
+              const uint64_t bd = sw128_desc(kResident ? smem_u32(resident + size_t(k) * kHidden)
+                                                       : smem_u32(stage0 + s * kStage + R * kStageW));
+              if (lane == 0) {
+  #pragma unroll
+                for (int kk = 0; kk < kChunk / kUmmaK; ++kk) {
+                  constexpr int per = kChunk / kUmmaK / S;  // MMAs of a group
+                  // the descriptor's address field counts 16 bytes
+                  umma_f16_ts(d + (kk / per) * N, a + kk * (kUmmaK / 2),
+                              bd + (kk / 4) * (N * 128 / 16) + (kk % 4) * 2, kDesc,
+                              kk % per != 0 ? 1u : 0u);
+                }
+                umma_commit(&a_empty[ab]);
+                umma_commit(&d_full[db]);
+                if (!kResident) umma_commit(&empty[s]);
+              }
+              __syncwarp();
+              q += 2;
             }
-            mbar_expect_tx(&full[s], kStage);
-            unsigned char* w = stage0 + s * kStage;
-            for (int r = 0; r < R; ++r)
-              tma_load_2d(w + r * kStageW, &map_w, k * (kStageK / 4),
-                          static_cast<int32_t>((t * R + r) * kTileV), &full[s]);
-            if (!kResident) {
-              if (!prepared) pdl_wait();
-              prepared = true;
-              for (int b = 0; b < kStageK / 64; ++b)
-                tma_load_2d(w + R * kStageW + b * (N * 128), &map_h, k * kStageK + b * 64,
-                            static_cast<int32_t>(rb * N), &full[s]);
-            }
-            issued |= 1u << s;
-            issue_par = (issue_par & ~(1u << s)) | (ph << s);
             if (++s == stages) {
               s = 0;
               ph ^= 1u;
             }
           }
         }
+        if (kResident && ok && lane == 0) umma_commit(h_empty);
       }
-      // copies in flight land before the CTA exits (immediate unless aborted)
-      for (int i = 0; i < stages; ++i)
-        if (issued & (1u << i)) mbar_wait(&full[i], (issue_par >> i) & 1u, nullptr, kDrainNs);
-    }
-  } else if (warp == 3) {
-    if (kResident && lane == 0) {
-      // ---------------- resident hidden rows: one load a pass ----------------
-      pdl_wait();
-      int64_t loads = 0;
-      for (int64_t rb = 0; rb < p.row_blocks; ++rb, ++loads) {
-        if (rb > 0 && !thread_wait(h_empty, static_cast<uint32_t>(rb - 1) & 1u)) break;
-        mbar_expect_tx(h_full, static_cast<uint32_t>(p.stages_k) * (N * kStageK * 2));
-        for (int b = 0; b < p.stages_k * (kStageK / 64); ++b)
-          tma_load_2d(resident + b * (N * 128), &map_h, b * 64, static_cast<int32_t>(rb * N),
-                      h_full);
+      // every arrival of this warp's MMAs lands before the CTA may exit and the
+      // TMEM is freed, also those that no one waits for any more
+      if (lane == 0) {
+        umma_commit(&mma_done[mw]);
+        mbar_wait(&mma_done[mw], 0, nullptr, kDrainNs);
       }
-      if (loads > 0)
-        mbar_wait(h_full, static_cast<uint32_t>(loads - 1) & 1u, nullptr, kDrainNs);
+      __syncwarp();
     }
-  } else if (warp == 1 || warp == 2) {
-    // ---------------- MMA issuers: one for each unpacking warpgroup ----------------
-    // The whole warp runs the loop, so that addresses and descriptors stay
-    // warp-uniform; lane 0 issues.
-    const uint32_t mw = static_cast<uint32_t>(warp) - 1u;
-    int s = 0;
-    uint32_t ph = 0;
-    bool ok = true;
-    uint32_t q = mw;  // chunk number; its barriers' parities need its low bits only
-    for (int64_t rb = 0; ok && rb < p.row_blocks; ++rb) {
-      if (kResident && !warp_wait(h_full, static_cast<uint32_t>(rb) & 1u)) break;
-      for (int64_t t = t0; ok && t < t1; ++t) {
-        for (int k = 0; ok && k < p.stages_k; ++k) {
-          // the codes reach this role through TMEM; with resident hidden rows a
-          // stage is refilled without it and its barrier must not be waited for
-          if (!kResident && !warp_wait(&full[s], ph)) {
-            ok = false;
-            break;
-          }
-          const uint32_t b0 = kResident ? smem_u32(resident + size_t(k) * (N * kStageK * 2))
-                                        : smem_u32(stage0 + s * kStage + R * kStageW);
-          for (int c = static_cast<int>(mw); c < 2 * R; c += 2, q += 2) {
-            const uint32_t ab = (q & 1u) * 2 + ((q >> 1) & 1u), db = q % kDBufs;
-            if (!warp_wait(&a_full[ab], (q >> 2) & 1u) ||
-                !warp_wait(&d_empty[db], (q / kDBufs & 1u) ^ 1u)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-            const uint32_t a = tmem_base + ab * kChunkCols, d = d_base + db * kDCols;
-            const uint64_t bd = sw128_desc(b0 + (c / R) * (2 * N * 128));
-            if (lane == 0) {
-#pragma unroll
-              for (int kk = 0; kk < kChunk / kUmmaK; ++kk) {
-                constexpr int per = kChunk / kUmmaK / S;  // MMAs of a group
-                // the descriptor's address field counts 16 bytes
-                umma_f16_ts(d + (kk / per) * N, a + kk * (kUmmaK / 2),
-                            bd + (kk / 4) * (N * 128 / 16) + (kk % 4) * 2, kDesc,
-                            kk % per != 0 ? 1u : 0u);
-              }
-              umma_commit(&a_empty[ab]);
-              umma_commit(&d_full[db]);
-            }
-            __syncwarp();
-          }
-          if (!ok) break;
-          if (!kResident && lane == 0) umma_commit(&empty[s]);
-          if (++s == stages) {
-            s = 0;
-            ph ^= 1u;
-          }
-        }
-      }
-      if (kResident && ok && lane == 0) umma_commit(h_empty);
-    }
-    // every arrival of this warp's MMAs lands before the CTA may exit and the
-    // TMEM is freed, also those that no one waits for any more
-    if (lane == 0) {
-      umma_commit(&mma_done[mw]);
-      mbar_wait(&mma_done[mw], 0, nullptr, kDrainNs);
-    }
-    __syncwarp();
   } else if (warp >= 4 + 4 * R) {
     // ---------------- unpacking: thread = weight row ----------------
+    if (R == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kUnpackRegs));
     const int wg = (warp - 4 - 4 * R) >> 2, quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     int s = 0;
     uint32_t ph = 0, n = 0;  // n: chunks of this warpgroup so far, q = 2 n + wg
-    bool ok = true;
-    const int64_t total = p.row_blocks * (t1 - t0) * p.stages_k;
-    for (int64_t i = 0; ok && i < total; ++i) {
-      if (!warp_wait(&full[s], ph)) break;
-      const unsigned char* row = stage0 + s * kStage + (R == 2 ? wg * kStageW : 0) + r * 128;
-#pragma unroll
-      for (int c = 0; c < R; ++c, ++n) {  // R == 1: half wg of the stage; R == 2: both halves
-        const int half = R == 1 ? wg : c;
-        uint4 w[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          w[j] = *reinterpret_cast<const uint4*>(row + (((half * 4 + j) ^ (r & 7)) << 4));
-        if (c == R - 1) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&empty[s]);
-        }
-        const uint32_t ab = static_cast<uint32_t>(wg) * 2 + (n & 1u);
-        if (!warp_wait(&a_empty[ab], (n >> 1 & 1u) ^ 1u)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t dst = tmem_base + lane_off + ab * kChunkCols;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          uint32_t a[32];
-          unpack8(w[2 * j].x, a);
-          unpack8(w[2 * j].y, a + 4);
-          unpack8(w[2 * j].z, a + 8);
-          unpack8(w[2 * j].w, a + 12);
-          unpack8(w[2 * j + 1].x, a + 16);
-          unpack8(w[2 * j + 1].y, a + 20);
-          unpack8(w[2 * j + 1].z, a + 24);
-          unpack8(w[2 * j + 1].w, a + 28);
-          tmem_store32(dst + 32 * j, a);
-        }
-        tmem_wait_store();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&a_full[ab]);
-      }
+    auto next_stage = [&]() {
       if (++s == stages) {
         s = 0;
         ph ^= 1u;
       }
+    };
+    const int64_t total = p.row_blocks * (t1 - t0) * chunks;
+    if (R == 1 && wg == 1) next_stage();
+    for (int64_t i = R == 1 ? wg : 0; i < total; i += R == 1 ? 2 : 1, ++n) {
+      if (!warp_wait(&full[s], ph)) break;
+      // 64 bytes of codes a weight row, in the 64-byte swizzle
+      const unsigned char* row = stage0 + s * kStage + (R == 2 ? wg * kStageW : 0) + r * 64;
+      uint4 w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        w[j] = *reinterpret_cast<const uint4*>(row + ((j ^ ((r >> 1) & 3)) << 4));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[s]);
+      const uint32_t ab = static_cast<uint32_t>(wg) * 2 + (n & 1u);
+      if (!warp_wait(&a_empty[ab], (n >> 1 & 1u) ^ 1u)) break;
+      tc_fence_after();
+      const uint32_t dst = tmem_base + lane_off + ab * kChunkCols;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint32_t a[32];
+        unpack8(w[2 * j].x, a);
+        unpack8(w[2 * j].y, a + 4);
+        unpack8(w[2 * j].z, a + 8);
+        unpack8(w[2 * j].w, a + 12);
+        unpack8(w[2 * j + 1].x, a + 16);
+        unpack8(w[2 * j + 1].y, a + 20);
+        unpack8(w[2 * j + 1].z, a + 24);
+        unpack8(w[2 * j + 1].w, a + 28);
+        tmem_store32(dst + 32 * j, a);
+      }
+      tmem_wait_store();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&a_full[ab]);
+      next_stage();
+      if (R == 1) next_stage();
     }
-  } else if (warp >= 4) {
+  } else {
     // ---------------- read-back: thread = weight row ----------------
+    if (R == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kReadRegs));
     const int wg = (warp - 4) >> 2, quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint16_t* scales = static_cast<const uint16_t*>(p.scales);
-    float* tile_xch = xch + wg * (N * kXchPitch);
-    const int own = r / kPer, sub = r % kPer;  // this thread's hidden row and share of columns
+    float* tile_xch = xch + wg * (kXN * kXchPitch);
+    constexpr int kParts = N / kXN;            // of the hidden rows, transposed one after another
+    const int own = r / kPer, sub = r % kPer;  // this thread's row of a part and share of columns
     uint32_t join_par = 0;
     auto join = [&](uint64_t* bar, uint32_t par) {
       __syncwarp();
@@ -503,10 +517,16 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
         sums[group_slots * N + threadIdx.x - 128] = p.row_scale[row0 + threadIdx.x - 128];
       if (!join(joined_all, all_par)) break;
       all_par ^= 1u;
-      RowStats st{-INFINITY, 0.0f, -1, -1};
-      float cur = 0.0f;
-      const bool live = p.out == nullptr && row0 + own < p.rows;
-      const int64_t id = live ? p.ids[row0 + own] : -1;
+      RowStats st[kParts];
+      float cur[kParts];
+      int64_t id[kParts];
+#pragma unroll
+      for (int h = 0; h < kParts; ++h) {
+        st[h] = RowStats{-INFINITY, 0.0f, -1, -1};
+        cur[h] = 0.0f;
+        const int64_t hr = row0 + h * kXN + own;
+        id[h] = p.out == nullptr && hr < p.rows ? p.ids[hr] : -1;
+      }
       for (int64_t t = t0; ok && t < t1; ++t) {
         const int64_t v0 = (t * R + wg) * kTileV, v = v0 + r;
         float acc[N];
@@ -570,50 +590,49 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
           continue;
         }
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-          float z = acc[j];
-          if (p.round_bf16) z = __bfloat162float(__float2bfloat16_rn(z));
-          tile_xch[j * kXchPitch + r] = v < p.vocab ? z : -INFINITY;
-        }
-        if (!join(&joined[wg], join_par)) {
-          ok = false;
-          break;
-        }
-        join_par ^= 1u;
-        if (live) {
-          // columns sub, sub + kPer, ... of the tile, in two passes: the
-          // maximum, then the exponentials
+        for (int h = 0; h < kParts; ++h) {
+#pragma unroll
+          for (int j = 0; j < kXN; ++j) {
+            float z = acc[h * kXN + j];
+            if (p.round_bf16) z = __bfloat162float(__float2bfloat16_rn(z));
+            tile_xch[j * kXchPitch + r] = v < p.vocab ? z : -INFINITY;
+          }
+          if (!join(&joined[wg], join_par)) {
+            ok = false;
+            break;
+          }
+          join_par ^= 1u;
+          // columns sub, sub + kPer, ... of the tile: the maximum, then the
+          // exponentials; where they stand is looked up only when it matters
           const float* x = tile_xch + own * kXchPitch + sub;
-          RowStats b{-INFINITY, 0.0f, -1, -1};
-          const int c0 = static_cast<int>(v0) + sub;
-#pragma unroll 4
-          for (int e = 0; e < N; ++e) {
-            const float z = x[e * kPer];
-            const int c = c0 + e * kPer;
-            if (c < p.vocab && (z > b.m || b.where < 0)) {
-              // a first -inf is a maximum too; a first NaN is not
-              if (z == z) {
-                b.m = z;
-                b.where = c;
-              }
-            }
-            if (z != z && b.nan < 0) b.nan = c;
-          }
+          constexpr int kShare = kTileV / kPer;
+          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 8
+          for (int e = 0; e < kShare; ++e) m4[e & 3] = fmaxf(m4[e & 3], x[e * kPer]);
+          RowStats b{fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), 0.0f, -1, -1};
           const float off = b.m == -INFINITY ? 0.0f : b.m;
-#pragma unroll 4
-          for (int e = 0; e < N; ++e) {
-            const float z = x[e * kPer];
-            b.s += ex2((z - off) * kLog2e);
+          float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+          for (int e = 0; e < kShare; ++e) s4[e & 3] += ex2((x[e * kPer] - off) * kLog2e);
+          b.s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+          const int c0 = static_cast<int>(v0) + sub;
+          if (b.m > st[h].m || st[h].where < 0) {
+            for (int e = kShare - 1; e >= 0; --e)
+              if (x[e * kPer] == b.m && c0 + e * kPer < p.vocab) b.where = c0 + e * kPer;
           }
-          merge_stats(st, b);
-          const int64_t rel = id - v0;
-          if (rel >= 0 && rel < kTileV && rel % kPer == sub) cur = x[rel - sub];
+          if (b.s != b.s) {  // a NaN, or an infinite maximum
+            for (int e = kShare - 1; e >= 0; --e)
+              if (x[e * kPer] != x[e * kPer]) b.nan = c0 + e * kPer;
+          }
+          merge_stats(st[h], b);
+          const int64_t rel = id[h] - v0;
+          if (rel >= 0 && rel < kTileV && rel % kPer == sub) cur[h] = x[rel - sub];
+          if (!join(&joined[wg], join_par)) {  // the part may be overwritten
+            ok = false;
+            break;
+          }
+          join_par ^= 1u;
         }
-        if (!join(&joined[wg], join_par)) {  // the tile may be overwritten
-          ok = false;
-          break;
-        }
-        join_par ^= 1u;
       }
       if (!ok) break;
       if (p.out != nullptr) {
@@ -624,38 +643,53 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
       }
       // ---- the part's record of each row: over the row's threads, then the warpgroups ----
 #pragma unroll
-      for (int d = 1; d < kPer; d <<= 1) {
-        RowStats o;
-        o.m = __shfl_xor_sync(0xffffffffu, st.m, d);
-        o.s = __shfl_xor_sync(0xffffffffu, st.s, d);
-        o.where = __shfl_xor_sync(0xffffffffu, st.where, d);
-        o.nan = __shfl_xor_sync(0xffffffffu, st.nan, d);
-        merge_stats(st, o);
-        cur += __shfl_xor_sync(0xffffffffu, cur, d);  // one thread at most has seen the token
+      for (int h = 0; h < kParts; ++h) {
+#pragma unroll
+        for (int d = 1; d < kPer; d <<= 1) {
+          RowStats o;
+          o.m = __shfl_xor_sync(0xffffffffu, st[h].m, d);
+          o.s = __shfl_xor_sync(0xffffffffu, st[h].s, d);
+          o.where = __shfl_xor_sync(0xffffffffu, st[h].where, d);
+          o.nan = __shfl_xor_sync(0xffffffffu, st[h].nan, d);
+          merge_stats(st[h], o);
+          cur[h] += __shfl_xor_sync(0xffffffffu, cur[h], d);  // one thread at most has seen it
+        }
       }
       if (R == 2) {
-        float* slot = xch + N * kXchPitch + own * 8;  // the second warpgroup's tile is free
-        if (wg == 1 && sub == 0) {
-          slot[0] = st.m;
-          slot[1] = st.s;
-          slot[2] = __int_as_float(st.where);
-          slot[3] = __int_as_float(st.nan);
-          slot[4] = cur;
+        float* slots = xch + kXN * kXchPitch;  // the second warpgroup's tile is free
+#pragma unroll
+        for (int h = 0; h < kParts; ++h) {
+          float* slot = slots + (h * kXN + own) * 8;
+          if (wg == 1 && sub == 0) {
+            slot[0] = st[h].m;
+            slot[1] = st[h].s;
+            slot[2] = __int_as_float(st[h].where);
+            slot[3] = __int_as_float(st[h].nan);
+            slot[4] = cur[h];
+          }
         }
         if (!join(joined_all, all_par)) break;
         all_par ^= 1u;
         if (wg == 0) {
-          const RowStats o{slot[0], slot[1], __float_as_int(slot[2]), __float_as_int(slot[3])};
-          merge_stats(st, o);
-          cur += slot[4];
+#pragma unroll
+          for (int h = 0; h < kParts; ++h) {
+            const float* slot = slots + (h * kXN + own) * 8;
+            merge_stats(st[h], RowStats{slot[0], slot[1], __float_as_int(slot[2]),
+                                        __float_as_int(slot[3])});
+            cur[h] += slot[4];
+          }
         }
       }
       // the next pass overwrites the slots and sums
       if (!join(joined_all, all_par)) break;
       all_par ^= 1u;
-      if (live && wg == 0 && sub == 0)
-        p.records[part * p.rows + row0 + own] =
-            record_of(st, cur, static_cast<int>(t0 * R * kTileV));
+#pragma unroll
+      for (int h = 0; h < kParts; ++h) {
+        const int64_t hr = row0 + h * kXN + own;
+        if (wg == 0 && sub == 0 && hr < p.rows)
+          p.records[part * p.rows + hr] =
+              record_of(st[h], cur[h], static_cast<int>(t0 * R * kTileV));
+      }
     }
   }
 
@@ -1178,7 +1212,7 @@ bool int4_weight_ok(int64_t vocab, int64_t dim, int group) {
   int64_t n = 0;
   return (group == 32 || group == 64 || group == 128) && vocab > 0 &&
          vocab <= INT32_MAX - 2 * kTileV && dim > 0 && dim % group == 0 &&
-         dim <= INT32_MAX - kStageK && count_ok(vocab, dim, &n) && n <= kMaxCount &&
+         dim <= INT32_MAX / 2 && count_ok(vocab, dim, &n) && n <= kMaxCount &&
          n / (8 * kQuantThreads) < INT32_MAX;
 }
 
@@ -1199,17 +1233,18 @@ size_t rows_smem(int row_warps, int64_t blocks, int group) {
          size_t{2} * (kRowsWarps / row_warps) * n * (32 * row_warps) * 4;
 }
 
-size_t int4_smem(int n, int r, bool resident, int stages, int64_t stages_k, int64_t slots) {
-  const size_t hidden = static_cast<size_t>(n) * kStageK * 2;
+size_t int4_smem(int n, int r, bool resident, int stages, int64_t chunks, int64_t slots) {
+  const size_t hidden = static_cast<size_t>(n) * kChunk * 2;
   return stages * (r * size_t{kStageW} + (resident ? 0 : hidden)) +
-         (resident ? stages_k * hidden : 0) +
-         (static_cast<size_t>(r) * kXchPitch + slots + 1) * n * 4 + 1024 + 512;
+         (resident ? chunks * hidden : 0) +
+         (static_cast<size_t>(r) * (n < kXchRows ? n : kXchRows) * kXchPitch + (slots + 1) * n) * 4 +
+         1024 + 512;
 }
 
 // Hidden rows of a pass: the accumulators of a chunk's groups are at most 64
 // columns wide, so a group of 128 takes up to 64 rows a pass, one of 64 up to
 // 32, one of 32 sixteen; more rows read the weight again.  The hidden rows stay
-// in shared memory where they leave room for four stages of codes; where they
+// in shared memory where they leave room for eight stages of codes; where they
 // do not, their slices are read again for every tile, and tiles of 256 weight
 // rows halve that traffic.
 //
@@ -1245,14 +1280,14 @@ Int4Plan int4_plan(int64_t rows, int64_t vocab, int64_t dim, int group) {
     return pl;
   }
   const int most = group / 2;
-  const int64_t stages_k = (dim + kStageK - 1) / kStageK, slots = stages_k * kStageK / group;
+  const int64_t slots = blocks * kChunk / group;
   pl.n = rows > 32 && most >= 64 ? 64 : (rows > 16 && most >= 32 ? 32 : 16);
   for (;; pl.n /= 2) {  // the widest hidden rows leave room for 16 of them only
-    pl.resident = int4_smem(pl.n, 1, true, 4, stages_k, slots) <= kSmemLimit;
+    pl.resident = int4_smem(pl.n, 1, true, 8, blocks, slots) <= kSmemLimit;
     pl.r = pl.resident ? 1 : 2;
     pl.stages = kMaxStages;
     while (pl.stages > 1 &&
-           int4_smem(pl.n, pl.r, pl.resident, pl.stages, stages_k, slots) > kSmemLimit)
+           int4_smem(pl.n, pl.r, pl.resident, pl.stages, blocks, slots) > kSmemLimit)
       --pl.stages;
     if (pl.stages > 1 || pl.n == 16) break;
   }
@@ -1289,11 +1324,19 @@ template <typename T, int N, int S, int R, bool kResident>
 int launch_int4(const CUtensorMap& map_w, const CUtensorMap& map_h, const Int4Params& p,
                 cudaStream_t stream) {
   const size_t smem =
-      int4_smem(N, R, kResident, p.stages, p.stages_k, static_cast<int64_t>(p.stages_k) * 2 * S);
+      int4_smem(N, R, kResident, p.stages, p.chunks, static_cast<int64_t>(p.chunks) * S);
   const cudaError_t e = cudaFuncSetAttribute(int4_head_kernel<T, N, S, R, kResident>,
                                              cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              static_cast<int>(smem));
   if (e != cudaSuccess) return record_cuda_error(e);
+  if (R == 2) {  // the split of registers is sized for this launch
+    static const bool sized = [] {
+      cudaFuncAttributes fa;
+      return cudaFuncGetAttributes(&fa, int4_head_kernel<T, N, S, R, kResident>) == cudaSuccess &&
+             fa.numRegs == kLaunchRegs;
+    }();
+    if (!sized) return CID_ERR_LAUNCH;
+  }
   // a programmatic dependent of the kernel that prepares the hidden rows: the
   // codes start streaming while that one runs
   return launch_pdl(int4_head_kernel<T, N, S, R, kResident>, dim3(static_cast<unsigned>(p.parts)),
@@ -1329,7 +1372,7 @@ int dispatch_int4(const void* hidden, int64_t dim, const void* packed, int group
                   const Int4Plan& pl, unsigned char* ws, const Int4Layout& l,
                   cudaStream_t stream) {
   p.groups = dim / group;
-  p.stages_k = static_cast<int>((dim + kStageK - 1) / kStageK);
+  p.chunks = static_cast<int>((dim + kChunk - 1) / kChunk);
   p.row_blocks = (p.rows + pl.n - 1) / pl.n;
   p.tiles = pl.tiles;
   p.parts = pl.parts;
@@ -1364,7 +1407,8 @@ int dispatch_int4(const void* hidden, int64_t dim, const void* packed, int group
   if (rc != CID_OK) return rc;
   CUtensorMap map_w, map_h;
   // codes copied as 16-bit elements, four columns each
-  rc = make_map_sw128(&map_w, CID_DTYPE_F16, packed, dim / 4, p.vocab, dim / 4, 64, kTileV);
+  rc = make_map_sw128(&map_w, CID_DTYPE_F16, packed, dim / 4, p.vocab, dim / 4, kChunk / 4, kTileV,
+                      CU_TENSOR_MAP_SWIZZLE_64B);
   if (rc == CID_OK)
     rc = make_map_sw128(&map_h, CID_DTYPE_F16, ws + l.hidden, dim, p.rows, dim, 64, pl.n);
   if (rc != CID_OK) return rc;

@@ -112,24 +112,25 @@ struct Grid {
   int64_t mt, nt, splits, units, kslices;
 };
 
-// K splits of dh: the number that makes the slowest SM's share of slices
-// smallest.  A unit costs its slices and about kUnitCost slices of epilogue.
-// The count is fixed by a whole piece's slices, so that every piece adds to the
-// same partial tiles.
-__device__ inline int dh_splits(int64_t tiles, int kslices, int workers) {
+// K splits of dh: the number that makes the slowest worker's share of slices
+// smallest, the lowest of equals.  A unit costs its slices and about kUnitCost
+// slices of epilogue.  The count is fixed by a whole piece's slices, so that every
+// piece adds to the same partial tiles.  The lanes of a warp weigh 32 numbers each
+// round (one thread alone took 7 us over them).
+__device__ inline int dh_splits(int64_t tiles, int kslices, int workers, int lane) {
   constexpr int kUnitCost = 8;
-  int best = 1;
-  int64_t best_cost = INT64_MAX;
-  for (int s = 1; s <= kMaxSplits; ++s) {
-    if (s > 1 && (tiles * s > kSplitUnits || s * 8 > kslices)) break;
-    const int64_t waves = (tiles * s + workers - 1) / workers;
-    const int64_t cost = waves * ((kslices + s - 1) / s + kUnitCost);
-    if (cost < best_cost) {
-      best_cost = cost;
-      best = s;
-    }
+  unsigned best = 0xffffffffu;  // cost << 7 | splits; lane 0 always weighs one
+  if (tiles > kSplitUnits / 2) return 1;
+  const int t = static_cast<int>(tiles);
+  for (int s = lane + 1; s <= kMaxSplits; s += 32) {
+    if (s > 1 && (t * s > kSplitUnits || s * 8 > kslices)) continue;
+    const int waves = (t * s + workers - 1) / workers;
+    const int64_t cost = static_cast<int64_t>(waves) * ((kslices + s - 1) / s + kUnitCost);
+    const unsigned key =
+        (static_cast<unsigned>(cost < (1 << 24) ? cost : (1 << 24) - 1) << 7) | static_cast<unsigned>(s);
+    best = key < best ? key : best;
   }
-  return best;
+  return static_cast<int>(__reduce_min_sync(0xffffffffu, best) & 127u);
 }
 
 __device__ __forceinline__ Grid make_grid(Mode mode, const Params& p, int n, int tile_m) {
@@ -362,6 +363,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (kPair) cluster_sync();  // the peer's barriers are initialised
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  // every kernel of a call is a programmatic dependent of the one before: set-up
+  // overlaps its tail, global memory waits for its end
+  pdl_trigger();
+  pdl_wait();
   const int n = *p.count;
   const Grid g = make_grid(kMode, p, n, kTM);
   const int64_t ksteps = (n > 0 ? n + kUmmaK - 1 : kUmmaK) / kUmmaK;  // of kDweight
@@ -679,6 +684,8 @@ __global__ void __launch_bounds__(32 * kPrepRows) head_prepare_kernel(PrepParams
   __shared__ int warp_sum[kPrepRows];
   __shared__ int slots[kPrepRows];
   __shared__ int total;
+  pdl_trigger();
+  pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t r0 = static_cast<int64_t>(blockIdx.x) * kPrepRows;
   int before = 0;
@@ -740,11 +747,14 @@ __global__ void __launch_bounds__(32 * kPrepRows) head_prepare_kernel(PrepParams
     const int64_t pad = n > 0 ? (static_cast<int64_t>(n) + 15) / 16 * 16 : 16;
     for (int64_t i = n * p.vecs + threadIdx.x; i < pad * p.vecs; i += blockDim.x)
       p.packed[i] = make_uint4(0, 0, 0, 0);
-    if (threadIdx.x == 0) {
+    if (warp == 0) {
       const int64_t mt = ((n > 0 ? n : 1) + p.tile_m - 1) / p.tile_m;
       const int64_t nt = (p.vecs * 8 + kBN - 1) / kBN;
-      p.count[0] = n;
-      p.count[2] = dh_splits(mt * nt, p.piece_slices, p.workers);
+      const int splits = dh_splits(mt * nt, p.piece_slices, p.workers, lane);
+      if (lane == 0) {
+        p.count[0] = n;
+        p.count[2] = splits;
+      }
     }
   }
 }
@@ -758,6 +768,8 @@ __global__ void __launch_bounds__(32 * kLossParts)
                      const float* label_logit, const int* slot_of, int64_t rows, float* loss,
                      float* lse) {
   __shared__ float sm[kLossParts][32], ss[kLossParts][32];
+  pdl_trigger();
+  pdl_wait();
   const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
   const int64_t r = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   const int slot = r < rows ? slot_of[r] : kIgnored;
@@ -805,6 +817,8 @@ template <typename T>
 __global__ void __launch_bounds__(256)
     head_dhidden_kernel(const float* partial, const int* slot_of, const int* count,
                         int64_t hidden, int tile_m, const uint32_t* top, T* out) {
+  pdl_trigger();
+  pdl_wait();
   const int64_t r = blockIdx.x;
   const int slot = slot_of[r];
   const int64_t n = *count;
@@ -926,13 +940,15 @@ int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = kSmemBytes<kPair>;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = kPair ? 2 : 1;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = kPair ? 2 : 1;
   return record_cuda_error(
       cudaLaunchKernelEx(&cfg, head_gemm_kernel<T, kMode, kPair>, a, b, out, p));
 }
@@ -995,8 +1011,8 @@ int launch_prepare(const Call& c, const Layout& l, const float* lse, const float
     if (e != cudaSuccess) return record_cuda_error(e);
   }
   const int64_t blocks = (c.rows + kPrepRows - 1) / kPrepRows;
-  head_prepare_kernel<<<static_cast<unsigned>(blocks), 32 * kPrepRows, 0, c.stream>>>(q);
-  return launch_result();
+  return launch_pdl(head_prepare_kernel, dim3(static_cast<unsigned>(blocks)),
+                    dim3(32 * kPrepRows), 0, c.stream, q);
 }
 
 template <typename T, bool kPair>
@@ -1023,10 +1039,10 @@ int run_loss(const Call& c, float* loss, float* lse) {
   rc = launch_gemm<T, kLoss, kPair>(map_a, map_b, map_a, p, padded / kTileM<kPair> * tiles,
                                     c.stream);
   if (rc != CID_OK) return rc;
-  head_loss_kernel<<<static_cast<unsigned>((c.rows + 31) / 32), 32 * kLossParts, 0, c.stream>>>(
-      p.records, tiles, padded, p.label_logit, reinterpret_cast<const int*>(c.ws + l.slot_of),
-      c.rows, loss, lse);
-  return launch_result();
+  return launch_pdl(head_loss_kernel, dim3(static_cast<unsigned>((c.rows + 31) / 32)),
+                    dim3(32 * kLossParts), 0, c.stream, static_cast<const float2*>(p.records),
+                    tiles, padded, static_cast<const float*>(p.label_logit),
+                    reinterpret_cast<const int*>(c.ws + l.slot_of), c.rows, loss, lse);
 }
 
 template <typename T, bool kPair>
@@ -1078,11 +1094,10 @@ int run_backward(const Call& c, const float* lse, const float* grad_loss, const 
     if (rc != CID_OK) return rc;
   }
   if (grad_hidden == nullptr) return CID_OK;
-  head_dhidden_kernel<T><<<static_cast<unsigned>(c.rows), 256, 0, c.stream>>>(
-      reinterpret_cast<const float*>(c.ws + l.partial),
-      reinterpret_cast<const int*>(c.ws + l.slot_of), p.count, c.dim, kTM, p.top,
-      static_cast<T*>(grad_hidden));
-  return launch_result();
+  return launch_pdl(head_dhidden_kernel<T>, dim3(static_cast<unsigned>(c.rows)), dim3(256), 0,
+                    c.stream, reinterpret_cast<const float*>(c.ws + l.partial),
+                    reinterpret_cast<const int*>(c.ws + l.slot_of), p.count, c.dim, kTM, p.top,
+                    static_cast<T*>(grad_hidden));
 }
 
 template <typename T>

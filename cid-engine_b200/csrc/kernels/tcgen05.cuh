@@ -170,10 +170,11 @@ inline PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
 
 // 2-D tensor map of 16-bit elements (bf16 or fp16) over a row-major matrix of
 // `outer` rows of `inner` elements, `pitch` elements apart; box [box_outer,
-// box_inner] with the 128-byte swizzle.  base and pitch * 2 are multiples of
-// 16 bytes.
+// box_inner] with the 128-byte swizzle (or another).  base and pitch * 2 are
+// multiples of 16 bytes.
 inline int make_map_sw128(CUtensorMap* map, cid_dtype_t dtype, const void* base, int64_t inner,
-                          int64_t outer, int64_t pitch, int box_inner, int box_outer) {
+                          int64_t outer, int64_t pitch, int box_inner, int box_outer,
+                          CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
   auto encode = tensor_map_encoder();
   if (encode == nullptr) return record_cuda_error(cudaErrorNotSupported);
   cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
@@ -184,7 +185,7 @@ inline int make_map_sw128(CUtensorMap* map, cid_dtype_t dtype, const void* base,
                 dtype == CID_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                        : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
                 2, const_cast<void*>(base), dims, strides, box, estr,
-                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
              ? CID_OK
