@@ -131,17 +131,6 @@ __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[32]) {
   tmem_wait32(r);
 }
 
-// True in one lane of a converged warp, always the same one.  A branch on it (and
-// not on a lane number) tells the compiler that one thread runs what follows, so
-// that the MMAs' operands stay in uniform registers: against `lane == 0` the whole
-// kernel went from 102 to 77 us at 16 rows x 128256 x 4096, from 143 to 117 us at 64.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t is;
-  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}"
-               : "=r"(is));
-  return is != 0;
-}
-
 // D[tmem] (+)= A[tmem] * B[shared], K = 16.
 __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b,
                                             uint32_t idesc, uint32_t accumulate) {

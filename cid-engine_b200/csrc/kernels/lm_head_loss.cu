@@ -429,48 +429,61 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (issued & (1u << i)) mbar_wait(&empty[i], (issue_par >> i) & 1u, nullptr, kDrainNs);
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       // ---------------- MMA issuer ----------------
+      // The whole warp runs the loop and an elected lane issues: operands stay in
+      // uniform registers, which keeps an MMA's issue short of its run time.
       int s = 0, buf = 0;
       uint32_t ph = 0, aph = 0;
       uint64_t* last_bar = nullptr;
       uint32_t last_par = 0;
       bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        bool got = true;
+        if (lane == 0) {
+          got = mbar_wait(bar, parity, abort, kWaitNs);
+          if (!got && !*abort) raise_abort(abort, p.status);
+        }
+        return __shfl_sync(0xffffffffu, static_cast<int>(got), 0) != 0;
+      };
       for (int64_t u = first; ok && u < g.units; u += stride) {
         const Unit x = unit_at(kMode, g, u, kTM);
-        if (!mbar_wait(&acc_empty[buf], aph ^ 1u, abort, kWaitNs)) {
-          if (!*abort) raise_abort(abort, p.status);
-          break;
-        }
+        if (!wait(&acc_empty[buf], aph ^ 1u)) break;
         tc_fence_after();
         const uint32_t d = tmem_base + static_cast<uint32_t>(buf * kBN);
         for (int64_t k = x.k0; k < x.k1; ++k) {
-          if (!mbar_wait(&full[s], ph, abort, kWaitNs)) {
-            if (!*abort) raise_abort(abort, p.status);
+          if (!wait(&full[s], ph)) {
             ok = false;
             break;
           }
           tc_fence_after();
           const uint32_t a0 = smem_u32(stage_a + s * kStageA);
           const uint32_t b0 = smem_u32(stage_b + s * kStageB<kPair>);
+          // K advance: 32 bytes inside a K-major row, two 8-row atoms otherwise
+          // (the address field counts 16 bytes)
+          const uint64_t ad = kAMn<kMode> ? mn_desc(a0) : sw128_desc(a0);
+          const uint64_t bd = kBMn<kMode> ? mn_desc(b0) : sw128_desc(b0);
           // rows past the last step of kDweight are not zero: they are not multiplied
           const int64_t left = kMode == kDweight ? ksteps - k * (kBK / kUmmaK) : kBK / kUmmaK;
+          const uint32_t more = k > x.k0 ? 1u : 0u;
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < kBK / kUmmaK; ++kk) {
-            if (kk >= left) break;
-            // K advance: 32 bytes inside a K-major row, two 8-row atoms otherwise
-            const uint64_t ad = kAMn<kMode> ? mn_desc(a0 + kk * 2048) : sw128_desc(a0 + kk * 32);
-            const uint64_t bd = kBMn<kMode> ? mn_desc(b0 + kk * 2048) : sw128_desc(b0 + kk * 32);
-            mma<kPair>(d, ad, bd, idesc<T, kMode, kPair>(), (k > x.k0 || kk > 0) ? 1u : 0u);
+            for (int kk = 0; kk < kBK / kUmmaK; ++kk) {
+              if (kk >= left) break;
+              mma<kPair>(d, ad + kk * (kAMn<kMode> ? 128 : 2), bd + kk * (kBMn<kMode> ? 128 : 2),
+                         idesc<T, kMode, kPair>(), kk > 0 ? 1u : more);
+            }
+            commit<kPair>(&empty[s]);
           }
-          commit<kPair>(&empty[s]);
+          __syncwarp();
           if (++s == kS) {
             s = 0;
             ph ^= 1u;
           }
         }
         if (!ok) break;
-        commit<kPair>(&acc_full[buf]);
+        if (elect_one()) commit<kPair>(&acc_full[buf]);
+        __syncwarp();
         last_bar = &acc_full[buf];
         last_par = aph;
         if (++buf == kAccBufs) {
@@ -479,7 +492,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       // MMAs in flight finish before the TMEM is freed (immediate unless aborted)
-      if (last_bar != nullptr) mbar_wait(last_bar, last_par, nullptr, kDrainNs);
+      if (lane == 0 && last_bar != nullptr) mbar_wait(last_bar, last_par, nullptr, kDrainNs);
+      __syncwarp();
     }
   } else {
     // ---------------- epilogue: thread = tile row, TMEM lane = tile row ----------------
