@@ -61,7 +61,7 @@ constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kDRegion = kTmemCols - 4 * kChunkCols;  // columns left for accumulators
 constexpr int kMaxParts = 256;  // vocabulary parts of the statistics: record combine limit
 constexpr int kXchRows = 32;           // hidden rows that a tile is transposed in at a time
-constexpr int kXchPitch = kTileV + 2;  // floats between them
+constexpr int kXchMost = kTileV + 8;   // floats between them, at most
 constexpr size_t kSmemLimit = 227 * 1024;
 
 struct Int4Params {
@@ -236,6 +236,7 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
       (1u << 4) | (uint32_t(N >> 3) << 17) | (uint32_t(kTileV >> 4) << 24);
   constexpr int kXN = N < kXchRows ? N : kXchRows;
   constexpr int kPer = kTileV / kXN;  // threads of a warpgroup that keep one hidden row's statistics
+  constexpr int kXchPitch = kTileV + kPer;  // a warp's reads fall on 32 banks
 
   extern __shared__ unsigned char smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -757,7 +758,10 @@ __device__ __forceinline__ uint4 scaled_columns(uint4 v, float up, float& sum) {
 // ---------------------------------------------------------------------------
 
 constexpr int kRowsThreads = 512;
-constexpr int kRowsWarps = kRowsThreads / 32;
+// Warps of a tile: four along its 128 weight rows, four along the columns.
+constexpr int kRowWarps = 4;
+constexpr int kColWarps = kRowsThreads / 32 / kRowWarps;
+constexpr int kRowsTile = 32 * kRowWarps;
 constexpr int kRowsN = 8;  // hidden rows: the MMA's columns
 // Blocks of codes a thread holds ahead.  Measured at 8 rows x 128256 x 4096 with 2 /
 // 3 / 4: groups of 128 70.4 / 66.7 / 64.3 us, of 64 94.8 / 98.9 / 103.0 us.
@@ -771,7 +775,6 @@ struct RowsParams {
   const uint4* hidden;  // [rows][words]
   int64_t rows, vocab;
   int words, groups, blocks;  // a weight row's words, groups and blocks of 128 columns
-  int row_warps;              // 1, 2 or 4 warps along the weight rows, the others along K
   int64_t tiles, parts;
   void* out;
   cid_shard_record_t* records;
@@ -825,14 +828,14 @@ __global__ void __launch_bounds__(kRowsThreads, 1) int4_rows_kernel(RowsParams p
   constexpr int kRun = 4 / S;    // consecutive words of a group a thread takes
   extern __shared__ unsigned char smem[];
   const int pitch = p.blocks * 256 + kRowsPad;
-  const int rw = p.row_warps, kws = kRowsWarps / rw, tile_rows = 32 * rw;
+  constexpr int rw = kRowWarps, kws = kColWarps, tile_rows = kRowsTile;
   unsigned char* hid = smem;                                     // [N][pitch]
   float* sums = reinterpret_cast<float*>(smem + N * pitch);      // [blocks * S][N] of -8 sum h
   float* rscale = sums + p.blocks * S * N;                       // [N]
   float* red = rscale + N;                                       // [2][kws][N][tile_rows]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int rwi = warp % rw, kw = warp / rw;
+  const int rwi = warp / kws, kw = warp % kws;  // neighbours share a weight row's lines
   const int64_t t0 = blockIdx.x * p.tiles / p.parts, t1 = (blockIdx.x + 1) * p.tiles / p.parts;
   const int per_tile = (p.blocks + kws - 1) / kws;  // blocks of a warp, the last perhaps empty
   const int64_t total = (t1 - t0) * per_tile;
@@ -924,9 +927,9 @@ __global__ void __launch_bounds__(kRowsThreads, 1) int4_rows_kernel(RowsParams p
   }
 
   // outputs of this thread: tile row tid % tile_rows, hidden rows tid / tile_rows, + step, ...
-  constexpr int kOwn = 128 * N / kRowsThreads;  // at most, with tiles of 128 rows
+  constexpr int kOwn = tile_rows * N / kRowsThreads;
   const int orow = threadIdx.x % tile_rows, on = threadIdx.x / tile_rows;
-  const int step = kRowsThreads / tile_rows;
+  constexpr int step = kRowsThreads / tile_rows;
   RowStats st[kOwn];
   float cur[kOwn];
 #pragma unroll
@@ -990,6 +993,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) int4_rows_kernel(RowsParams p
       const int n = on + j * step;
       if (n < N && n < p.rows) {
         float z = 0.0f;
+#pragma unroll
         for (int q = 0; q < kws; ++q) z += rb[(q * N + n) * tile_rows + orow];
         z *= rscale[n];
         if (!kStats) {
@@ -1229,22 +1233,21 @@ struct Int4Plan {
   int n, r;        // r: 0 for int4_rows_kernel
   bool resident;
   int stages;
-  int row_warps;   // of int4_rows_kernel
   int tile_rows;
   int64_t tiles, parts;
 };
 
-size_t rows_smem(int row_warps, int64_t blocks, int group) {
+size_t rows_smem(int64_t blocks, int group) {
   constexpr int n = kRowsN;
   return n * (blocks * 256 + kRowsPad) + (blocks * (kChunk / group) * n + n) * 4 +
-         size_t{2} * (kRowsWarps / row_warps) * n * (32 * row_warps) * 4;
+         size_t{2} * kColWarps * n * kRowsTile * 4;
 }
 
 size_t int4_smem(int n, int r, bool resident, int stages, int64_t chunks, int64_t slots) {
   const size_t hidden = static_cast<size_t>(n) * kChunk * 2;
   return stages * (r * size_t{kStageW} + (resident ? 0 : hidden)) +
          (resident ? chunks * hidden : 0) +
-         (static_cast<size_t>(r) * (n < kXchRows ? n : kXchRows) * kXchPitch + (slots + 1) * n) * 4 +
+         (static_cast<size_t>(r) * (n < kXchRows ? n : kXchRows) * kXchMost + (slots + 1) * n) * 4 +
          1024 + 512;
 }
 
@@ -1259,31 +1262,19 @@ size_t int4_smem(int n, int r, bool resident, int stages, int64_t chunks, int64_
 // they fit shared memory beside the sums.  Measured at 8 rows x 128256 x 4096, it
 // against the other: groups of 128 70 and 97 us, of 64 95 and 109 us, of 32 (an
 // accumulator and a load for every word) 166 and 130 us; 16 rows of groups of 128
-// 114 and 97 us.  Its tiles are 32, 64 or 128 weight rows with 16, 8 or 4 warps
-// along K: the height whose largest part is smallest, the higher of equals
-// (fewer sums to join).
+// 114 and 97 us.
 Int4Plan int4_plan(int64_t rows, int64_t vocab, int64_t dim, int group) {
   Int4Plan pl;
   const int64_t blocks = (dim + kChunk - 1) / kChunk;
   pl.n = kRowsN;
-  if (rows <= kRowsN && group >= 64 && rows_smem(1, blocks, group) <= kSmemLimit) {
-    const int64_t sms = sm_count() < kMaxParts ? sm_count() : kMaxParts;
-    int64_t best = INT64_MAX;
+  const int64_t sms = sm_count() < kMaxParts ? sm_count() : kMaxParts;
+  if (rows <= kRowsN && group >= 64 && rows_smem(blocks, group) <= kSmemLimit) {
     pl.r = 0;
     pl.resident = true;
     pl.stages = 0;
-    for (int rw = 4; rw >= 1; rw /= 2) {
-      if (kRowsWarps / rw > blocks && rw < 4) break;
-      const int64_t tiles = (vocab + 32 * rw - 1) / (32 * rw);
-      const int64_t part = (tiles + sms - 1) / sms * rw;
-      if (part < best) {
-        best = part;
-        pl.row_warps = rw;
-        pl.tile_rows = 32 * rw;
-        pl.tiles = tiles;
-        pl.parts = tiles < sms ? tiles : sms;
-      }
-    }
+    pl.tile_rows = kRowsTile;
+    pl.tiles = (vocab + kRowsTile - 1) / kRowsTile;
+    pl.parts = pl.tiles < sms ? pl.tiles : sms;
     return pl;
   }
   const int most = group / 2;
@@ -1298,11 +1289,9 @@ Int4Plan int4_plan(int64_t rows, int64_t vocab, int64_t dim, int group) {
       --pl.stages;
     if (pl.stages > 1 || pl.n == 16) break;
   }
-  pl.row_warps = 0;
   pl.tile_rows = pl.r * kTileV;
   pl.tiles = (vocab + pl.tile_rows - 1) / pl.tile_rows;
-  pl.parts = sm_count() < kMaxParts ? sm_count() : kMaxParts;
-  if (pl.tiles < pl.parts) pl.parts = pl.tiles;
+  pl.parts = pl.tiles < sms ? pl.tiles : sms;
   return pl;
 }
 
@@ -1315,7 +1304,7 @@ struct Int4Layout {
 Int4Layout int4_layout(int64_t rows, int64_t dim, int64_t vocab, int group, bool stats) {
   auto up = [](size_t x) { return (x + 1023) / 1024 * 1024; };
   const size_t padded = static_cast<size_t>((rows + 63) / 64 * 64);
-  const int64_t tiles = (vocab + 31) / 32;  // of the lowest tiles
+  const int64_t tiles = (vocab + kTileV - 1) / kTileV;
   Int4Layout l;
   l.hidden = 0;
   l.sums = up(static_cast<size_t>(rows) * dim * 2);
@@ -1396,14 +1385,13 @@ int dispatch_int4(const void* hidden, int64_t dim, const void* packed, int group
     q.words = static_cast<int>(dim / 8);
     q.groups = static_cast<int>(p.groups);
     q.blocks = static_cast<int>((dim + kChunk - 1) / kChunk);
-    q.row_warps = pl.row_warps;
     q.tiles = pl.tiles;
     q.parts = pl.parts;
     q.out = p.out;
     q.records = p.records;
     q.ids = p.ids;
     q.round_bf16 = p.round_bf16;
-    const size_t smem = rows_smem(pl.row_warps, q.blocks, group);
+    const size_t smem = rows_smem(q.blocks, group);
     return group == 128 ? launch_rows<T, 1>(q, smem, stream) : launch_rows<T, 2>(q, smem, stream);
   }
   int4_prepare_kernel<T><<<static_cast<unsigned>(p.row_blocks * pl.n), kPrepThreads, 0, stream>>>(

@@ -223,7 +223,7 @@ def test_int4_c_abi_checks(lib: ctypes.CDLL) -> None:
             i64(rows), i64(dim), i64(vocab), ctypes.c_int(group), ctypes.c_int(statistics))
 
     assert 0 < need(2, 128, 300, 64, 0)
-    assert need(2, 128, 300, 64, 1) == need(2, 128, 300, 64, 0) + 10 * 2 * 16
+    assert need(2, 128, 300, 64, 1) == need(2, 128, 300, 64, 0) + 3 * 2 * 16
     for bad in ((0, 128, 300, 64), (-1, 128, 300, 64), (2, 0, 300, 64), (2, 128, 0, 64),
                 (2, 128, 2**31, 64), (2, 128, 300, 48), (2, 32768 + 128, 300, 64)):
         assert need(*bad, 1) == 0
