@@ -82,8 +82,21 @@ struct HeadLossBackward : torch::autograd::Function<HeadLossBackward> {
   }
 };
 
+// Whether a graph is being recorded over any of the tensors; without one the
+// nodes below would cost a call their set-up for nothing.
+bool recording(std::initializer_list<const at::Tensor*> tensors) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const auto* t : tensors)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
 Pair forward_autograd(const at::Tensor& labels, const at::Tensor& hidden,
                       const at::Tensor& weight, std::int64_t ignore) {
+  if (!recording({&hidden, &weight})) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return call_forward(labels, hidden, weight, ignore);
+  }
   auto out = HeadLoss::apply(labels, hidden, weight, ignore);
   return {out[0], out[1]};
 }
@@ -92,6 +105,11 @@ Pair backward_autograd(const std::optional<at::Tensor>& gl, const std::optional<
                        const at::Tensor& labels, const at::Tensor& hidden,
                        const at::Tensor& weight, const at::Tensor& lse, std::int64_t ignore,
                        bool need_hidden, bool need_weight) {
+  const at::Tensor none;
+  if (!recording({gl ? &*gl : &none, ge ? &*ge : &none, &hidden, &weight, &lse})) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return call_backward(gl, ge, labels, hidden, weight, lse, ignore, need_hidden, need_weight);
+  }
   auto out = HeadLossBackward::apply(gl, ge, labels, hidden, weight, lse, ignore, need_hidden,
                                      need_weight);
   return {out[0], out[1]};
