@@ -145,10 +145,12 @@ def test_kept_rows(rows, keep) -> None:
         assert not bool(dw.any())
 
 
-@pytest.mark.parametrize("rows,vocab,hidden", [(9000, 5003, 64), (40, 70001, 128), (3000, 12000, 256)])
+@pytest.mark.parametrize("rows,vocab,hidden", [
+    (9000, 20011, 64), (33000, 9001, 16), (40, 70001, 128), (3000, 12000, 256)])
 def test_pieces_of_the_vocabulary(rows, vocab, hidden) -> None:
-    """Sizes at which the backward takes several pieces (9000 rows: 4096-column
-    pieces, the last one short) or splits the sum over the vocabulary."""
+    """Sizes at which the backward takes several pieces (9000 rows: 14336 columns
+    and a short piece; 33000: the least, 4096) or splits the sum over the
+    vocabulary."""
     _check(*_inputs(rows, vocab, hidden, BF16))
 
 
