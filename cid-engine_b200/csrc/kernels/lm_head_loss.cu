@@ -19,7 +19,8 @@
 //
 // Roundings to 16 bits: d, because the tensor cores take 16-bit operands (the
 // same step as a 16-bit gradient of the logits; at most half a step of each
-// element, and the elements' errors are independent), and the outputs.  fp16 d
+// element, and the elements' errors are independent; dh gets what the label's
+// element lost back in f32), and the outputs.  fp16 d
 // is scaled by a power of two from the largest coefficient, so that neither a
 // loss scale nor a division by the number of rows leaves fp16's range.
 #include <cuda_bf16.h>
@@ -92,6 +93,7 @@ struct Params {
   float2* records;      // [tiles][rec_stride]
   float* label_logit;   // [rec_stride]
   int64_t rec_stride;
+  float* rest;          // kDlogits: what rounding took from d at the label, packed rows
   int accumulate;       // kDhidden: add to the partial sums of the pieces before
   uint32_t* status;
 };
@@ -220,6 +222,19 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   else
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+
+template <typename T>
+__device__ __forceinline__ float round16(float x) {
+  if (std::is_same<T, __nv_bfloat16>::value) return __bfloat162float(__float2bfloat16_rn(x));
+  return __half2float(__float2half_rn(x));
+}
+
+__device__ __forceinline__ float2 pair_of(__nv_bfloat16, uint32_t u) {
+  return make_float2(bf16_bits_lo(u), bf16_bits_hi(u));
+}
+__device__ __forceinline__ float2 pair_of(__half, uint32_t u) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&u));
 }
 
 // ---- cluster and pair forms of the wrappers ----
@@ -583,6 +598,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (j == rel) q -= cb;
             v[j] = valid && c0 + j < width ? q : 0.0f;
           }
+          if (valid && rel >= 0 && rel < 32) {
+            float at = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j == rel) at = v[j];
+            p.rest[row] = at - round16<T>(at);
+          }
         } else if (kMode == kDweight) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] *= inv;
@@ -824,11 +846,14 @@ __global__ void __launch_bounds__(32 * kLossParts)
   }
 }
 
-// dh of every row: the splits' partial sums in ascending order, 16 bits; zero
-// for an ignored row, NaN for a label that is no token
+// dh of every row: the splits' partial sums in ascending order, and what rounding
+// took from d at the label times the label's weight row (d is largest there, and
+// its rounding is most of what the sum would be off by); 16 bits.  Zero for an
+// ignored row, NaN for a label that is no token.
 template <typename T>
 __global__ void __launch_bounds__(256)
-    head_dhidden_kernel(const float* partial, const int* slot_of, const int* count,
+    head_dhidden_kernel(const float* partial, const int* slot_of, const int* plabel,
+                        const float* rest, const uint4* weight, const int* count,
                         int64_t hidden, int tile_m, const uint32_t* top, T* out) {
   pdl_trigger();
   pdl_wait();
@@ -838,6 +863,8 @@ __global__ void __launch_bounds__(256)
   const int64_t mt = ((n > 0 ? n : 1) + tile_m - 1) / tile_m, nt = (hidden + kBN - 1) / kBN;
   const int splits = count[2];
   const float inv = 1.0f / coef_scale(top);
+  const float left = slot >= 0 ? rest[slot] : 0.0f;
+  const uint4* own = weight + (slot >= 0 ? plabel[slot] : 0) * (hidden / 8);
   for (int64_t c = threadIdx.x * 8; c < hidden; c += blockDim.x * 8) {
     float v[8];
 #pragma unroll
@@ -857,6 +884,16 @@ __global__ void __launch_bounds__(256)
         v[5] += y.y;
         v[6] += y.z;
         v[7] += y.w;
+      }
+      if (left != 0.0f) {
+        const uint4 w = own[c / 8];
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = pair_of(T{}, u[j]);
+          v[2 * j] = fmaf(left, f.x, v[2 * j]);
+          v[2 * j + 1] = fmaf(left, f.y, v[2 * j + 1]);
+        }
       }
     }
     uint4 o;
@@ -897,7 +934,7 @@ int64_t piece_cols(int64_t rows, int64_t vocab) {
 
 // Byte offsets of the workspace's parts.
 struct Layout {
-  size_t count, slot_of, plabel, plse, pa, pb, label_logit, packed, records, d, partial, bytes;
+  size_t count, slot_of, plabel, plse, pa, pb, label_logit, rest, packed, records, d, partial, bytes;
   int64_t partial_rows;
 };
 
@@ -921,6 +958,7 @@ Layout layout(int64_t rows, int64_t hidden, int64_t vocab, bool backward) {
     l.plse = take(padded * 4);
     l.pa = take(padded * 4);
     l.pb = take(padded * 4);
+    l.rest = take(padded * 4);
     l.d = take(padded * piece_cols(rows, vocab) * 2);
     const int64_t tiles = padded / tile_m * ((hidden + kBN - 1) / kBN);
     l.partial_rows = (tiles > kSplitUnits ? tiles : kSplitUnits) * tile_m;
@@ -1092,6 +1130,7 @@ int run_backward(const Call& c, const float* lse, const float* grad_loss, const 
   p.ca = reinterpret_cast<const float*>(c.ws + l.pa);
   p.cb = reinterpret_cast<const float*>(c.ws + l.pb);
   p.top = scaled ? reinterpret_cast<const uint32_t*>(c.ws + l.count) + 1 : nullptr;
+  p.rest = reinterpret_cast<float*>(c.ws + l.rest);
   p.status = c.status;
   constexpr int kTM = kTileM<kPair>;
   const int64_t mt = padded / kTM, ht = (c.dim + kBN - 1) / kBN;
@@ -1111,7 +1150,9 @@ int run_backward(const Call& c, const float* lse, const float* grad_loss, const 
   if (grad_hidden == nullptr) return CID_OK;
   return launch_pdl(head_dhidden_kernel<T>, dim3(static_cast<unsigned>(c.rows)), dim3(256), 0,
                     c.stream, reinterpret_cast<const float*>(c.ws + l.partial),
-                    reinterpret_cast<const int*>(c.ws + l.slot_of), p.count, c.dim, kTM, p.top,
+                    reinterpret_cast<const int*>(c.ws + l.slot_of), p.labels,
+                    static_cast<const float*>(p.rest), static_cast<const uint4*>(c.weight),
+                    p.count, c.dim, kTM, p.top,
                     static_cast<T*>(grad_hidden));
 }
 
