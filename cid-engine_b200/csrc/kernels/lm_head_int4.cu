@@ -86,6 +86,12 @@ __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162f
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 
 template <typename T>
+__device__ __forceinline__ float2 pair_floats(uint32_t u) {
+  if (std::is_same<T, __nv_bfloat16>::value) return make_float2(bf16_bits_lo(u), bf16_bits_hi(u));
+  return __half22float2(*reinterpret_cast<const __half2*>(&u));
+}
+
+template <typename T>
 __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
   uint32_t r;
   if (std::is_same<T, __nv_bfloat16>::value)
@@ -1114,24 +1120,40 @@ constexpr int kQuantThreads = 256;
 constexpr int kQuantWords = 4;  // words a thread, a block apart: loads in flight
 constexpr int64_t kQuantBlock = kQuantThreads * kQuantWords;
 
-// Code of w for scale s and r = 1 / s rounded: rint(w / s), ties to even, without a
-// division.  The sum with 1.5 2^23 rounds w r to an integer q; it can differ from
-// the rounded quotient only where w / s is a tie (no other quotient of two 11-bit
-// numbers is nearer to one than 2^-13), and there the remainder w - q s, exact in
-// f32, is half of s: then an odd q moves to the even neighbour on its side.
-__device__ __forceinline__ uint32_t code_of(float w, float s, float r) {
-  const float t = fmaf(w, r, 12582912.0f);
-  float q = t - 12582912.0f;
-  const float rest = fmaf(-q, s, w);
-  if (2.0f * fabsf(rest) == s && (__float_as_uint(t) & 1u)) q += copysignf(1.0f, rest);
-  // 1.5 2^23 + 8 + q in [0, 15]: the code is the low bits
-  return __float_as_uint(fminf(fmaxf(q, -8.0f), 7.0f) + 12582920.0f) & 15u;
+// rint(w / s) + 8, ties to even, as the low bits of a float; r is 1 / s to a few
+// units.  The first sum rounds w r to a multiple of 2^-14: a quotient that is a tie
+// becomes one exactly, and no other can, since a quotient of two 11-bit numbers is
+// a tie or 2^-12 away from it.  The second rounds to an integer, ties to even.
+__device__ __forceinline__ float code_float(float w, float r) {
+  return fmaf(w, r, 768.0f) + (12582920.0f - 768.0f);  // 1.5 2^9, then 1.5 2^23 + 8
+}
+
+// The word of eight columns.  kClamp: a quotient may leave [-8, 7].
+template <typename T, bool kClamp>
+__device__ __forceinline__ uint32_t code_word(uint4 v, float r, float grow) {
+  const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+  uint32_t word = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 w = pair_floats<T>(u[j]);
+    float lo = code_float(kClamp ? w.x * grow : w.x, r);
+    float hi = code_float(kClamp ? w.y * grow : w.y, r);
+    if (kClamp) {
+      lo = fminf(fmaxf(lo, 12582912.0f), 12582927.0f);
+      hi = fminf(fmaxf(hi, 12582912.0f), 12582927.0f);
+    }
+    word |= (__float_as_uint(lo) & 15u) << (4 * j);
+    word |= (__float_as_uint(hi) & 15u) << (4 * j + 16);
+  }
+  return word;
 }
 
 // A lane holds 8 columns (16 bytes) and writes their word; the group's lanes
 // (4, 8 or 16) share the maximum.  |w| compares as its bits, NaN above all, so
 // a NaN or infinite weight leaves its group's scale NaN or infinite.
-// Bound by memory: 2.5 bytes a weight.
+// Bound by memory, 2.5 bytes a weight, once the divisions are gone: with them, and
+// a word every thread, 128256 x 4096 took 720 us; with one reciprocal a group and
+// exact remainders for the ties 493 us, 90 % of the issue slots.
 template <typename T>
 __global__ void __launch_bounds__(kQuantThreads)
     quantize_kernel(const uint4* weight, int64_t words, int lanes_log2, uint32_t* packed,
@@ -1148,32 +1170,32 @@ __global__ void __launch_bounds__(kQuantThreads)
 #pragma unroll
   for (int k = 0; k < kQuantWords; ++k) {
     const int64_t i = first + k * kQuantThreads;
-    const uint32_t u[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-    uint32_t top = top_bits(v[k]);
+    uint32_t top = __vmaxu2(__vmaxu2(v[k].x & 0x7fff7fffu, v[k].y & 0x7fff7fffu),
+                            __vmaxu2(v[k].z & 0x7fff7fffu, v[k].w & 0x7fff7fffu));
+    top = max(top & 0xffffu, top >> 16);
     for (int d = 1; d < lanes; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
     if (i >= words) continue;
-    const uint16_t bits = static_cast<uint16_t>(top);
-    const float amax = to_float(*reinterpret_cast<const T*>(&bits));
+    const float amax = pair_floats<T>(top).x;
+    // times 1/7 rounds to 16 bits as the quotient does: 7 times an odd number of
+    // half steps has more bits than a maximum, so no quotient is a tie, and the
+    // nearest to one is 2^-16 away
     T scale;
     if (std::is_same<T, __nv_bfloat16>::value)
-      *reinterpret_cast<__nv_bfloat16*>(&scale) = __float2bfloat16_rn(__fdiv_rn(amax, 7.0f));
+      *reinterpret_cast<__nv_bfloat16*>(&scale) = __float2bfloat16_rn(amax * (1.0f / 7.0f));
     else
-      *reinterpret_cast<__half*>(&scale) = __float2half_rn(__fdiv_rn(amax, 7.0f));
-    float s = to_float(scale);
-    // below 2^-100 the reciprocal could overflow: scale and weights grow alike
-    const float grow = s < 7.9e-31f ? 1.2676506e30f : 1.0f;  // 2^100
-    s *= grow;
-    const bool usable = s > 0.0f && s < INFINITY;
-    const float r = usable ? __frcp_rn(s) : 0.0f;
-    uint32_t word = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint16_t b0 = static_cast<uint16_t>(u[j]), b1 = static_cast<uint16_t>(u[j] >> 16);
-      const float w0 = to_float(*reinterpret_cast<const T*>(&b0)) * grow;
-      const float w1 = to_float(*reinterpret_cast<const T*>(&b1)) * grow;
-      word |= code_of(w0, s, r) << (4 * j) | code_of(w1, s, r) << (4 * j + 16);
+      *reinterpret_cast<__half*>(&scale) = __float2half_rn(amax * (1.0f / 7.0f));
+    const float s = to_float(scale);
+    // a scale of the 16-bit type's last binades has few bits: quotients may pass 7,
+    // and the reciprocal f32's range (scale and weights then grow alike)
+    constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
+    uint32_t word = 0x88888888u;
+    if (s >= (bf ? 1e-30f : 1e-3f) && s < INFINITY) {
+      word = code_word<T, false>(v[k], __fdividef(1.0f, s), 1.0f);
+    } else if (s > 0.0f && s < INFINITY) {
+      const float grow = bf ? 1.2676506e30f : 1.0f;  // 2^100
+      word = code_word<T, true>(v[k], __frcp_rn(s * grow), grow);
     }
-    packed[i] = usable ? word : 0x88888888u;
+    packed[i] = word;
     if ((i & (lanes - 1)) == 0) scales[i >> lanes_log2] = scale;
   }
 }
