@@ -380,3 +380,48 @@ def test_train_quantize_decode() -> None:
             by_hand = cid_engine.refine_step_from_hidden(by_hand, hidden, head, **kw).token_ids
         torch.cuda.synchronize()
         assert torch.equal(loop.ids, by_hand)
+
+
+@pytest.mark.parametrize("rows", [3, 40])
+def test_fp16_hidden_rows_rounded_to_bf16(rows) -> None:
+    """round_bf16 rounds the float32 logits to bfloat16 whatever the hidden type."""
+    import cid_engine
+
+    ids, h, head, z, dz = _inputs(rows, 3000, 256, 64, FP16)
+    conf, pred, _ = cid_engine.lm_head_quantized_display_statistics(ids, h, *head)
+    zb = z.to(BF16).double()
+    p = torch.softmax(zb, 1).amax(1)
+    # a logit near a rounding border may fall on the other side: one step of it
+    step = zb.abs().amax(1) * 2.0**-7
+    assert bool(((conf.double() - p).abs() <= (2 * dz.amax(1) + 2 * step) * p).all())
+    held = zb.gather(1, pred[:, None])[:, 0]
+    assert bool((zb.amax(1) - held <= step).all())
+
+
+@pytest.mark.parametrize("rows,dtype", [(4, BF16), (30, BF16), (4, FP16), (30, FP16)])
+def test_hidden_rows_of_every_size(rows, dtype) -> None:
+    """Rows from the type's subnormals to its largest values, and rows whose
+    elements span its range: the power of two that a row is scaled by is undone."""
+    import cid_engine
+
+    _, h, head, _, _ = _inputs(rows, 600, 256, 128, dtype)
+    tiny, big = torch.finfo(dtype).smallest_normal, torch.finfo(dtype).max
+    scale = torch.logspace(-1, 1, rows, device="cuda", dtype=torch.float64)
+    h = h.double()
+    h[0] *= tiny / 8
+    h[1] *= big / 1e6
+    h[2, ::3] *= 1e-4
+    h[3] = 0
+    h = (h * scale[:, None]).to(dtype)
+    got = cid_engine.lm_head_quantized_logits(h, *head).double()
+    V = head.packed.shape[0]
+    values = (_unpack(head.packed).view(V, 2, 128) * head.scales.double()[..., None]).view(V, 256)
+    z = h.double() @ values.T
+    dz = (256 / 16 + 2 + 16) * 2.0**-22 * (h.double().abs() @ values.abs().T)
+    # elements below 2^-24 of their row's largest lose up to 2^-35 of it
+    dz += 2.0**-35 * h.double().abs().amax(1)[:, None] * values.abs().sum(1)[None]
+    u = torch.finfo(dtype).eps / 2
+    ok = z.abs() < big * 0.99
+    tol = dz * (1 + u) + u * z.abs() + torch.finfo(dtype).smallest_normal * u * 2 + 2.0**-149
+    assert bool(((got - z).abs() <= tol)[ok].all())
+    assert not bool(got[3].any())

@@ -379,3 +379,23 @@ def test_corruption_to_loss() -> None:
     _within("grad_hidden", got[2].view(-1, H), flat[2], flat[6])
     _within("grad_weight", got[3], flat[3], flat[7])
     assert torch.equal(got[0] != 0, labels >= 0)
+
+
+def test_gradient_through_log_sum_exp_alone() -> None:
+    """A penalty on the log-sum-exp: d = a p without the label's term."""
+    import cid_engine
+
+    y, h, w, _, ge = _inputs(90, 700, 128, BF16)
+    hr, wr = h.detach().requires_grad_(), w.detach().requires_grad_()
+    _, lse = cid_engine.lm_head_cross_entropy(y, hr, wr)
+    dh, dw = torch.autograd.grad(lse, (hr, wr), grad_outputs=ge)
+    exact = _exact(y, h, w, torch.zeros_like(ge), ge)
+    _within("grad_hidden", dh, exact[2], exact[6])
+    _within("grad_weight", dw, exact[3], exact[7])
+
+
+def test_many_rows_few_labels() -> None:
+    """Tiles and splits follow the kept rows, not the rows."""
+    y, h, w, gl, ge = _inputs(2000, 4000, 192, BF16, "all")
+    y[torch.arange(2000, device=y.device) % 167 != 3] = -100
+    _check(y, h, w, gl, ge)
