@@ -19,8 +19,8 @@
 //
 // Roundings to 16 bits: d, because the tensor cores take 16-bit operands (the
 // same step as a 16-bit gradient of the logits; at most half a step of each
-// element, and the elements' errors are independent; dh gets what the label's
-// element lost back in f32), and the outputs.  fp16 d
+// element, and the elements' errors are independent; dh and dW get what the
+// label's element lost back in f32), and the outputs.  fp16 d
 // is scaled by a power of two from the largest coefficient, so that neither a
 // loss scale nor a division by the number of rows leaves fp16's range.
 #include <cuda_bf16.h>
@@ -48,6 +48,9 @@ constexpr uint32_t kStageA = kCtaM * kBK * 2;
 // each epilogue warp.
 constexpr uint32_t kBoxBytes = 32 * 128;
 constexpr uint32_t kBoxRegion = 4 * 2 * kBoxBytes;
+// Labels among a warp's 32 tokens whose part of dW gets its rounding back.
+constexpr int kHits = 64;
+constexpr int kNear = 4;  // of them held in registers
 constexpr int kThreads = 192;  // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
 constexpr int kRowGroup = 4096;  // rows whose row blocks share weight tiles in L2
 constexpr int kPrepRows = 8;   // rows a prepare block packs, one a warp
@@ -69,7 +72,8 @@ constexpr uint32_t kStageBytes = kStageA + kStageB<kPair>;
 template <bool kPair>
 constexpr int kStages = kPair ? 6 : 4;
 template <bool kPair>
-constexpr size_t kSmemBytes = kStages<kPair> * size_t{kStageBytes<kPair>} + kBoxRegion + 1024 + 512;
+constexpr size_t kSmemBytes =
+    kStages<kPair> * size_t{kStageBytes<kPair>} + kBoxRegion + 4 * kHits * sizeof(int) + 1024 + 512;
 static_assert(kSmemBytes<true> <= 227 * 1024 && kSmemBytes<false> <= 227 * 1024,
               "shared memory of one CTA");
 
@@ -93,7 +97,8 @@ struct Params {
   float2* records;      // [tiles][rec_stride]
   float* label_logit;   // [rec_stride]
   int64_t rec_stride;
-  float* rest;          // kDlogits: what rounding took from d at the label, packed rows
+  float* rest;          // what rounding took from d at the label, packed rows
+  const void* packed;   // kDweight: the packed hidden rows
   int accumulate;       // kDhidden: add to the partial sums of the pieces before
   uint32_t* status;
 };
@@ -336,7 +341,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   unsigned char* stage_a = smem;
   unsigned char* stage_b = smem + kS * kStageA;
   unsigned char* boxes = smem + kS * kStageBytes<kPair>;
-  uint64_t* full = reinterpret_cast<uint64_t*>(boxes + kBoxRegion);
+  int* hits = reinterpret_cast<int*>(boxes + kBoxRegion);  // [4][kHits]
+  uint64_t* full = reinterpret_cast<uint64_t*>(hits + 4 * kHits);
   uint64_t* empty = full + kS;
   uint64_t* acc_full = empty + kS;
   uint64_t* acc_empty = acc_full + kAccBufs;
@@ -518,6 +524,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t box = 0;  // the next of the warp's two boxes
     int buf = 0;
     uint32_t aph = 0;
+    // the first 128 labels (the array is padded to as many)
+    const int4 labels0 = kMode == kDweight ? reinterpret_cast<const int4*>(p.labels)[lane]
+                                           : make_int4(-1, -1, -1, -1);
     for (int64_t u = first; u < g.units; u += stride) {
       const Unit x = unit_at(kMode, g, u, kTM);
       const int64_t row0 = x.m * kTM + rank * kCtaM;  // the CTA's first row
@@ -534,6 +543,63 @@ __global__ void __launch_bounds__(kThreads, 1)
           cb = p.cb[row] * scale;
         }
       }
+      // dW's rows of labels: d is largest there, and what its rounding took is added
+      // back below, b times 2^-9 of a hidden row.  The warp looks for its 32 tokens
+      // among the labels; where many of them are found their roundings average out,
+      // and stay.
+      const int token0 = static_cast<int>(p.col0 + row0) + quarter * 32;
+      int* mine = hits + quarter * kHits;
+      int found = 0;
+      if (kMode == kDweight) {
+        __syncwarp();
+        for (int i0 = 0; i0 < n; i0 += 128) {
+          const int i = i0 + lane * 4;
+          const int4 y = i0 == 0 ? labels0 : *reinterpret_cast<const int4*>(p.labels + i);
+          const int rel[4] = {y.x - token0, y.y - token0, y.z - token0, y.w - token0};
+          unsigned own = 0;  // bits of this lane's four
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            own |= (static_cast<unsigned>(rel[k]) < 32u && i + k < n ? 1u : 0u) << k;
+          if (!__any_sync(0xffffffffu, own != 0)) continue;
+          // in ascending order, so that sums have one order
+          int at = found;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const unsigned m = __ballot_sync(0xffffffffu, (own >> k & 1u) != 0);
+            at += __popc(m & ((1u << lane) - 1u));
+            found += __popc(m);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if ((own >> k & 1u) != 0) {
+              if (at < kHits) mine[at] = i + k;
+              ++at;
+            }
+        }
+        __syncwarp();
+        if (found > kHits) found = 0;
+      }
+      // the tile's columns of the first labels' hidden rows, eight a lane: asked for
+      // here, while the product runs, and handed around below
+      uint4 seg[kNear];
+      float left[kNear];
+      int who[kNear];
+      if (kMode == kDweight) {
+#pragma unroll
+        for (int e = 0; e < kNear; ++e) {
+          seg[e] = make_uint4(0, 0, 0, 0);
+          left[e] = 0.0f;
+          who[e] = -1;
+          if (e < found) {
+            const int slot = mine[e];
+            const int64_t col = x.n * kBN + lane * 8;
+            if (col < p.hidden)
+              seg[e] = static_cast<const uint4*>(p.packed)[slot * (p.hidden / 8) + col / 8];
+            left[e] = p.rest[slot];
+            who[e] = p.labels[slot] - token0;
+          }
+        }
+      }
       bool got = mbar_wait(&acc_full[buf], aph, abort, kWaitNs);
       got = __all_sync(0xffffffffu, got);
       if (!got) {
@@ -545,10 +611,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                              static_cast<uint32_t>(buf * kBN);
       const int64_t width = kMode == kLoss || kMode == kDlogits ? p.cols : p.hidden;
       const bool empty_split = kMode == kDhidden && x.k0 == x.k1;  // no product: zeros
-#pragma unroll 1
-      for (int c = 0; c < kBN; c += 32) {
+      // d is written to the tile's end, zeros past the vocabulary
+      const int64_t rest_cols = width - x.n * kBN;
+      const int cols = kMode == kDlogits || rest_cols > kBN ? kBN : static_cast<int>(rest_cols);
+      auto columns = [&](int c, auto corrected) {  // 32 of them
         const int64_t c0 = x.n * kBN + c;  // column of the output tile's matrix
-        if (c0 >= width && kMode != kDlogits) break;
         uint32_t t[32];
         tmem_issue32(taddr + static_cast<uint32_t>(c), t);
         tmem_wait32(t);
@@ -588,7 +655,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             add2(b0, b1, ex2(x2), ex2(x3));
           }
           sum += (a0 + a1) + (b0 + b1);
-          continue;
+          return;
         }
         if (kMode == kDlogits) {
           const int64_t rel = label - p.col0 - c0;
@@ -606,6 +673,43 @@ __global__ void __launch_bounds__(kThreads, 1)
             p.rest[row] = at - round16<T>(at);
           }
         } else if (kMode == kDweight) {
+          if constexpr (corrected.value) {
+            auto add = [&](float by, int q, uint32_t u0, uint32_t u1, uint32_t u2, uint32_t u3) {
+              const uint32_t u[4] = {u0, u1, u2, u3};
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float2 f = pair_of(T{}, u[j]);
+                v[8 * q + 2 * j] = fmaf(by, f.x, v[8 * q + 2 * j]);
+                v[8 * q + 2 * j + 1] = fmaf(by, f.y, v[8 * q + 2 * j + 1]);
+              }
+            };
+#pragma unroll
+            for (int e = 0; e < kNear; ++e) {
+              if (e >= found) break;
+              const float by = who[e] == lane ? left[e] : 0.0f;
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const int from = c / 8 + q;
+                add(by, q, __shfl_sync(0xffffffffu, seg[e].x, from),
+                    __shfl_sync(0xffffffffu, seg[e].y, from),
+                    __shfl_sync(0xffffffffu, seg[e].z, from),
+                    __shfl_sync(0xffffffffu, seg[e].w, from));
+              }
+            }
+            for (int e = kNear; e < found; ++e) {  // rarely more: straight from memory
+              const int slot = mine[e];
+              if (p.labels[slot] - token0 != lane) continue;
+              const uint4* h = static_cast<const uint4*>(p.packed) + slot * (p.hidden / 8) + c0 / 8;
+              const float by = p.rest[slot];
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                if (c0 + 8 * q >= width) break;
+                const uint4 w = h[q];
+                add(by, q, w.x, w.y, w.z, w.w);
+              }
+            }
+            __syncwarp();
+          }
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] *= inv;
         }
@@ -650,6 +754,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           box ^= 1u;
         }
+      };
+      // the loop without labels stays short: of few rows, dW is bound by it
+      if (kMode == kDweight && found > 0) {
+#pragma unroll 1
+        for (int c = 0; c < cols; c += 32) columns(c, std::true_type{});
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < cols; c += 32) columns(c, std::false_type{});
       }
       tc_fence_before();
       __syncwarp();
@@ -1131,6 +1243,7 @@ int run_backward(const Call& c, const float* lse, const float* grad_loss, const 
   p.cb = reinterpret_cast<const float*>(c.ws + l.pb);
   p.top = scaled ? reinterpret_cast<const uint32_t*>(c.ws + l.count) + 1 : nullptr;
   p.rest = reinterpret_cast<float*>(c.ws + l.rest);
+  p.packed = c.ws + l.packed;
   p.status = c.status;
   constexpr int kTM = kTileM<kPair>;
   const int64_t mt = padded / kTM, ht = (c.dim + kBN - 1) / kBN;
