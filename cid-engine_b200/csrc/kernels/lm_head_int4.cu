@@ -228,6 +228,12 @@ static_assert(128 * kCtrlRegs + 256 * kReadRegs + 256 * kUnpackRegs <=
 // blocks.  Unpacking warpgroup q & 1 fills A buffer (q & 1, (q >> 1) & 1), so with
 // one row block the warpgroups take turns at the stages; the accumulators form a
 // ring.
+//
+// Bound by issue slots: the unpacking warps' at few rows (16 x 128256 x 4096: 77
+// us, 272 MB from memory, 53 % of the slots), the read-back's at 64 rows, where
+// each group's 64 sums a weight row are scaled and added (147 us with the
+// statistics).  Three A buffers a warpgroup (104 us at 16 rows), four unpacking
+// warpgroups (87) and MMAs issued by the unpacking warps (201) were slower.
 template <typename T, int N, int S, int R, bool kResident>
 __global__ void __launch_bounds__(int4_threads(R), 1)
     int4_head_kernel(const __grid_constant__ CUtensorMap map_w,
@@ -828,6 +834,9 @@ __device__ __forceinline__ void load_codes(uint32_t* to, const uint32_t* from) {
 }
 
 // kStats: statistics instead of logits (their state costs registers).
+// Bound by the codes' bytes and the instructions that mask them, about evenly:
+// 8 rows x 128256 x 4096 in groups of 128 take 62 us (270 MB, 4.4 TB/s), in groups
+// of 64 95 us; 1 row x 32000 x 2048 is 15.7 us, most of it the call's own issue.
 template <typename T, int S, bool kStats>
 __global__ void __launch_bounds__(kRowsThreads, 1) int4_rows_kernel(RowsParams p) {
   constexpr int N = kRowsN;
@@ -1073,7 +1082,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1) int4_rows_kernel(RowsParams p
 }
 
 // One block turns one hidden row into the fp16 row of the products, its group
-// sums (8 sum h) and its scale 2^-e; rows past the last get zero sums.
+// sums (8 sum h) and its scale 2^-e; rows past the last get zero sums.  Bound by
+// latency: the product kernel's first codes are on their way meanwhile.
 constexpr int kPrepThreads = 256;
 
 template <typename T>
@@ -1153,7 +1163,8 @@ __device__ __forceinline__ uint32_t code_word(uint4 v, float r, float grow) {
 // a NaN or infinite weight leaves its group's scale NaN or infinite.
 // Bound by memory, 2.5 bytes a weight, once the divisions are gone: with them, and
 // a word every thread, 128256 x 4096 took 720 us; with one reciprocal a group and
-// exact remainders for the ties 493 us, 90 % of the issue slots.
+// exact remainders for the ties 493 us, 90 % of the issue slots; with the two
+// roundings 270 to 290 us, 4.6 to 4.9 TB/s.
 template <typename T>
 __global__ void __launch_bounds__(kQuantThreads)
     quantize_kernel(const uint4* weight, int64_t words, int lanes_log2, uint32_t* packed,
@@ -1200,6 +1211,7 @@ __global__ void __launch_bounds__(kQuantThreads)
   }
 }
 
+// Bound by memory: 128256 x 4096 in 199 us, 1.32 GB at 6.6 TB/s.
 template <typename T>
 __global__ void __launch_bounds__(kQuantThreads)
     dequantize_kernel(const uint32_t* packed, const T* scales, int64_t words, int lanes_log2,
@@ -1282,9 +1294,9 @@ size_t int4_smem(int n, int r, bool resident, int stages, int64_t chunks, int64_
 //
 // Up to 8 hidden rows against groups of 64 or 128 take int4_rows_kernel, where
 // they fit shared memory beside the sums.  Measured at 8 rows x 128256 x 4096, it
-// against the other: groups of 128 70 and 97 us, of 64 95 and 109 us, of 32 (an
-// accumulator and a load for every word) 166 and 130 us; 16 rows of groups of 128
-// 114 and 97 us.
+// against the other: groups of 128 62 and 77 us, of 64 95 and 107 us, of 32 (an
+// accumulator and a load for every word) 166 and 121 us; 16 rows of groups of 128
+// 114 and 77 us.
 Int4Plan int4_plan(int64_t rows, int64_t vocab, int64_t dim, int group) {
   Int4Plan pl;
   const int64_t blocks = (dim + kChunk - 1) / kChunk;

@@ -13,8 +13,9 @@
 // repeated calls give identical bits.
 //
 // The backward goes over the vocabulary in pieces: a piece's logits are
-// computed again, turned into d (16 bits) in a workspace, and multiplied with the weight (dh, summed in f32 over the pieces) and the
-// hidden rows (that piece's rows of dW).  8 n V H flops a step (2 forward, 2
+// computed again, turned into d (16 bits) in a workspace, and multiplied with the
+// weight (dh, summed in f32 over the pieces) and the hidden rows (that piece's rows
+// of dW).  8 n V H flops a step (2 forward, 2
 // again, 4 gradients) instead of 6 with kept logits, which would be n V floats.
 //
 // Roundings to 16 bits: d, because the tensor cores take 16-bit operands (the
@@ -53,7 +54,8 @@ constexpr int kHits = 64;
 constexpr int kNear = 4;  // of them held in registers
 constexpr int kThreads = 192;  // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
 constexpr int kRowGroup = 4096;  // rows whose row blocks share weight tiles in L2
-constexpr int kPrepRows = 8;   // rows a prepare block packs, one a warp
+constexpr int kPrepRows = 8;   // rows a prepare block packs at a time, one a warp
+constexpr int kPrepBlocks = 8;  // prepare blocks an SM, at most
 constexpr int kMaxSplits = 64;
 // Units the split of dh aims at: with four waves of 148 SMs the last wave
 // costs little, and the partial tiles stay within 75 MB.
@@ -327,6 +329,12 @@ __device__ __forceinline__ void box_out(const CUtensorMap* map, int32_t x, int32
 // In a pair, both CTAs load, and read back their half of the rows; the leader
 // (rank 0) counts both CTAs' loads on its `full` barriers and issues the MMAs,
 // whose commits arrive in both.
+//
+// Bound by the tensor cores and, at one to four waves of tiles, by the last wave:
+// 2867 kept rows x 128256 x 4096 run loss, d, dh and dW at 1541, 1547, 1447
+// and 1575 TFLOP/s one at a time (1270 to 1300 together, under the power cap);
+// 512 x 32000 x 2048 take 54.6, 58, 52 and 63.9 us (tensor pipe 63, 59, 66, 53 %).  Up to 128 rows it is
+// bound by memory: 24 x 128256 x 4096, 1.05 GB a launch, 176, 188, 154 and 244 us.
 
 template <typename T, Mode kMode, bool kPair>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -823,10 +831,13 @@ struct PrepParams {
   uint32_t* status;
 };
 
-// One block packs kPrepRows rows: it counts the kept rows before its own
-// (reading their labels, 8 bytes each from L2), then copies them.
+// One block packs kPrepRows rows at a time: it counts the kept rows before its own
+// (reading their labels, 8 bytes each from L2), then copies them.  Of many rows a
+// block packs several such groups one after the other, so that the labels are
+// read by kPrepBlocks blocks an SM at most.
 // The last block leaves the count and zeroes the rows up to the next multiple
-// of 16, the K step of dW = d^T h.
+// of 16, the K step of dW = d^T h.  Bound by latency, 7 to 8 us at 1024 rows and 14 at
+// 4096.
 __global__ void __launch_bounds__(32 * kPrepRows) head_prepare_kernel(PrepParams p) {
   __shared__ int warp_sum[kPrepRows];
   __shared__ int slots[kPrepRows];
@@ -834,63 +845,71 @@ __global__ void __launch_bounds__(32 * kPrepRows) head_prepare_kernel(PrepParams
   pdl_trigger();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * kPrepRows;
+  const int64_t groups = (p.rows + kPrepRows - 1) / kPrepRows;
+  const int64_t each = (groups + gridDim.x - 1) / gridDim.x;
+  const int64_t g0 = blockIdx.x * each, g1 = g0 + each < groups ? g0 + each : groups;
+  if (g0 >= g1) return;
   int before = 0;
-  for (int64_t i = threadIdx.x; i < r0; i += blockDim.x) {
+  for (int64_t i = threadIdx.x; i < g0 * kPrepRows; i += blockDim.x) {
     const int64_t y = p.labels[i];
     before += (y != p.ignore && y >= 0 && y < p.vocab) ? 1 : 0;
   }
   before = __reduce_add_sync(0xffffffffu, before);
   if (lane == 0) warp_sum[warp] = before;
   __syncthreads();
-  if (warp == 0) {
-    int base = lane < kPrepRows ? warp_sum[lane] : 0;
-    base = __reduce_add_sync(0xffffffffu, base);
-    const int64_t r = r0 + lane;
-    const bool mine = lane < kPrepRows && r < p.rows;
-    const int64_t y = mine ? p.labels[r] : p.ignore;
-    const bool ignored = y == p.ignore;
-    const bool kept = mine && !ignored && y >= 0 && y < p.vocab;
-    const unsigned mask = __ballot_sync(0xffffffffu, kept);
-    const int slot =
-        kept ? base + __popc(mask & ((1u << lane) - 1u)) : (ignored ? kIgnored : kBadLabel);
-    if (mine) {
-      p.slot_of[r] = slot;
-      if (slot == kBadLabel && p.status) atomicOr(p.status, CID_STATUS_TOKEN_ID_OUT_OF_RANGE);
-    }
-    if (kept) {
-      p.plabel[slot] = static_cast<int>(y);
-      if (p.lse != nullptr) {
-        const float gl = p.grad_loss ? p.grad_loss[r] : 0.0f;
-        const float ge = p.grad_lse ? p.grad_lse[r] : 0.0f;
-        p.plse[slot] = p.lse[r];
-        p.pa[slot] = gl + ge;
-        p.pb[slot] = gl;
-        if (p.top) atomicMax(p.top, __float_as_uint(fmaxf(fabsf(gl + ge), fabsf(gl))));
+  int base = lane < kPrepRows ? warp_sum[lane] : 0;  // kept rows before the group
+  base = __reduce_add_sync(0xffffffffu, base);
+  for (int64_t g = g0; g < g1; ++g) {
+    const int64_t r0 = g * kPrepRows;
+    if (warp == 0) {
+      const int64_t r = r0 + lane;
+      const bool mine = lane < kPrepRows && r < p.rows;
+      const int64_t y = mine ? p.labels[r] : p.ignore;
+      const bool ignored = y == p.ignore;
+      const bool kept = mine && !ignored && y >= 0 && y < p.vocab;
+      const unsigned mask = __ballot_sync(0xffffffffu, kept);
+      const int slot =
+          kept ? base + __popc(mask & ((1u << lane) - 1u)) : (ignored ? kIgnored : kBadLabel);
+      if (mine) {
+        p.slot_of[r] = slot;
+        if (slot == kBadLabel && p.status) atomicOr(p.status, CID_STATUS_TOKEN_ID_OUT_OF_RANGE);
       }
+      if (kept) {
+        p.plabel[slot] = static_cast<int>(y);
+        if (p.lse != nullptr) {
+          const float gl = p.grad_loss ? p.grad_loss[r] : 0.0f;
+          const float ge = p.grad_lse ? p.grad_lse[r] : 0.0f;
+          p.plse[slot] = p.lse[r];
+          p.pa[slot] = gl + ge;
+          p.pb[slot] = gl;
+          if (p.top) atomicMax(p.top, __float_as_uint(fmaxf(fabsf(gl + ge), fabsf(gl))));
+        }
+      }
+      if (lane < kPrepRows) slots[lane] = mine ? slot : kIgnored;
+      if (lane == 0) total = base + __popc(mask);
     }
-    if (lane < kPrepRows) slots[lane] = mine ? slot : kIgnored;
-    if (lane == 0) total = base + __popc(mask);
-  }
-  __syncthreads();
-  // the block's kept rows, piece by piece: eight loads of a thread in flight
-  constexpr int kFlight = 8;
-  const uint32_t vecs = static_cast<uint32_t>(p.vecs), units = kPrepRows * vecs;
-  for (uint32_t i0 = threadIdx.x; i0 < units; i0 += kFlight * blockDim.x) {
-    uint4 v[kFlight];
-    int to[kFlight];
+    __syncthreads();
+    // the block's kept rows, piece by piece: eight loads of a thread in flight
+    constexpr int kFlight = 8;
+    const uint32_t vecs = static_cast<uint32_t>(p.vecs), units = kPrepRows * vecs;
+    for (uint32_t i0 = threadIdx.x; i0 < units; i0 += kFlight * blockDim.x) {
+      uint4 v[kFlight];
+      int to[kFlight];
 #pragma unroll
-    for (int j = 0; j < kFlight; ++j) {
-      const uint32_t i = i0 + j * blockDim.x;
-      to[j] = i < units ? slots[i / vecs] : kIgnored;
-      if (to[j] >= 0) v[j] = p.hidden[r0 * p.vecs + i];
+      for (int j = 0; j < kFlight; ++j) {
+        const uint32_t i = i0 + j * blockDim.x;
+        to[j] = i < units ? slots[i / vecs] : kIgnored;
+        if (to[j] >= 0) v[j] = p.hidden[r0 * p.vecs + i];
+      }
+#pragma unroll
+      for (int j = 0; j < kFlight; ++j)
+        if (to[j] >= 0) p.packed[to[j] * p.vecs + (i0 + j * blockDim.x) % vecs] = v[j];
     }
-#pragma unroll
-    for (int j = 0; j < kFlight; ++j)
-      if (to[j] >= 0) p.packed[to[j] * p.vecs + (i0 + j * blockDim.x) % vecs] = v[j];
+    base = total;
+    __syncthreads();  // slots and total are free for the next group
   }
-  if (r0 + kPrepRows >= p.rows) {
-    const int n = total;
+  if (g1 == groups) {
+    const int n = base;
     const int64_t pad = n > 0 ? (static_cast<int64_t>(n) + 15) / 16 * 16 : 16;
     for (int64_t i = n * p.vecs + threadIdx.x; i < pad * p.vecs; i += blockDim.x)
       p.packed[i] = make_uint4(0, 0, 0, 0);
@@ -907,7 +926,8 @@ __global__ void __launch_bounds__(32 * kPrepRows) head_prepare_kernel(PrepParams
 }
 
 // loss and log-sum-exp of 32 rows a block from the tiles' (max, sum of exp), the
-// tiles dealt to kLossParts warps
+// tiles dealt to kLossParts warps: 7.5 us for 512 rows of 125 tiles, 11 us for 2867
+// rows of 501.  The sums' merges chain, so more warps a row, not more bytes, count.
 constexpr int kLossParts = 32;
 
 __global__ void __launch_bounds__(32 * kLossParts)
@@ -961,7 +981,8 @@ __global__ void __launch_bounds__(32 * kLossParts)
 // dh of every row: the splits' partial sums in ascending order, and what rounding
 // took from d at the label times the label's weight row (d is largest there, and
 // its rounding is most of what the sum would be off by); 16 bits.  Zero for an
-// ignored row, NaN for a label that is no token.
+// ignored row, NaN for a label that is no token.  Bound by memory and latency: 12 us
+// for 1024 rows x 2048, 35 us for 4096 x 4096.
 template <typename T>
 __global__ void __launch_bounds__(256)
     head_dhidden_kernel(const float* partial, const int* slot_of, const int* plabel,
@@ -1175,7 +1196,8 @@ int launch_prepare(const Call& c, const Layout& l, const float* lse, const float
     const cudaError_t e = cudaMemsetAsync(q.top, 0, 4, c.stream);
     if (e != cudaSuccess) return record_cuda_error(e);
   }
-  const int64_t blocks = (c.rows + kPrepRows - 1) / kPrepRows;
+  int64_t blocks = (c.rows + kPrepRows - 1) / kPrepRows;
+  if (blocks > int64_t{kPrepBlocks} * sm_count()) blocks = int64_t{kPrepBlocks} * sm_count();
   return launch_pdl(head_prepare_kernel, dim3(static_cast<unsigned>(blocks)),
                     dim3(32 * kPrepRows), 0, c.stream, q);
 }

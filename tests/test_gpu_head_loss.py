@@ -399,3 +399,37 @@ def test_many_rows_few_labels() -> None:
     y, h, w, gl, ge = _inputs(2000, 4000, 192, BF16, "all")
     y[torch.arange(2000, device=y.device) % 167 != 3] = -100
     _check(y, h, w, gl, ge)
+
+
+@pytest.mark.parametrize("keep", ["half", "last"])
+def test_more_rows_than_packing_blocks(keep) -> None:
+    """Of many rows a packing block takes several groups, one after the other."""
+    _check(*_inputs(20011, 300, 64, BF16, keep))
+
+
+def test_fp16_graphs_that_share_a_pool() -> None:
+    """Two captured steps whose workspaces come from one pool, replayed in turn."""
+    import cid_engine
+
+    pool = torch.cuda.graph_pool_handle()
+    steps = []
+    for rows, vocab, hidden in ((300, 2000, 128), (60, 5000, 72)):
+        y, h, w, gl, ge = _inputs(rows, vocab, hidden, FP16)
+        hr, wr = h.clone().requires_grad_(), w.clone().requires_grad_()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            out = cid_engine.lm_head_cross_entropy(y, hr, wr)
+            torch.autograd.grad(out, (hr, wr), grad_outputs=(gl, ge))
+        torch.cuda.current_stream().wait_stream(side)
+        del out
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            out = cid_engine.lm_head_cross_entropy(y, hr, wr)
+            got = (*out, *torch.autograd.grad(out, (hr, wr), grad_outputs=(gl, ge)))
+        steps.append((graph, got, _step(y, h, w, gl, ge), (y, hr, wr, gl, ge)))
+    for _ in range(3):
+        for graph, got, want, _ in steps:
+            graph.replay()
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)
