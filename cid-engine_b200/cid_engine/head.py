@@ -74,9 +74,9 @@ def lm_head_dequantize(packed: Tensor, scales: Tensor) -> Tensor:
 def lm_head_quantized_logits(hidden: Tensor, packed: Tensor, scales: Tensor) -> Tensor:
     """``hidden [*, H]`` times the 4-bit weight: ``[*, vocab]`` logits in
     hidden's dtype (the scales' dtype too).  Each group's sum is accumulated
-    and scaled in float32; the logits are rounded once.  Made for few rows, up
-    to some hundred: the weight is read once for every 64 of them (32 with
-    groups of 64, 16 with groups of 32).  H is at most 32768.  A hidden row with
+    and scaled in float32; the logits are rounded once.  Made for few rows:
+    the weight is read once for every 64 of them (32 with groups of 64, 16
+    with groups of 32), and beyond that the 16-bit weight is faster.  H is at most 32768.  A hidden row with
     a NaN or infinite value has NaN logits.  Not differentiable."""
     return torch.ops.cid_engine.lm_head_quantized_logits(hidden, packed, scales)
 
