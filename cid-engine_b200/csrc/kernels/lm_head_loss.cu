@@ -51,7 +51,8 @@ constexpr uint32_t kBoxBytes = 32 * 128;
 constexpr uint32_t kBoxRegion = 4 * 2 * kBoxBytes;
 // Labels among a warp's 32 tokens whose part of dW gets its rounding back.
 constexpr int kHits = 64;
-constexpr int kNear = 4;  // of them held in registers
+constexpr int kNear = 4;  // no more than these: their hidden rows wait in registers
+constexpr int kLabelMost = 4;  // of one token, where there are more than kNear
 constexpr int kThreads = 192;  // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
 constexpr int kRowGroup = 4096;  // rows whose row blocks share weight tiles in L2
 constexpr int kPrepRows = 8;   // rows a prepare block packs at a time, one a warp
@@ -75,9 +76,12 @@ template <bool kPair>
 constexpr int kStages = kPair ? 6 : 4;
 template <bool kPair>
 constexpr size_t kSmemBytes =
-    kStages<kPair> * size_t{kStageBytes<kPair>} + kBoxRegion + 4 * kHits * sizeof(int) + 1024 + 512;
+    kStages<kPair> * size_t{kStageBytes<kPair>} + kBoxRegion + 4 * kHits * (sizeof(int) + 1) + 1024 + 512;
 static_assert(kSmemBytes<true> <= 227 * 1024 && kSmemBytes<false> <= 227 * 1024,
               "shared memory of one CTA");
+
+// Where an epilogue of kDweight finds the hidden rows of its tokens' labels.
+enum Labels { kNone, kClose, kFar };
 
 enum Mode {
   kLoss,     // A = hidden rows, B = weight rows: (max, sum of exp) a row and tile, label logits
@@ -350,7 +354,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   unsigned char* stage_b = smem + kS * kStageA;
   unsigned char* boxes = smem + kS * kStageBytes<kPair>;
   int* hits = reinterpret_cast<int*>(boxes + kBoxRegion);  // [4][kHits]
-  uint64_t* full = reinterpret_cast<uint64_t*>(hits + 4 * kHits);
+  unsigned char* hit_tokens = reinterpret_cast<unsigned char*>(hits + 4 * kHits);
+  uint64_t* full = reinterpret_cast<uint64_t*>(hit_tokens + 4 * kHits);
   uint64_t* empty = full + kS;
   uint64_t* acc_full = empty + kS;
   uint64_t* acc_empty = acc_full + kAccBufs;
@@ -557,6 +562,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // and stay.
       const int token0 = static_cast<int>(p.col0 + row0) + quarter * 32;
       int* mine = hits + quarter * kHits;
+      unsigned char* tokens = hit_tokens + quarter * kHits;
       int found = 0;
       if (kMode == kDweight) {
         __syncwarp();
@@ -580,15 +586,22 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             if ((own >> k & 1u) != 0) {
-              if (at < kHits) mine[at] = i + k;
+              if (at < kHits) {
+                mine[at] = i + k;
+                tokens[at] = static_cast<unsigned char>(rel[k]);
+              }
               ++at;
             }
         }
         __syncwarp();
         if (found > kHits) found = 0;
       }
-      // the tile's columns of the first labels' hidden rows, eight a lane: asked for
-      // here, while the product runs, and handed around below
+      // Few labels: the tile's columns of their hidden rows, eight a lane, asked for
+      // here, while the product runs, and handed around below.  More of them: each lane
+      // keeps those of its own token and reads their rows as it comes to them; a token
+      // with more than kLabelMost is left as it is, its roundings average out.  (Read
+      // one label after another by the whole warp, a backward of 512 rows x 4096 x 512
+      // took 73 us, and of 64 rows with labels among 32 tokens 252; so 50 and 46.)
       uint4 seg[kNear];
       float left[kNear];
       int who[kNear];
@@ -598,13 +611,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           seg[e] = make_uint4(0, 0, 0, 0);
           left[e] = 0.0f;
           who[e] = -1;
-          if (e < found) {
+          if (e < found && found <= kNear) {
             const int slot = mine[e];
             const int64_t col = x.n * kBN + lane * 8;
             if (col < p.hidden)
               seg[e] = static_cast<const uint4*>(p.packed)[slot * (p.hidden / 8) + col / 8];
             left[e] = p.rest[slot];
-            who[e] = p.labels[slot] - token0;
+            who[e] = tokens[e];
           }
         }
       }
@@ -622,8 +635,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       // d is written to the tile's end, zeros past the vocabulary
       const int64_t rest_cols = width - x.n * kBN;
       const int cols = kMode == kDlogits || rest_cols > kBN ? kBN : static_cast<int>(rest_cols);
-      auto columns = [&](int c, auto corrected) {  // 32 of them
+      auto columns = [&](int c, auto corrected, uint64_t own_hits) {  // 32 of them
         const int64_t c0 = x.n * kBN + c;  // column of the output tile's matrix
+        // the lane's next label: its hidden row's columns and what rounding took
+        uint64_t ahead = own_hits;
+        uint4 far[4] = {};
+        float far_by = 0.0f;
+        bool fetched = false;
+        auto fetch = [&] {
+          fetched = ahead != 0;
+          if (!fetched) return;
+          const int slot = mine[__ffsll(static_cast<long long>(ahead)) - 1];
+          const uint4* h = static_cast<const uint4*>(p.packed) + slot * (p.hidden / 8) + c0 / 8;
+          far_by = p.rest[slot];
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (c0 + 8 * q < width) far[q] = h[q];
+          ahead &= ahead - 1;
+        };
+        if constexpr (corrected.value == kFar) {
+          fetch();
+          __syncwarp();
+        }
         uint32_t t[32];
         tmem_issue32(taddr + static_cast<uint32_t>(c), t);
         tmem_wait32(t);
@@ -681,7 +714,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             p.rest[row] = at - round16<T>(at);
           }
         } else if (kMode == kDweight) {
-          if constexpr (corrected.value) {
+          if constexpr (corrected.value != kNone) {
             auto add = [&](float by, int q, uint32_t u0, uint32_t u1, uint32_t u2, uint32_t u3) {
               const uint32_t u[4] = {u0, u1, u2, u3};
 #pragma unroll
@@ -692,7 +725,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             };
 #pragma unroll
-            for (int e = 0; e < kNear; ++e) {
+            for (int e = 0; e < (corrected.value == kClose ? kNear : 0); ++e) {
               if (e >= found) break;
               const float by = who[e] == lane ? left[e] : 0.0f;
 #pragma unroll
@@ -704,17 +737,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     __shfl_sync(0xffffffffu, seg[e].w, from));
               }
             }
-            for (int e = kNear; e < found; ++e) {  // rarely more: straight from memory
-              const int slot = mine[e];
-              if (p.labels[slot] - token0 != lane) continue;
-              const uint4* h = static_cast<const uint4*>(p.packed) + slot * (p.hidden / 8) + c0 / 8;
-              const float by = p.rest[slot];
+            while (corrected.value == kFar && fetched) {
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                if (c0 + 8 * q >= width) break;
-                const uint4 w = h[q];
-                add(by, q, w.x, w.y, w.z, w.w);
-              }
+              for (int q = 0; q < 4; ++q) add(far_by, q, far[q].x, far[q].y, far[q].z, far[q].w);
+              fetch();
             }
             __syncwarp();
           }
@@ -764,12 +790,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       };
       // the loop without labels stays short: of few rows, dW is bound by it
-      if (kMode == kDweight && found > 0) {
+      if (kMode != kDweight || found == 0) {
 #pragma unroll 1
-        for (int c = 0; c < cols; c += 32) columns(c, std::true_type{});
+        for (int c = 0; c < cols; c += 32) columns(c, std::integral_constant<int, kNone>{}, 0);
+      } else if (found <= kNear) {
+#pragma unroll 1
+        for (int c = 0; c < cols; c += 32) columns(c, std::integral_constant<int, kClose>{}, 0);
       } else {
+        uint64_t own_hits = 0;
 #pragma unroll 1
-        for (int c = 0; c < cols; c += 32) columns(c, std::false_type{});
+        for (int e = 0; e < found; ++e)
+          own_hits |= static_cast<uint64_t>(tokens[e] == lane ? 1 : 0) << e;
+        if (__popcll(own_hits) > kLabelMost) own_hits = 0;
+#pragma unroll 1
+        for (int c = 0; c < cols; c += 32) columns(c, std::integral_constant<int, kFar>{}, own_hits);
       }
       tc_fence_before();
       __syncwarp();

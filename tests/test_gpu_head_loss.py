@@ -433,3 +433,24 @@ def test_fp16_graphs_that_share_a_pool() -> None:
             graph.replay()
             for a, b in zip(got, want):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("rows,tokens,hidden", [
+    (64, 40, 72),     # two warps' tokens take every label, no more than are looked after
+    (64, 32, 264),
+    (40, 1, 520),     # one token's alone
+    (200, 40, 136),   # more than are looked after
+    (30, 17, 256),
+])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_labels_of_few_tokens(rows, tokens, hidden, dtype) -> None:
+    """dW's rows of the labels, where many of them are neighbours; a row without a
+    gradient stands among them."""
+    y, h, w, gl, ge = _inputs(rows, 2000, hidden, dtype, "all")
+    y = 32 * 11 + y % tokens
+    gl[rows // 2] = ge[rows // 2] = 0.0
+    _check(y, h, w, gl, ge)
+    y[rows // 4] = -100
+    got = _check(y, h, w, gl, ge)
+    for a, b in zip(_step(y, h, w, gl, ge), got):
+        assert torch.equal(a, b)
