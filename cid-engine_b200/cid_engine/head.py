@@ -39,8 +39,9 @@ def lm_head_cross_entropy(
 
     Differentiable once in ``hidden`` and ``weight``, through both outputs:
     weight the positions (``(loss * scale).sum()``), average them, or add a
-    penalty of the log-sum-exp.  The backward computes the logits again, a
-    piece of the vocabulary at a time."""
+    penalty of the log-sum-exp.  Inputs with a forward-mode tangent (dual
+    tensors, ``torch.func.jvp``) are refused.  The backward computes the logits
+    again, a piece of the vocabulary at a time."""
     return torch.ops.cid_engine.lm_head_cross_entropy(labels, hidden, weight, ignore_index)
 
 

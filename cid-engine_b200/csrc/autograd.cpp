@@ -82,6 +82,15 @@ struct HeadLossBackward : torch::autograd::Function<HeadLossBackward> {
   }
 };
 
+// There is no forward-mode derivative.  A tensor with a tangent need not require a
+// gradient, so this is looked at whether or not a graph is recorded: without the
+// check the outputs would carry no tangent, which reads as a derivative of zero.
+void refuse_tangents(const char* op, std::initializer_list<const at::Tensor*> tensors) {
+  for (const auto* t : tensors)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), "cid_engine.", op,
+                " has no forward-mode derivative (dual tensors, torch.func.jvp)");
+}
+
 // Whether a graph is being recorded over any of the tensors; without one the
 // nodes below would cost a call their set-up for nothing.
 bool recording(std::initializer_list<const at::Tensor*> tensors) {
@@ -93,6 +102,7 @@ bool recording(std::initializer_list<const at::Tensor*> tensors) {
 
 Pair forward_autograd(const at::Tensor& labels, const at::Tensor& hidden,
                       const at::Tensor& weight, std::int64_t ignore) {
+  refuse_tangents("lm_head_cross_entropy", {&hidden, &weight});
   if (!recording({&hidden, &weight})) {
     at::AutoDispatchBelowADInplaceOrView below;
     return call_forward(labels, hidden, weight, ignore);
@@ -106,7 +116,10 @@ Pair backward_autograd(const std::optional<at::Tensor>& gl, const std::optional<
                        const at::Tensor& weight, const at::Tensor& lse, std::int64_t ignore,
                        bool need_hidden, bool need_weight) {
   const at::Tensor none;
-  if (!recording({gl ? &*gl : &none, ge ? &*ge : &none, &hidden, &weight, &lse})) {
+  const std::initializer_list<const at::Tensor*> inputs = {gl ? &*gl : &none, ge ? &*ge : &none,
+                                                           &hidden, &weight, &lse};
+  refuse_tangents("lm_head_cross_entropy_backward", inputs);
+  if (!recording(inputs)) {
     at::AutoDispatchBelowADInplaceOrView below;
     return call_backward(gl, ge, labels, hidden, weight, lse, ignore, need_hidden, need_weight);
   }

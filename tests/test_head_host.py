@@ -250,3 +250,65 @@ def test_int4_c_abi_checks(lib: ctypes.CDLL) -> None:
     assert stats(ids=0x4004) == MISALIGNED and stats(ws=0x6008) == MISALIGNED
     assert stats(ids=0) == INVALID and stats(ws=0) == INVALID and stats(rows=0) == OK
     assert stats(bytes_=need(2, 128, 300, 64, 1) - 1) == SCRATCH
+
+
+@pytest.mark.parametrize("which", ["hidden", "weight"])
+@pytest.mark.parametrize("recorded", [False, True])
+@pytest.mark.parametrize("grad_mode", [False, True])
+def test_loss_refuses_tangents(which, recorded, grad_mode) -> None:
+    """A dual tensor is refused whether or not a graph is being recorded: outputs
+    without a tangent would stand for a derivative of zero."""
+    y, h, w = _loss_inputs("meta", grad=recorded)
+    with torch.autograd.forward_ad.dual_level(), torch.set_grad_enabled(grad_mode):
+        make = torch.autograd.forward_ad.make_dual
+        if which == "hidden":
+            h = make(h, torch.ones_like(h))
+        else:
+            w = make(w, torch.ones_like(w))
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            cid_engine.lm_head_cross_entropy(y, h, w)
+
+
+def test_loss_refuses_forward_transforms() -> None:
+    y, h, w = _loss_inputs("meta")
+    with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+        torch.func.jvp(lambda a: cid_engine.lm_head_cross_entropy(y, a, w)[0], (h,),
+                       (torch.ones_like(h),))
+    with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+        torch.func.jacfwd(lambda a: cid_engine.lm_head_cross_entropy(y[0, :1], a, w)[0])(h[0, :1])
+    with pytest.raises(RuntimeError, match="functorch"):
+        torch.func.grad(lambda a: cid_engine.lm_head_cross_entropy(y, a, w)[0].sum())(h)
+
+
+@pytest.mark.parametrize("place", [0, 1, 3, 4, 5])
+def test_loss_backward_refuses_tangents(place) -> None:
+    y, h, w = _loss_inputs("meta")
+    args = [torch.zeros(3, 5, device="meta"), torch.zeros(3, 5, device="meta"), y, h, w,
+            torch.zeros(3, 5, device="meta")]
+    b = torch.ops.cid_engine.lm_head_cross_entropy_backward
+    assert b(*args, -100, True, True)[0].shape == h.shape
+    with torch.autograd.forward_ad.dual_level():
+        args[place] = torch.autograd.forward_ad.make_dual(args[place], torch.ones_like(args[place]))
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            b(*args, -100, True, True)
+
+
+def test_loss_backward_refuses_a_dual_output_gradient() -> None:
+    y, h, w = _loss_inputs("meta", grad=True)
+    loss, _ = cid_engine.lm_head_cross_entropy(y, h, w)
+    with torch.autograd.forward_ad.dual_level():
+        g = torch.autograd.forward_ad.make_dual(torch.ones(3, 5, device="meta"),
+                                                torch.ones(3, 5, device="meta"))
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            torch.autograd.grad(loss, h, g)
+
+
+@pytest.mark.filterwarnings("ignore:There is a performance drop")
+def test_loss_under_vmap_keeps_shapes() -> None:
+    """vmap runs the operator once for each item; a graph is recorded through it."""
+    y, h, w = _loss_inputs("meta")
+    h.requires_grad_()
+    loss, lse = torch.vmap(lambda a, b: cid_engine.lm_head_cross_entropy(a, b, w))(y, h)
+    assert loss.shape == lse.shape == (3, 5) and loss.requires_grad
+    (gh,) = torch.autograd.grad(loss.sum(), h)
+    assert gh.shape == h.shape
