@@ -425,3 +425,39 @@ def test_hidden_rows_of_every_size(rows, dtype) -> None:
     tol = dz * (1 + u) + u * z.abs() + torch.finfo(dtype).smallest_normal * u * 2 + 2.0**-149
     assert bool(((got - z).abs() <= tol)[ok].all())
     assert not bool(got[3].any())
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("rows,vocab,hidden,group", [
+    # hidden rows in shared memory, 16 a pass, two groups a chunk
+    (12, 1000, 320, 64),
+    (16, 40000, 2112, 64),
+    # hidden rows streamed beside the codes, one and two tiles of 256 weight rows a CTA
+    (24, 40000, 4096, 64),
+    (12, 40000, 5184, 64),   # a K tail of a chunk
+    (12, 40000, 8192, 128),
+    (16, 40000, 8224, 32),
+    (33, 3000, 32768, 128),  # the widest hidden rows
+    (32, 3000, 32768, 64),
+    (16, 3000, 32768, 32),
+    (5, 3000, 32768, 128),   # 8 rows that do not fit the small-row kernel
+    (8, 1001, 16384, 64),
+    # the small-row kernel with half a block of columns at the end
+    (4, 3000, 64, 64),
+    (7, 1000, 192, 64),
+    (8, 20000, 1088, 64),
+    (1, 129, 64, 64),
+])
+def test_every_form_of_the_products(rows, vocab, hidden, group, dtype) -> None:
+    """Sizes that reach the forms of the two product kernels beside those above,
+    for the logits and for the statistics."""
+    import cid_engine
+
+    cid_engine.device_status(0, reset=True)
+    ids, h, head, z, dz = _inputs(rows, vocab, hidden, group, dtype)
+    got = cid_engine.lm_head_quantized_logits(h, *head)
+    u = torch.finfo(dtype).eps / 2
+    off = (got.double() - z).abs()
+    tol = dz * (1 + u) + u * z.abs() + (2.0**-25 if dtype == FP16 else 0.0)
+    assert bool((off <= tol).all()), f"worst {float((off / tol).max()):.3g} of the tolerance"
+    _check_stats(ids, h, head, z, dz)
