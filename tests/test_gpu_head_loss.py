@@ -454,3 +454,20 @@ def test_labels_of_few_tokens(rows, tokens, hidden, dtype) -> None:
     got = _check(y, h, w, gl, ge)
     for a, b in zip(_step(y, h, w, gl, ge), got):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("scale,small", [(65536.0, 2.0**-8), (1e-6, 1.0)])
+def test_loss_scales_of_fp16_training(scale, small) -> None:
+    """A loss scale of 65536 (on inputs small enough for the outputs' range) and
+    position weights of 1e-6."""
+    y, h, w, gl, ge = _inputs(100, 3000, 64, FP16)
+    _check(y, h * small, w * small, gl * scale, ge * scale)
+
+
+def test_coefficients_of_many_binades_in_fp16() -> None:
+    """Rows whose coefficients span 2^30: one power of two serves all of them, so
+    elements of d keep an absolute 2^-37 of the largest coefficient (the term
+    ``dsub`` of the tolerances)."""
+    y, h, w, gl, ge = _inputs(160, 3000, 64, FP16)
+    s = torch.exp2(5.0 - torch.arange(160, device=h.device) % 31)
+    _check(y, h, w, gl * s, ge * s)
