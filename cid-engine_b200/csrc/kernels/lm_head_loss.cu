@@ -49,10 +49,13 @@ constexpr uint32_t kStageA = kCtaM * kBK * 2;
 // each epilogue warp.
 constexpr uint32_t kBoxBytes = 32 * 128;
 constexpr uint32_t kBoxRegion = 4 * 2 * kBoxBytes;
-// Labels among a warp's 32 tokens whose part of dW gets its rounding back.
-constexpr int kHits = 64;
-constexpr int kNear = 4;  // no more than these: their hidden rows wait in registers
-constexpr int kLabelMost = 4;  // of one token, where there are more than kNear
+// Labels whose part of dW gets its rounding back: up to kLabelMost of a token, whatever
+// the other tokens' labels.  Where a warp's 32 tokens have no more than kNear in all,
+// the labels' hidden rows wait in registers.
+constexpr int kNear = 4;
+constexpr int kLabelMost = 4;
+// Of each epilogue warp: a word for each of its tokens, and kNear rows and tokens.
+constexpr uint32_t kHitBytes = 4 * (32 + 2 * kNear);
 constexpr int kThreads = 192;  // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
 constexpr int kRowGroup = 4096;  // rows whose row blocks share weight tiles in L2
 constexpr int kPrepRows = 8;   // rows a prepare block packs at a time, one a warp
@@ -76,7 +79,7 @@ template <bool kPair>
 constexpr int kStages = kPair ? 6 : 4;
 template <bool kPair>
 constexpr size_t kSmemBytes =
-    kStages<kPair> * size_t{kStageBytes<kPair>} + kBoxRegion + 4 * kHits * (sizeof(int) + 1) + 1024 + 512;
+    kStages<kPair> * size_t{kStageBytes<kPair>} + kBoxRegion + 4 * kHitBytes + 1024 + 512;
 static_assert(kSmemBytes<true> <= 227 * 1024 && kSmemBytes<false> <= 227 * 1024,
               "shared memory of one CTA");
 
@@ -353,9 +356,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   unsigned char* stage_a = smem;
   unsigned char* stage_b = smem + kS * kStageA;
   unsigned char* boxes = smem + kS * kStageBytes<kPair>;
-  int* hits = reinterpret_cast<int*>(boxes + kBoxRegion);  // [4][kHits]
-  unsigned char* hit_tokens = reinterpret_cast<unsigned char*>(hits + 4 * kHits);
-  uint64_t* full = reinterpret_cast<uint64_t*>(hit_tokens + 4 * kHits);
+  unsigned char* hits = boxes + kBoxRegion;
+  uint64_t* full = reinterpret_cast<uint64_t*>(hits + 4 * kHitBytes);
   uint64_t* empty = full + kS;
   uint64_t* acc_full = empty + kS;
   uint64_t* acc_empty = acc_full + kAccBufs;
@@ -537,6 +539,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t box = 0;  // the next of the warp's two boxes
     int buf = 0;
     uint32_t aph = 0;
+    unsigned* seen = reinterpret_cast<unsigned*>(hits + quarter * kHitBytes);  // [32]
+    int* mine = reinterpret_cast<int*>(seen + 32);                             // [kNear]
+    int* tokens = mine + kNear;                                                // [kNear]
+    if (kMode == kDweight) seen[lane] = 0;
     // the first 128 labels (the array is padded to as many)
     const int4 labels0 = kMode == kDweight ? reinterpret_cast<const int4*>(p.labels)[lane]
                                            : make_int4(-1, -1, -1, -1);
@@ -556,16 +562,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           cb = p.cb[row] * scale;
         }
       }
-      // dW's rows of labels: d is largest there, and what its rounding took is added
-      // back below, b times 2^-9 of a hidden row.  The warp looks for its 32 tokens
-      // among the labels; where many of them are found their roundings average out,
-      // and stay.
+      // dW's rows of labels: the label's element of d is b (1 - p) large, and what its
+      // rounding took is added back below, b times 2^-9 of a hidden row.  The warp looks
+      // for its 32 tokens among the labels, and each lane keeps those of its own token
+      // in ascending order, so that sums have one order.  A token with more than
+      // kLabelMost keeps its elements' roundings and is looked for no further, so that a
+      // frequent label takes nothing from its neighbours.
       const int token0 = static_cast<int>(p.col0 + row0) + quarter * 32;
-      int* mine = hits + quarter * kHits;
-      unsigned char* tokens = hit_tokens + quarter * kHits;
-      int found = 0;
+      int found = 0, own_count = 0, own_slot[kLabelMost] = {};  // of all tokens, of the lane's
       if (kMode == kDweight) {
         __syncwarp();
+        unsigned many = 0;  // tokens with more than kLabelMost
         for (int i0 = 0; i0 < n; i0 += 128) {
           const int i = i0 + lane * 4;
           const int4 y = i0 == 0 ? labels0 : *reinterpret_cast<const int4*>(p.labels + i);
@@ -575,31 +582,59 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int k = 0; k < 4; ++k)
             own |= (static_cast<unsigned>(rel[k]) < 32u && i + k < n ? 1u : 0u) << k;
           if (!__any_sync(0xffffffffu, own != 0)) continue;
-          // in ascending order, so that sums have one order
-          int at = found;
+          if (many != 0) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if ((many >> (rel[k] & 31) & 1u) != 0) own &= ~(1u << k);
+          }
+          found = 1;
+          // the lanes whose k-th label is this lane's token, by way of the token's word
+          unsigned by[4], left_over = 0;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const unsigned m = __ballot_sync(0xffffffffu, (own >> k & 1u) != 0);
-            at += __popc(m & ((1u << lane) - 1u));
-            found += __popc(m);
+            by[k] = 0;
+            if (!__any_sync(0xffffffffu, (own >> k & 1u) != 0)) continue;
+            if ((own >> k & 1u) != 0) atomicOr(&seen[rel[k]], 1u << lane);
+            __syncwarp();
+            by[k] = seen[lane];
+            seen[lane] = 0;
+            left_over |= by[k];
+            __syncwarp();
           }
+          while (left_over != 0 && own_count <= kLabelMost) {
+            const int from = __ffs(static_cast<int>(left_over)) - 1;
+            left_over &= left_over - 1;
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if ((own >> k & 1u) != 0) {
-              if (at < kHits) {
-                mine[at] = i + k;
-                tokens[at] = static_cast<unsigned char>(rel[k]);
+            for (int k = 0; k < 4; ++k)
+              if ((by[k] >> from & 1u) != 0) {
+#pragma unroll
+                for (int e = 0; e < kLabelMost; ++e)
+                  if (own_count == e) own_slot[e] = i0 + from * 4 + k;
+                ++own_count;
               }
-              ++at;
+          }
+          many = __ballot_sync(0xffffffffu, own_count > kLabelMost);
+        }
+        if (found != 0)
+          found = static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(own_count)));
+        if (found != 0 && found <= kNear) {
+          int at = 0;
+#pragma unroll
+          for (int e = 0; e < kNear; ++e)
+            at += __popc(__ballot_sync(0xffffffffu, own_count > e) & ((1u << lane) - 1u));
+#pragma unroll
+          for (int e = 0; e < kLabelMost; ++e)
+            if (e < own_count) {
+              mine[at + e] = own_slot[e];
+              tokens[at + e] = lane;
             }
         }
         __syncwarp();
-        if (found > kHits) found = 0;
+        if (own_count > kLabelMost) own_count = 0;
       }
       // Few labels: the tile's columns of their hidden rows, eight a lane, asked for
       // here, while the product runs, and handed around below.  More of them: each lane
-      // keeps those of its own token and reads their rows as it comes to them; a token
-      // with more than kLabelMost is left as it is, its roundings average out.  (Read
+      // reads the rows of its own token's as it comes to them.  (Read
       // one label after another by the whole warp, a backward of 512 rows x 4096 x 512
       // took 73 us, and of 64 rows with labels among 32 tokens 252; so 50 and 46.)
       uint4 seg[kNear];
@@ -635,23 +670,27 @@ __global__ void __launch_bounds__(kThreads, 1)
       // d is written to the tile's end, zeros past the vocabulary
       const int64_t rest_cols = width - x.n * kBN;
       const int cols = kMode == kDlogits || rest_cols > kBN ? kBN : static_cast<int>(rest_cols);
-      auto columns = [&](int c, auto corrected, uint64_t own_hits) {  // 32 of them
+      auto columns = [&](int c, auto corrected) {  // 32 of them
         const int64_t c0 = x.n * kBN + c;  // column of the output tile's matrix
         // the lane's next label: its hidden row's columns and what rounding took
-        uint64_t ahead = own_hits;
+        int next[kLabelMost], ahead = own_count;
+#pragma unroll
+        for (int e = 0; e < kLabelMost; ++e) next[e] = own_slot[e];
         uint4 far[4] = {};
         float far_by = 0.0f;
         bool fetched = false;
         auto fetch = [&] {
           fetched = ahead != 0;
           if (!fetched) return;
-          const int slot = mine[__ffsll(static_cast<long long>(ahead)) - 1];
+          const int slot = next[0];
+#pragma unroll
+          for (int e = 0; e + 1 < kLabelMost; ++e) next[e] = next[e + 1];
+          --ahead;
           const uint4* h = static_cast<const uint4*>(p.packed) + slot * (p.hidden / 8) + c0 / 8;
           far_by = p.rest[slot];
 #pragma unroll
           for (int q = 0; q < 4; ++q)
             if (c0 + 8 * q < width) far[q] = h[q];
-          ahead &= ahead - 1;
         };
         if constexpr (corrected.value == kFar) {
           fetch();
@@ -792,18 +831,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       // the loop without labels stays short: of few rows, dW is bound by it
       if (kMode != kDweight || found == 0) {
 #pragma unroll 1
-        for (int c = 0; c < cols; c += 32) columns(c, std::integral_constant<int, kNone>{}, 0);
+        for (int c = 0; c < cols; c += 32) columns(c, std::integral_constant<int, kNone>{});
       } else if (found <= kNear) {
 #pragma unroll 1
-        for (int c = 0; c < cols; c += 32) columns(c, std::integral_constant<int, kClose>{}, 0);
+        for (int c = 0; c < cols; c += 32) columns(c, std::integral_constant<int, kClose>{});
       } else {
-        uint64_t own_hits = 0;
 #pragma unroll 1
-        for (int e = 0; e < found; ++e)
-          own_hits |= static_cast<uint64_t>(tokens[e] == lane ? 1 : 0) << e;
-        if (__popcll(own_hits) > kLabelMost) own_hits = 0;
-#pragma unroll 1
-        for (int c = 0; c < cols; c += 32) columns(c, std::integral_constant<int, kFar>{}, own_hits);
+        for (int c = 0; c < cols; c += 32) columns(c, std::integral_constant<int, kFar>{});
       }
       tc_fence_before();
       __syncwarp();

@@ -456,6 +456,127 @@ def test_labels_of_few_tokens(rows, tokens, hidden, dtype) -> None:
         assert torch.equal(a, b)
 
 
+# ---------------------------------------------------------------------------
+# The label's element of d
+# ---------------------------------------------------------------------------
+
+
+def _steep(rows, vocab, hidden, dtype, labels, seed=0):
+    """Inputs whose gradients are all but those of the labels: every logit but
+    token 0's is about -24, so p is 1 at token 0 and below 1e-8 elsewhere, and
+    token 0's weight row is zero.  ``labels`` are above 0."""
+    dev = torch.device("cuda", 0)
+    g = torch.Generator(device=dev).manual_seed(seed + rows + vocab)
+    h = torch.randn(rows, hidden, generator=g, device=dev)
+    w = torch.randn(vocab, hidden, generator=g, device=dev) / hidden**0.5
+    h[:, 0], w[:, 0], w[0] = 1.0, -24.0, 0.0
+    gl = torch.rand(rows, generator=g, device=dev) + 0.25
+    ge = torch.randn(rows, generator=g, device=dev) * 0.1
+    return labels.to(dev), h.to(dtype), w.to(dtype), gl, ge
+
+
+def _half_step(x, dtype):
+    """Half the distance between the two numbers of `dtype` that enclose x."""
+    info = torch.finfo(dtype)
+    e = torch.floor(torch.log2(x.abs().clamp_min(info.smallest_normal)))
+    return torch.exp2(e) * (info.eps / 2)
+
+
+def _label_exact(y, h, w, gl, ge, cap):
+    """Gradients in 64 bits, tolerances under which the label's element of d
+    carries no 16-bit rounding, and the gradients of a d that does.
+
+    Off the label an element of d is off by (u + 2 dz + 2^-20) |a| p; at the
+    label by (2 dz + 2^-20) |a| p + 2^-22 |b| (one float32 subtraction, and the
+    part rounding took held in float32); float32 sums as in ``_exact``; the
+    output by half a step.  In dW a token with more than ``cap`` labels keeps
+    its roundings."""
+    keep = y >= 0
+    hd = torch.where(keep[:, None], h.double(), 0.0)
+    wd = w.double()
+    z = hd @ wd.T
+    p = torch.exp(z - torch.logsumexp(z, 1)[:, None])
+    at = torch.where(keep, y, 0)
+    one = torch.zeros_like(z).scatter_(1, at[:, None], 1.0)
+    a, b = (gl + ge).double() * keep, gl.double() * keep
+    d = a[:, None] * p - b[:, None] * one
+    N, V, H = h.shape[0], w.shape[0], h.shape[1]
+    dz = (H / 16 + 16) * 2.0**-22 * (hd.abs() @ wd.abs().T).amax(1)
+    u = torch.finfo(h.dtype).eps / 2
+    fp16 = h.dtype == FP16
+    sub = 2.0**-25 if fp16 else 0.0
+    dsub = sub * float(torch.maximum(a.abs(), b.abs()).max()) * 2.0**-12
+    exactly = (2 * dz[:, None] + 2.0**-20) * a.abs()[:, None] * p + 2.0**-22 * b.abs()[:, None] * one
+    off = exactly + u * a.abs()[:, None] * p * (1 - one) + dsub * (1 - one)
+    many = torch.bincount(at[keep], minlength=V) > cap
+    off_w = off + u * d.abs() * one * many[None]
+    dabs = d.abs()
+    top_h, top_w = hd.abs(), wd.abs()
+    dh, dw = d @ wd, d.T @ hd
+    tol_dh = off @ top_w + (V / 16 + 80) * 2.0**-22 * (dabs @ top_w) + _half_step(dh, h.dtype)
+    tol_dw = off_w.T @ top_h + (N / 16 + 80) * 2.0**-22 * (dabs.T @ top_h) + _half_step(dw, h.dtype)
+    scale = 1.0
+    if fp16:
+        scale = 2.0 ** (12 - torch.floor(torch.log2(torch.maximum(a.abs(), b.abs()).max())))
+    lost = (d * scale).to(h.dtype).double() / scale * one - d * one
+    return (dh, dw, tol_dh, tol_dw, (dh + lost @ wd).to(h.dtype), (dw + lost.T @ hd).to(h.dtype),
+            many)
+
+
+def _labels(kind, rows, vocab):
+    g = torch.Generator().manual_seed(rows)
+    if kind == "apart":       # hardly two in 32 tokens
+        return torch.randint(1, vocab, (rows,), generator=g)
+    if kind == "neighbours":  # three labels for each of 32 tokens
+        return 352 + torch.arange(rows) % 32
+    assert kind == "flood"    # one token with most labels among 31 with one
+    y = torch.full((rows,), 352 + 5)
+    y[rows - 32 :] = 352 + torch.randperm(32, generator=g)
+    return y
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("kind,rows,vocab,hidden", [
+    ("apart", 1, 600, 72),
+    ("apart", 5, 600, 264),
+    ("apart", 100, 1200, 136),
+    ("apart", 300, 600, 64),       # a pair's tiles
+    ("neighbours", 96, 600, 520),
+    ("neighbours", 20, 600, 64),
+    ("flood", 131, 600, 264),
+    ("flood", 400, 600, 72),
+    ("flood", 40, 600, 136),
+])
+def test_label_rounding_is_given_back(kind, rows, vocab, hidden, dtype) -> None:
+    """What rounding takes from d at the label reaches dh of every row and dW of
+    every token with up to four labels, whatever labels its neighbours have."""
+    y = _labels(kind, rows, vocab)
+    if rows > 10:
+        y[3::11] = -100
+    x = _steep(rows, vocab, hidden, dtype, y)
+    dh, dw, tol_dh, tol_dw, dh_lost, dw_lost, many = _label_exact(*x, cap=4)
+    if kind == "flood":
+        assert 0 < int(many.sum()) <= 2
+    # the tolerances tell a d with its rounding from one without
+    for lost, want, tol in ((dh_lost, dh, tol_dh), (dw_lost, dw, tol_dw * (1 + many[:, None] * 1e9))):
+        # (one row's coefficient may happen to be nearly a 16-bit number)
+        assert int(((lost.double() - want).abs() > tol).sum()) > (hidden // 16 if rows > 1 else 0)
+    got = _step(*x)
+    _within("grad_hidden", got[2], dh, tol_dh)
+    _within("grad_weight", got[3], dw, tol_dw)
+
+
+def test_label_rounding_in_pieces_of_the_vocabulary() -> None:
+    y = _labels("apart", 5000, 30011)
+    x = _steep(5000, 30011, 64, BF16, y)
+    dh, dw, tol_dh, tol_dw, dh_lost, dw_lost, _ = _label_exact(*x, cap=4)
+    for lost, want, tol in ((dh_lost, dh, tol_dh), (dw_lost, dw, tol_dw)):
+        assert int(((lost.double() - want).abs() > tol).sum()) > 1000
+    got = _step(*x)
+    _within("grad_hidden", got[2], dh, tol_dh)
+    _within("grad_weight", got[3], dw, tol_dw)
+
+
 @pytest.mark.parametrize("scale,small", [(65536.0, 2.0**-8), (1e-6, 1.0)])
 def test_loss_scales_of_fp16_training(scale, small) -> None:
     """A loss scale of 65536 (on inputs small enough for the outputs' range) and
