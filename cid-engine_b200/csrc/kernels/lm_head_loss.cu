@@ -102,7 +102,7 @@ struct Params {
   const float* lse;
   const float* ca;
   const float* cb;
-  const uint32_t* top;  // bits of the largest |coefficient| (fp16), or NULL
+  const uint32_t* top;  // bits of the largest finite |coefficient| (fp16), or NULL
   float2* records;      // [tiles][rec_stride]
   float* label_logit;   // [rec_stride]
   int64_t rec_stride;
@@ -112,7 +112,7 @@ struct Params {
   uint32_t* status;
 };
 
-// Power of two that brings the largest coefficient near 2^11 (fp16 d).
+// Power of two that brings the largest finite coefficient to [2^12, 2^13) (fp16 d).
 __device__ __forceinline__ float coef_scale(const uint32_t* top) {
   if (top == nullptr) return 1.0f;
   const float m = __uint_as_float(*top);
@@ -893,7 +893,7 @@ struct PrepParams {
   float* plse;
   float* pa;
   float* pb;
-  uint32_t* top;           // fp16 backward: bits of the largest |coefficient|
+  uint32_t* top;           // fp16 backward: bits of the largest finite |coefficient|
   int* count;              // [0] kept rows, [2] K splits of dh
   int piece_slices, tile_m, workers;  // K slices of a whole piece of dh, rows of a tile, CTAs or pairs
   uint32_t* status;
@@ -950,7 +950,9 @@ __global__ void __launch_bounds__(32 * kPrepRows) head_prepare_kernel(PrepParams
           p.plse[slot] = p.lse[r];
           p.pa[slot] = gl + ge;
           p.pb[slot] = gl;
-          if (p.top) atomicMax(p.top, __float_as_uint(fmaxf(fabsf(gl + ge), fabsf(gl))));
+          // one that is not finite spoils its own row and dW, not the scale of the others
+          const float most = fmaxf(fabsf(gl + ge), fabsf(gl));
+          if (p.top && most < INFINITY) atomicMax(p.top, __float_as_uint(most));
         }
       }
       if (lane < kPrepRows) slots[lane] = mine ? slot : kIgnored;

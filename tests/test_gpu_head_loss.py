@@ -592,3 +592,22 @@ def test_coefficients_of_many_binades_in_fp16() -> None:
     y, h, w, gl, ge = _inputs(160, 3000, 64, FP16)
     s = torch.exp2(5.0 - torch.arange(160, device=h.device) % 31)
     _check(y, h, w, gl * s, ge * s)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")])
+def test_not_finite_coefficients_stay_in_their_rows(bad, dtype) -> None:
+    """An output gradient that is not finite (a loss scale too large for one row)
+    makes its own row of dh not finite and leaves the other rows the bits they have
+    beside a row without a gradient; dW takes the row in."""
+    y, h, w, gl, ge = _inputs(150, 3000, 64, dtype, "all")
+    gl, ge = gl * 1e-3, ge * 1e-3
+    gl[7] = ge[7] = 0.0
+    want = _step(y, h, w, gl, ge)
+    for through_loss in (True, False):
+        gl2, ge2 = gl.clone(), ge.clone()
+        (gl2 if through_loss else ge2)[7] = bad
+        got = _step(y, h, w, gl2, ge2)
+        others = torch.arange(150, device=h.device) != 7
+        assert torch.equal(got[2][others], want[2][others])
+        assert not bool(got[2][7].isfinite().any()) and not bool(got[3].isfinite().any())
