@@ -78,7 +78,8 @@ def lm_head_quantized_logits(hidden: Tensor, packed: Tensor, scales: Tensor) -> 
     and scaled in float32; the logits are rounded once.  Made for few rows:
     the weight is read once for every 64 of them (32 with groups of 64, 16
     with groups of 32), and beyond that the 16-bit weight is faster.  H is at most 32768.  A hidden row with
-    a NaN or infinite value has NaN logits.  Not differentiable."""
+    a NaN or infinite value has NaN logits, and so has a column with a NaN or
+    infinite scale.  Not differentiable."""
     return torch.ops.cid_engine.lm_head_quantized_logits(hidden, packed, scales)
 
 

@@ -166,6 +166,14 @@ __device__ __forceinline__ void unpack8(uint32_t w, uint32_t* out) {
   out[3] = (w >> 8) & 0x00f000f0u;
 }
 
+// A logit from the sum over its groups and the hidden row's power of two.  A group
+// with an infinite scale has codes of zero, and its part is 0 x inf; but sum c h and
+// 8 sum h are rounded apart, and infinity times what is left of them is an infinity of
+// either sign as often as NaN.  An infinite sum is therefore NaN.
+__device__ __forceinline__ float logit_of(float sum, float row_scale) {
+  return fmaf(sum, 0.0f, sum * row_scale);
+}
+
 // Running statistics of one hidden row over the columns a thread has seen.
 struct RowStats {
   float m, s;
@@ -593,7 +601,7 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
         }
         if (!ok) break;
 #pragma unroll
-        for (int j = 0; j < N; ++j) acc[j] *= sums[group_slots * N + j];
+        for (int j = 0; j < N; ++j) acc[j] = logit_of(acc[j], sums[group_slots * N + j]);
         // ---- the tile's logits: 128 weight rows x N hidden rows ----
         if (p.out != nullptr) {
           if (v < p.vocab) {
@@ -1010,7 +1018,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) int4_rows_kernel(RowsParams p
         float z = 0.0f;
 #pragma unroll
         for (int q = 0; q < kws; ++q) z += rb[(q * N + n) * tile_rows + orow];
-        z *= rscale[n];
+        z = logit_of(z, rscale[n]);
         if (!kStats) {
           if (v < p.vocab) {
             if (std::is_same<T, __nv_bfloat16>::value)

@@ -478,7 +478,7 @@ CID_API size_t cid_lm_head_quantized_workspace_bytes(int64_t rows, int64_t hidde
  * (the scales' type), 16-byte aligned (workspace too); each group's sum of
  * q * hidden is accumulated in f32 on the tcgen05 tensor cores and scaled in
  * f32; logits rows x vocab of `dtype`, rounded once.  A hidden row with a NaN or
- * infinite value has NaN logits.  Waits inside the kernel are bounded; one that
+ * infinite value has NaN logits, and so has a column with a NaN or infinite scale.  Waits inside the kernel are bounded; one that
  * runs out sets CID_STATUS_LM_HEAD_TIMEOUT. */
 CID_API int cid_lm_head_quantized_logits(cid_dtype_t dtype, const void* hidden, int64_t rows,
                         int64_t hidden_dim, const uint32_t* packed, const void* scales,

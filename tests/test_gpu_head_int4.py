@@ -461,3 +461,25 @@ def test_every_form_of_the_products(rows, vocab, hidden, group, dtype) -> None:
     tol = dz * (1 + u) + u * z.abs() + (2.0**-25 if dtype == FP16 else 0.0)
     assert bool((off <= tol).all()), f"worst {float((off / tol).max()):.3g} of the tolerance"
     _check_stats(ids, h, head, z, dz)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("rows,group", [(4, 128), (4, 64), (4, 32), (20, 128), (20, 64), (50, 128),
+                                        (50, 32)])
+def test_infinite_weights_make_their_columns_nan(rows, group, dtype) -> None:
+    """An infinite weight leaves its group an infinite scale and codes 0: 0 x inf,
+    a NaN logit in every row, and NaN statistics with the first such column."""
+    import cid_engine
+
+    w = _weight(2000, 512, dtype)
+    w[1333, 5], w[1700, 400] = float("inf"), -float("inf")
+    head = cid_engine.lm_head_quantize(w, group_size=group)
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    # values off zero on one side, so that sums of h are large beside their roundings
+    h = (torch.randn(rows, 512, generator=g, device="cuda") + 0.3).to(dtype)
+    logits = cid_engine.lm_head_quantized_logits(h, *head)
+    assert int(logits.isnan().sum()) == 2 * rows and not bool(logits.isinf().any())
+    assert bool(logits[:, [1333, 1700]].isnan().all())
+    conf, pred, cur = cid_engine.lm_head_quantized_display_statistics(
+        torch.zeros(rows, dtype=torch.long, device="cuda"), h, *head)
+    assert bool(conf.isnan().all()) and bool((pred == 1333).all()) and bool(cur.isnan().all())
