@@ -61,9 +61,10 @@ constexpr int kRowGroup = 4096;  // rows whose row blocks share weight tiles in 
 constexpr int kPrepRows = 8;   // rows a prepare block packs at a time, one a warp
 constexpr int kPrepBlocks = 8;  // prepare blocks an SM, at most
 constexpr int kMaxSplits = 64;
-// Units the split of dh aims at: with four waves of 148 SMs the last wave
-// costs little, and the partial tiles stay within 75 MB.
+// Units the split of dh may make: with four waves of 148 SMs the last wave costs
+// little, and the partial tiles stay within 155 MB (256 x 256; 78 MB of 128 x 256).
 constexpr int64_t kSplitUnits = 592;
+constexpr int kMinSlices = 8;
 
 // A CTA pair (cluster of two, tcgen05.mma.cta_group::2) computes 256 x 256
 // tiles: each CTA stages its own 128 rows of A and half of B, so operands cross
@@ -129,8 +130,8 @@ struct Grid {
 
 // K splits of dh: the number that makes the slowest worker's share of slices
 // smallest, the lowest of equals.  A unit costs its slices and about kUnitCost
-// slices of epilogue.  The count is fixed by a whole piece's slices, so that every
-// piece adds to the same partial tiles.  The lanes of a warp weigh 32 numbers each
+// slices of epilogue, and a part has kMinSlices at least.  The count is fixed by a
+// whole piece's slices, so that every piece adds to the same partial tiles.  The lanes of a warp weigh 32 numbers each
 // round (one thread alone took 7 us over them).
 __device__ inline int dh_splits(int64_t tiles, int kslices, int workers, int lane) {
   constexpr int kUnitCost = 8;
@@ -138,7 +139,7 @@ __device__ inline int dh_splits(int64_t tiles, int kslices, int workers, int lan
   if (tiles > kSplitUnits / 2) return 1;
   const int t = static_cast<int>(tiles);
   for (int s = lane + 1; s <= kMaxSplits; s += 32) {
-    if (s > 1 && (t * s > kSplitUnits || s * 8 > kslices)) continue;
+    if (s > 1 && (t * s > kSplitUnits || s * kMinSlices > kslices)) continue;
     const int waves = (t * s + workers - 1) / workers;
     const int64_t cost = static_cast<int64_t>(waves) * ((kslices + s - 1) / s + kUnitCost);
     const unsigned key =
@@ -1135,6 +1136,15 @@ int64_t piece_cols(int64_t rows, int64_t vocab) {
   return c < all ? c : all;
 }
 
+// Partial tiles of dh: what dh_splits makes of up to `tiles` tiles (fewer rows may be
+// kept) and a piece's K slices, at most.
+int64_t partial_tiles(int64_t tiles, int64_t slices) {
+  int64_t splits = slices / kMinSlices;
+  splits = splits < 1 ? 1 : (splits > kMaxSplits ? kMaxSplits : splits);
+  const int64_t most = tiles * splits < kSplitUnits ? tiles * splits : kSplitUnits;
+  return tiles > most ? tiles : most;
+}
+
 // Byte offsets of the workspace's parts.
 struct Layout {
   size_t count, slot_of, plabel, plse, pa, pb, label_logit, rest, packed, records, d, partial, bytes;
@@ -1164,7 +1174,7 @@ Layout layout(int64_t rows, int64_t hidden, int64_t vocab, bool backward) {
     l.rest = take(padded * 4);
     l.d = take(padded * piece_cols(rows, vocab) * 2);
     const int64_t tiles = padded / tile_m * ((hidden + kBN - 1) / kBN);
-    l.partial_rows = (tiles > kSplitUnits ? tiles : kSplitUnits) * tile_m;
+    l.partial_rows = partial_tiles(tiles, piece_cols(rows, vocab) / kBK) * tile_m;
     l.partial = take(l.partial_rows * kBN * 4);
   }
   l.bytes = at;

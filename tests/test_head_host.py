@@ -312,3 +312,22 @@ def test_loss_under_vmap_keeps_shapes() -> None:
     assert loss.shape == lse.shape == (3, 5) and loss.requires_grad
     (gh,) = torch.autograd.grad(loss.sum(), h)
     assert gh.shape == h.shape
+
+
+def test_loss_workspace_follows_the_call(lib: ctypes.CDLL) -> None:
+    """The backward's workspace holds a piece of the logits' gradient and the parts
+    of dh that the extents can make, not the most that any can."""
+    i64 = ctypes.c_int64
+
+    def need(rows, dim, vocab):
+        return lib.cid_lm_head_cross_entropy_workspace_bytes(i64(rows), i64(dim), i64(vocab),
+                                                             ctypes.c_int(1))
+
+    assert need(64, 64, 4096) < 4 << 20
+    assert need(1, 8, 7) < 1 << 20
+    assert need(129, 64, 4096) < 8 << 20
+    # parts of dh: 592 tiles of 256 x 256 where as many can be made, all of dh's where
+    # it has more, beside a piece of up to 256 MB
+    for rows, dim, vocab in ((1024, 2048, 32000), (4096, 4096, 128256), (8192, 8192, 50257)):
+        tiles = max(592, rows // 256 * (dim // 256))
+        assert tiles * 2**18 < need(rows, dim, vocab) < tiles * 2**18 + (257 << 20) + rows * (2 * dim + 64)
