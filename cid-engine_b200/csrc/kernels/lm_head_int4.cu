@@ -237,10 +237,10 @@ static_assert(128 * kCtrlRegs + 256 * kReadRegs + 256 * kUnpackRegs <=
 // one row block the warpgroups take turns at the stages; the accumulators form a
 // ring.
 //
-// Bound by issue slots: the unpacking warps' at few rows (16 x 128256 x 4096: 77
-// us, 272 MB from memory, 53 % of the slots), the read-back's at 64 rows, where
-// each group's 64 sums a weight row are scaled and added (147 us with the
-// statistics).  Three A buffers a warpgroup (104 us at 16 rows), four unpacking
+// No unit is full at 16 rows x 128256 x 4096 (77 us, 272 MB from memory: 43 % of DRAM,
+// 10 % of the tensor pipe, 53 % of the issue slots with the polling among them): the
+// roles wait for one another.  At 64 rows (147 us with the statistics) the
+// read-back of each group's 64 sums a weight row sets the pace.  Three A buffers a warpgroup (104 us at 16 rows), four unpacking
 // warpgroups (87) and MMAs issued by the unpacking warps (201) were slower.
 template <typename T, int N, int S, int R, bool kResident>
 __global__ void __launch_bounds__(int4_threads(R), 1)
@@ -341,7 +341,8 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
     if (warp == 0) {
       if (lane == 0) {
         // ---------------- TMA producer ----------------
-        // codes are in flight before the kernel that prepares the hidden rows ends
+        // codes need no wait for the kernel that prepares the hidden rows: it was
+        // launched in stream order, so what it follows, the codes' writer too, is done
         int s = 0;
         uint32_t ph = 0, issued = 0, issue_par = 0;
         bool ok = true, prepared = false;
@@ -1091,7 +1092,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1) int4_rows_kernel(RowsParams p
 
 // One block turns one hidden row into the fp16 row of the products, its group
 // sums (8 sum h) and its scale 2^-e; rows past the last get zero sums.  Bound by
-// latency: the product kernel's first codes are on their way meanwhile.
+// latency, which the product kernel waits out: it starts when every block of this one
+// has exited.
 constexpr int kPrepThreads = 256;
 
 template <typename T>
@@ -1375,8 +1377,8 @@ int launch_int4(const CUtensorMap& map_w, const CUtensorMap& map_h, const Int4Pa
     }();
     if (!sized) return CID_ERR_LAUNCH;
   }
-  // a programmatic dependent of the kernel that prepares the hidden rows: the
-  // codes start streaming while that one runs
+  // a programmatic dependent of the kernel that prepares the hidden rows: its set-up
+  // and first codes overlap that one's completion, not its run
   return launch_pdl(int4_head_kernel<T, N, S, R, kResident>, dim3(static_cast<unsigned>(p.parts)),
                     dim3(int4_threads(R)), smem, stream, map_w, map_h, p);
 }

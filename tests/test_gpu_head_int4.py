@@ -160,9 +160,9 @@ SIZES = [
     (20, 40000, 4096, 128), # hidden rows too many for shared memory
     (64, 80000, 1536, 128), # the same, several tiles of 256 weight rows a CTA
     (16, 3000, 8192, 32),
-    (9, 9999, 4096, 128),   # 16-row fragments, 16 warps along K
-    (8, 30011, 1152, 64),   # tiles of 64 weight rows
-    (2, 70001, 96, 32),     # one block of columns, tiles of 128 weight rows
+    (9, 9999, 4096, 128),   # 16 rows a pass, 15 weight rows in the last tile
+    (8, 30011, 1152, 64),   # the small-row kernel, nine blocks of columns
+    (2, 70001, 96, 32),     # one block of columns; groups of 32 take the other kernel
 ]
 
 
