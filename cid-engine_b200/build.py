@@ -17,6 +17,7 @@ from __future__ import annotations
 import argparse
 import concurrent.futures as cf
 import os
+import re
 import subprocess
 import sys
 import sysconfig
@@ -57,11 +58,42 @@ def _stale(target: Path, deps: list[Path]) -> bool:
     return any(d.stat().st_mtime > t for d in deps)
 
 
-def _run(cmd: list[str]) -> None:
+def _run(cmd: list[str]) -> str:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         sys.stderr.write(" ".join(map(str, cmd)) + "\n" + res.stdout + res.stderr)
         raise SystemExit(f"build failed: {cmd[0]}")
+    return res.stdout + res.stderr
+
+
+# Registers a thread that ptxas must give a kernel at launch, by source: those of
+# the 4-bit head's two-row-block form (its mangled name ends in R = 2, not
+# resident) are divided anew between its warps, in shares of exactly this sum.
+_LAUNCH_REGISTERS = {"lm_head_int4.cu": (r"int4_head_kernelI\S*Li2ELb0E", 96, 12)}
+
+
+def _compile_kernels(source: Path, obj: Path) -> None:
+    out = _run([str(NVCC), *NVCC_FLAGS, "-Xptxas", "-v", "-c", str(source), "-o", str(obj)])
+    if source.name not in _LAUNCH_REGISTERS:
+        return
+    name, registers, kernels = _LAUNCH_REGISTERS[source.name]
+    used = launch_registers(out, name)
+    if used != [registers] * kernels:
+        obj.unlink(missing_ok=True)
+        raise SystemExit(f"build failed: {source.name} needs {kernels} kernels {name} of "
+                         f"{registers} registers, ptxas made {used}")
+
+
+def launch_registers(ptxas_log: str, name: str) -> list[int]:
+    """Registers of the kernels whose mangled name matches `name`, from ptxas -v."""
+    found, own = [], False
+    for line in ptxas_log.splitlines():
+        if entry := re.search(r"Compiling entry function '(\S+)'", line):
+            own = re.search(name, entry[1]) is not None
+        elif own and (used := re.search(r"Used (\d+) registers", line)):
+            found.append(int(used[1]))
+            own = False
+    return found
 
 
 def _headers() -> list[Path]:
@@ -98,7 +130,7 @@ def build(force: bool = False, jobs: int | None = None) -> Path:
     ]
 
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
-        futs = [ex.submit(_run, [str(NVCC), *NVCC_FLAGS, "-c", str(s), "-o", str(o)]) for s, o in todo]
+        futs = [ex.submit(_compile_kernels, s, o) for s, o in todo]
         futs += [ex.submit(_run, [CXX, *cxx_flags, "-c", str(s), "-o", str(o)]) for s, o in todo_cpp]
         for f in futs:
             f.result()

@@ -215,10 +215,12 @@ __device__ __forceinline__ cid_shard_record_t record_of(const RowStats& a, float
 // the accumulators back, then two that unpack.
 __host__ __device__ constexpr int int4_threads(int r) { return 128 * (3 + r); }
 
-// With two row blocks (640 threads, 96 registers each at launch) the read-back
-// warps hold 64 accumulators apiece: registers move to them from the others.  The
-// shares add up to no more than the launch's, and on each SM sub-partition (a warp
-// of control, two of read-back, two of unpacking) to 32 x 472 of 16384.
+// With two row blocks (640 threads, 96 registers each at launch) the read-back warps
+// hold 64 accumulators apiece: registers move to them from the others.  The build
+// checks that every such kernel has the 96: a launch with fewer would wait for the
+// rest for good.  The shares add up to no more than the launch's, and on each SM
+// sub-partition (a warp of control, two of read-back, two of unpacking) to 32 x 472 of
+// 16384.
 constexpr int kLaunchRegs = 96;
 constexpr int kCtrlRegs = 40;
 constexpr int kReadRegs = 144;
@@ -239,9 +241,10 @@ static_assert(128 * kCtrlRegs + 256 * kReadRegs + 256 * kUnpackRegs <=
 //
 // No unit is full at 16 rows x 128256 x 4096 (77 us, 272 MB from memory: 43 % of DRAM,
 // 10 % of the tensor pipe, 53 % of the issue slots with the polling among them): the
-// roles wait for one another.  At 64 rows (147 us with the statistics) the
-// read-back of each group's 64 sums a weight row sets the pace.  Three A buffers a warpgroup (104 us at 16 rows), four unpacking
-// warpgroups (87) and MMAs issued by the unpacking warps (201) were slower.
+// roles wait for one another.  At 64 rows (147 us with the statistics) the read-back
+// of each group's 64 sums a weight row sets the pace.  Three A buffers a warpgroup
+// (104 us at 16 rows), four unpacking warpgroups (87) and MMAs issued by the unpacking
+// warps (201) were slower.
 template <typename T, int N, int S, int R, bool kResident>
 __global__ void __launch_bounds__(int4_threads(R), 1)
     int4_head_kernel(const __grid_constant__ CUtensorMap map_w,
@@ -1369,14 +1372,6 @@ int launch_int4(const CUtensorMap& map_w, const CUtensorMap& map_h, const Int4Pa
                                              cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              static_cast<int>(smem));
   if (e != cudaSuccess) return record_cuda_error(e);
-  if (R == 2) {  // the split of registers is sized for this launch
-    static const bool sized = [] {
-      cudaFuncAttributes fa;
-      return cudaFuncGetAttributes(&fa, int4_head_kernel<T, N, S, R, kResident>) == cudaSuccess &&
-             fa.numRegs == kLaunchRegs;
-    }();
-    if (!sized) return CID_ERR_LAUNCH;
-  }
   // a programmatic dependent of the kernel that prepares the hidden rows: its set-up
   // and first codes overlap that one's completion, not its run
   return launch_pdl(int4_head_kernel<T, N, S, R, kResident>, dim3(static_cast<unsigned>(p.parts)),

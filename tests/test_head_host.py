@@ -4,6 +4,7 @@ shapes on the meta device, autograd, and the C ABI's checks (no GPU)."""
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 from pathlib import Path
 
 import pytest
@@ -331,3 +332,36 @@ def test_loss_workspace_follows_the_call(lib: ctypes.CDLL) -> None:
     for rows, dim, vocab in ((1024, 2048, 32000), (4096, 4096, 128256), (8192, 8192, 50257)):
         tiles = max(592, rows // 256 * (dim // 256))
         assert tiles * 2**18 < need(rows, dim, vocab) < tiles * 2**18 + (257 << 20) + rows * (2 * dim + 64)
+
+
+def test_build_checks_the_registers_that_kernels_divide(tmp_path, monkeypatch) -> None:
+    """A kernel that divides its launch's registers anew between its warps does not
+    leave the build with another number of them."""
+    spec = importlib.util.spec_from_file_location("cid_build_check",
+                                                  ROOT / "cid-engine_b200" / "build.py")
+    build = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(build)
+    name, registers, kernels = build._LAUNCH_REGISTERS["lm_head_int4.cu"]
+
+    def log(used):
+        lines = []
+        for i in range(kernels):
+            lines += [f"ptxas info : Compiling entry function '_Z{i}int4_head_kernelI6__halfLi16ELi1ELi2ELb0EE' "
+                      "for 'sm_100a'", "ptxas info : Function properties", "    0 bytes stack frame",
+                      f"ptxas info : Used {used if i == 3 else registers} registers, used 1 barriers",
+                      f"ptxas info : Compiling entry function '_Z{i}int4_head_kernelI6__halfLi16ELi1ELi1ELb1EE'",
+                      "ptxas info : Used 128 registers"]
+        return "\n".join(lines)
+
+    source, obj = tmp_path / "lm_head_int4.cu", tmp_path / "x.o"
+    for used in (registers, registers - 8):
+        obj.write_text("")
+        monkeypatch.setattr(build, "_run", lambda cmd: log(used))
+        assert build.launch_registers(log(used), name).count(registers) == kernels - (used != registers)
+        if used == registers:
+            build._compile_kernels(source, obj)
+            assert obj.exists()
+        else:
+            with pytest.raises(SystemExit, match="96 registers"):
+                build._compile_kernels(source, obj)
+            assert not obj.exists()
