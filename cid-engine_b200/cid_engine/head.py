@@ -41,7 +41,9 @@ def lm_head_cross_entropy(
     weight the positions (``(loss * scale).sum()``), average them, or add a
     penalty of the log-sum-exp.  Inputs with a forward-mode tangent (dual
     tensors, ``torch.func.jvp``) are refused.  The backward computes the logits
-    again, a piece of the vocabulary at a time."""
+    again, a piece of the vocabulary at a time, and holds their gradient in the
+    inputs' dtype; in float16 it is scaled by one power of two, so that elements
+    below 2^-37 of the largest position weight are lost."""
     return torch.ops.cid_engine.lm_head_cross_entropy(labels, hidden, weight, ignore_index)
 
 

@@ -1,7 +1,8 @@
 // Softmax cross entropy of an LM head, without keeping the logits, and its
 // gradient.  For rows h_r (16-bit, H wide), weight rows w_v and labels y_r:
 //
-//   z_rv = h_r . w_v            (f32 accumulation on the tensor cores)
+//   z_rv = h_r . w_v            (f32 accumulation on the tensor cores, which truncates:
+//                                loss and lse are 1e-6 to 2e-6 off)
 //   lse_r = log sum_v exp z_rv,  loss_r = lse_r - z_{r, y_r}
 //   d_rv = a_r exp(z_rv - lse_r) - b_r [v = y_r],   a = g_loss + g_lse, b = g_loss
 //   dh = d W,   dW = d^T h
@@ -19,11 +20,12 @@
 // again, 4 gradients) instead of 6 with kept logits, which would be n V floats.
 //
 // Roundings to 16 bits: d, because the tensor cores take 16-bit operands (the
-// same step as a 16-bit gradient of the logits; at most half a step of each
-// element, and the elements' errors are independent; dh and dW get what the
-// label's element lost back in f32), and the outputs.  fp16 d
-// is scaled by a power of two from the largest coefficient, so that neither a
-// loss scale nor a division by the number of rows leaves fp16's range.
+// same step as a 16-bit gradient of the logits, at most half a step of each
+// element; dh and dW get what the label's element lost back in f32, the largest
+// of its row unless another token is favoured), and the outputs.  fp16 d is
+// scaled by a power of two from the largest coefficient, so that neither a loss
+// scale nor a division by the number of rows leaves fp16's range; elements below
+// 2^-37 of that coefficient are lost.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -341,8 +343,9 @@ __device__ __forceinline__ void box_out(const CUtensorMap* map, int32_t x, int32
 // Bound by the tensor cores and, at one to four waves of tiles, by the last wave:
 // 2867 kept rows x 128256 x 4096 run loss, d, dh and dW at 1541, 1547, 1447
 // and 1575 TFLOP/s one at a time (1270 to 1300 together, under the power cap);
-// 512 x 32000 x 2048 take 54.6, 58, 52 and 63.9 us (tensor pipe 63, 59, 66, 53 %).  Up to 128 rows it is
-// bound by memory: 24 x 128256 x 4096, 1.05 GB a launch, 176, 188, 154 and 244 us.
+// 512 x 32000 x 2048 take 54.6, 58, 52 and 63.9 us (tensor pipe 63, 59, 66, 53 %; of
+// dW's few slices a tile the epilogue takes longer than the products).  Up to 128 rows
+// it is bound by memory: 24 x 128256 x 4096, 1.05 GB a launch, 176, 188, 154 and 244 us.
 
 template <typename T, Mode kMode, bool kPair>
 __global__ void __launch_bounds__(kThreads, 1)

@@ -434,7 +434,9 @@ CID_API int cid_lm_head_cross_entropy(cid_dtype_t dtype, const void* hidden, int
  * outputs (rows f32 each; NULL means zero).  log_sum_exp: the forward's
  * output.  grad_hidden rows x hidden_dim and grad_weight vocab x hidden_dim of
  * `dtype`, 16-byte aligned, overwritten; either may be NULL when it is not
- * wanted.  The logits are computed again a piece of the vocabulary at a time.
+ * wanted.  The logits are computed again a piece of the vocabulary at a time, and
+ * their gradient is held in `dtype` (F16: scaled by one power of two a call,
+ * elements below 2^-37 of the largest finite grad_loss are lost).
  * Rows with ignore_index: zero grad_hidden, no part in grad_weight.  Rows with
  * another label outside [0, vocab): NaN grad_hidden, no part in grad_weight. */
 CID_API int cid_lm_head_cross_entropy_backward(cid_dtype_t dtype, const void* hidden,
