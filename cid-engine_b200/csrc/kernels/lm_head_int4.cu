@@ -479,8 +479,6 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         w[j] = *reinterpret_cast<const uint4*>(row + ((j ^ ((r >> 1) & 3)) << 4));
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[s]);
       const uint32_t ab = static_cast<uint32_t>(wg) * 2 + (n & 1u);
       if (!warp_wait(&a_empty[ab], (n >> 1 & 1u) ^ 1u)) break;
       tc_fence_after();
@@ -498,10 +496,20 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
         unpack8(w[2 * j + 1].w, a + 28);
         tmem_store32(dst + 32 * j, a);
       }
+      // The stage is handed back only now that every lane's codes have come in and been
+      // used, and its reads are fenced against the refill's writes.  An arrival right
+      // after the loads' issue overtook them: they wait their turn behind the read-back's
+      // scales, up to 2048 lines for its four warps, about a microsecond, and a refill
+      // takes less.  (147 us for 16 rows of groups of 32 then, 149 now; 137 and 141 for 32
+      // rows of groups of 64, 77.1 and 77.8 for 16 of 128.)
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tmem_wait_store();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&a_full[ab]);
+      if (lane == 0) {
+        mbar_arrive(&empty[s]);
+        mbar_arrive(&a_full[ab]);
+      }
       next_stage();
       if (R == 1) next_stage();
     }

@@ -483,3 +483,30 @@ def test_infinite_weights_make_their_columns_nan(rows, group, dtype) -> None:
     conf, pred, cur = cid_engine.lm_head_quantized_display_statistics(
         torch.zeros(rows, dtype=torch.long, device="cuda"), h, *head)
     assert bool(conf.isnan().all()) and bool((pred == 1333).all()) and bool(cur.isnan().all())
+
+
+@pytest.mark.parametrize("rows,vocab,hidden,group,dtype", [
+    (15, 37889, 2048, 32, FP16),
+    (1, 34741, 4096, 32, FP16),
+    (93, 18944, 3584, 32, BF16),
+    (135, 37888, 3456, 32, BF16),
+    (65, 2653, 2048, 64, BF16),
+    (64, 18945, 1024, 128, BF16),
+])
+def test_stages_are_refilled_after_they_are_read(rows, vocab, hidden, group, dtype) -> None:
+    """Where the read-back of many scales holds the loads of an SM up, a stage of
+    codes that is handed back before its loads have come in holds other columns'
+    codes for some weight rows.  Several operands at other addresses, each called
+    again and again: every call gives the oracle's logits and the first call's bits."""
+    import cid_engine
+
+    keep = []
+    for seed in range(4):
+        _, h, head, z, dz = _inputs(rows, vocab, hidden, group, dtype, seed)
+        keep.append((h, head))  # the next operands stand elsewhere
+        u = torch.finfo(dtype).eps / 2
+        tol = dz * (1 + u) + u * z.abs() + (2.0**-25 if dtype == FP16 else 0.0)
+        first = cid_engine.lm_head_quantized_logits(h, *head)
+        assert bool(((first.double() - z).abs() <= tol).all())
+        for _ in range(8):
+            assert torch.equal(cid_engine.lm_head_quantized_logits(h, *head), first)

@@ -489,7 +489,8 @@ def _label_exact(y, h, w, gl, ge, cap):
     Off the label an element of d is off by (u + 2 dz + 2^-20) |a| p; at the
     label by (2 dz + 2^-20) |a| p + 2^-22 |b| (one float32 subtraction, and the
     part rounding took held in float32); float32 sums as in ``_exact``; the
-    output by half a step.  In dW a token with more than ``cap`` labels keeps
+    output by half a step at most of the number that it rounds, |x| + the rest of
+    the tolerance (which may stand in the binade above x).  In dW a token with more than ``cap`` labels keeps
     its roundings."""
     keep = y >= 0
     hd = torch.where(keep[:, None], h.double(), 0.0)
@@ -513,8 +514,10 @@ def _label_exact(y, h, w, gl, ge, cap):
     dabs = d.abs()
     top_h, top_w = hd.abs(), wd.abs()
     dh, dw = d @ wd, d.T @ hd
-    tol_dh = off @ top_w + (V / 16 + 80) * 2.0**-22 * (dabs @ top_w) + _half_step(dh, h.dtype)
-    tol_dw = off_w.T @ top_h + (N / 16 + 80) * 2.0**-22 * (dabs.T @ top_h) + _half_step(dw, h.dtype)
+    tol_dh = off @ top_w + (V / 16 + 80) * 2.0**-22 * (dabs @ top_w)
+    tol_dw = off_w.T @ top_h + (N / 16 + 80) * 2.0**-22 * (dabs.T @ top_h)
+    tol_dh = tol_dh + _half_step(dh.abs() + tol_dh, h.dtype)
+    tol_dw = tol_dw + _half_step(dw.abs() + tol_dw, h.dtype)
     scale = 1.0
     if fp16:
         scale = 2.0 ** (12 - torch.floor(torch.log2(torch.maximum(a.abs(), b.abs()).max())))
