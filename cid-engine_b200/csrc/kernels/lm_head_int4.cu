@@ -236,8 +236,8 @@ static_assert(128 * kCtrlRegs + 256 * kReadRegs + 256 * kUnpackRegs <=
 //
 // Chunks are numbered q along the CTA's work: for every stage the tile's R row
 // blocks.  Unpacking warpgroup q & 1 fills A buffer (q & 1, (q >> 1) & 1), so with
-// one row block the warpgroups take turns at the stages; the accumulators form a
-// ring.
+// one row block the warpgroups take turns at the stages, whose number is even then;
+// the accumulators form a ring.
 //
 // No unit is full at 16 rows x 128256 x 4096 (77 us, 272 MB from memory: 43 % of DRAM,
 // 10 % of the tensor pipe, 53 % of the issue slots with the polling among them): the
@@ -1344,6 +1344,12 @@ Int4Plan int4_plan(int64_t rows, int64_t vocab, int64_t dim, int group) {
       --pl.stages;
     if (pl.stages > 1 || pl.n == 16) break;
   }
+  // With one row block the warpgroups take turns at the stages.  An even number gives
+  // each warpgroup its own: with an odd one it would wait for phases of a stage of
+  // which it has not seen the one before, and a parity cannot tell a phase from the
+  // next but one.  (At nine stages the warpgroup that is nine chunks ahead of a late load,
+  // as far as the buffers let it, took the stage for filled.)
+  if (pl.resident) pl.stages -= pl.stages % 2;
   pl.tile_rows = pl.r * kTileV;
   pl.tiles = (vocab + pl.tile_rows - 1) / pl.tile_rows;
   pl.parts = pl.tiles < sms ? pl.tiles : sms;

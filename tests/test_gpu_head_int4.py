@@ -510,3 +510,27 @@ def test_stages_are_refilled_after_they_are_read(rows, vocab, hidden, group, dty
         assert bool(((first.double() - z).abs() <= tol).all())
         for _ in range(8):
             assert torch.equal(cid_engine.lm_head_quantized_logits(h, *head), first)
+
+
+@pytest.mark.parametrize("rows,vocab,hidden,group", [
+    (64, 40001, 1024, 128), (40, 40001, 1024, 128), (32, 30011, 2048, 64), (12, 20011, 4352, 64),
+    (16, 20011, 4224, 32)])
+def test_late_loads_of_codes(rows, vocab, hidden, group) -> None:
+    """Sizes at which shared memory has room for nine stages of codes, while copies on
+    another stream delay some of their loads: the first call's bits every time."""
+    import cid_engine
+
+    _, h, head, z, dz = _inputs(rows, vocab, hidden, group, BF16)
+    first = cid_engine.lm_head_quantized_logits(h, *head)
+    u = torch.finfo(BF16).eps / 2
+    assert bool(((first.double() - z).abs() <= dz * (1 + u) + u * z.abs()).all())
+    big = torch.zeros(1 << 28, dtype=torch.uint8, device="cuda")
+    other = torch.empty_like(big)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(40):
+            other.copy_(big)
+    got = [cid_engine.lm_head_quantized_logits(h, *head) for _ in range(24)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, first) for g in got)
