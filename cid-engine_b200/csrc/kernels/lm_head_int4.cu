@@ -20,7 +20,7 @@
 // keeps all its bits unless it is below 2^-24 of its row's largest, and then
 // loses less than 2^-35 of that largest, far under the f32 sum's own rounding.
 // 8 sum h of every group is kept beside and subtracted from the group's sum:
-// sum c h - 8 sum h = sum q h.
+// sum c h - 8 sum h = sum q h, with roundings of 8 sum |h| in f32.
 //
 // Two product kernels; the weight's bytes bound both up to some 64 rows (128256 x
 // 4096: 270 MB, 42 us at the copy peak).
@@ -324,7 +324,8 @@ __global__ void __launch_bounds__(int4_threads(R), 1)
   const int chunks = p.chunks;
 
   // A bounded wait of a whole warp; false when it ran out or another role did.
-  // One lane polls: thirty-two take turns at the barrier and slow every role.
+  // One lane polls: thirty-two take turns at the barrier and slow every role.  The
+  // others' accesses are issued after the shuffle that waits for it.
   auto warp_wait = [&](uint64_t* bar, uint32_t parity) {
     bool got = true;
     if (lane == 0) {
