@@ -383,6 +383,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
+  // A pair takes its tensor memory as a pair: both CTAs have to be running before either
+  // asks.  Beside another stream's kernels one can start well before the other.
+  __syncthreads();
+  if (kPair) cluster_sync();
   if (warp == 1) {
     if (kPair) {
       asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -399,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   __syncthreads();
-  if (kPair) cluster_sync();  // the peer's barriers are initialised
+  if (kPair) cluster_sync();  // the peer has its tensor memory
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   // every kernel of a call is a programmatic dependent of the one before: set-up
@@ -874,6 +878,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                    "r"(kTmemCols)
                    : "memory");
   }
+  // A pair gives its tensor memory back as a pair: neither CTA leaves its SM to another
+  // kernel's while the other's deallocation is under way.
+  if (kPair) cluster_sync();
 }
 
 // ---------------------------------------------------------------------------

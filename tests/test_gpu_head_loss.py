@@ -614,3 +614,28 @@ def test_not_finite_coefficients_stay_in_their_rows(bad, dtype) -> None:
         others = torch.arange(150, device=h.device) != 7
         assert torch.equal(got[2][others], want[2][others])
         assert not bool(got[2][7].isfinite().any()) and not bool(got[3].isfinite().any())
+
+
+@pytest.mark.parametrize("one_,other", [((239, 29487, 16), (2, 160, 80)),
+                                        ((219, 13765, 16), (321, 246, 968)),
+                                        ((300, 4000, 64), (100, 3000, 64))])
+def test_short_kernels_of_two_streams(one_, other) -> None:
+    """Calls of more than 128 rows (CTA pairs) on one stream and of any number on
+    another, again and again: their kernels follow one another on the same SMs, and the
+    CTAs of a pair start and end apart."""
+    x, x2 = _inputs(*one_, BF16, "all"), _inputs(*other, FP16, seed=4)
+    want, want2 = _step(*x), _step(*x2)
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(300):
+        a, b = [], []
+        for _ in range(4):
+            with torch.cuda.stream(s1):
+                a.append(_step(*x))
+            with torch.cuda.stream(s2):
+                b.append(_step(*x2))
+        torch.cuda.synchronize()
+        for got, ref in ((a, want), (b, want2)):
+            for one in got:
+                for p, q in zip(one, ref):
+                    assert torch.equal(p, q)
