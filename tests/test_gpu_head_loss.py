@@ -639,3 +639,17 @@ def test_short_kernels_of_two_streams(one_, other) -> None:
             for one in got:
                 for p, q in zip(one, ref):
                     assert torch.equal(p, q)
+
+
+@pytest.mark.filterwarnings("ignore:There is a performance drop")
+def test_vmap_is_the_loop() -> None:
+    import cid_engine
+
+    y, h, w, gl, _ = _inputs(60, 400, 64, BF16)
+    loss, lse, dh, dw = _step(y, h, w, gl, torch.zeros_like(gl))
+    hr, wr = h.clone().requires_grad_(), w.clone().requires_grad_()
+    l2, e2 = torch.vmap(lambda a, b: cid_engine.lm_head_cross_entropy(a, b, wr))(
+        y.view(3, 20), hr.view(3, 20, 64))
+    assert torch.equal(l2.detach().view(60), loss) and torch.equal(e2.detach().view(60), lse)
+    dh2, _ = torch.autograd.grad(l2, (hr, wr), grad_outputs=gl.view(3, 20))
+    assert torch.equal(dh2, dh)
